@@ -406,6 +406,134 @@ int volta_mi355x_resident_device_ptr(void* ctx, uint64_t id, size_t off_bytes, s
 int volta_mi355x_stream(void* ctx, void** out);
 int volta_mi355x_synchronize(void* ctx);
 
+/* ---- Fixed-point model operators ------------------------------------------
+ * The forward pass of a model over its committed i16 tensors, in exact integer
+ * arithmetic.  rs(a, s) is a / 2^s rounded to the nearest integer, halves up
+ * (a for s = 0); sat clamps to 16 bits.  Offsets and strides are in elements
+ * unless said otherwise, and rows may start at any element.  An id of 0 leaves
+ * an optional tensor out.  All are counted as Gemm calls in RawStats. */
+
+/* Weights w[k x n] (rows `stride` apart; `transposed`: n rows of k) packed for
+ * volta_mi355x_fixed_linear_device; k <= 65,535.  The packed form takes
+ * volta_mi355x_fixed_weights_bytes bytes (0: invalid sizes) at a byte offset
+ * that is a multiple of 16, and holds the values themselves: w may be freed. */
+size_t volta_mi355x_fixed_weights_bytes(size_t k, size_t n);
+int volta_mi355x_fixed_weights_device(void* ctx, uint64_t w_id, size_t w_off, size_t k, size_t n, size_t stride,
+                                      int transposed, uint64_t out_id, size_t out_off_bytes);
+
+/* acc = sum_k x[m][k] w[k][n] + (bias[n] << bias_shift);
+ * raw != 0:  out (i64) = acc, with `shift`, `table` and `residual` unused;
+ * otherwise  h = sat(rs(acc, shift)); h = table[h + 2^15] with a table (65,536
+ * i16); out (i16) = sat(h + residual[m][n]) with a residual.
+ * bias_shift <= 46, shift <= 62.  The output may be the residual itself (same
+ * place and stride); it may not overlap an input otherwise. */
+typedef struct VoltaFixedLinear {
+    uint64_t x_id;
+    size_t x_off, x_stride;
+    uint64_t weights_id;
+    size_t weights_off_bytes;
+    uint64_t bias_id;
+    size_t bias_off;
+    uint64_t table_id;
+    size_t table_off;
+    uint64_t residual_id;
+    size_t residual_off, residual_stride;
+    uint64_t out_id;
+    size_t out_off, out_stride;
+    size_t rows, k, n;
+    uint32_t bias_shift, shift;
+    uint32_t raw, reserved;
+} VoltaFixedLinear;
+int volta_mi355x_fixed_linear_device(void* ctx, const VoltaFixedLinear* args);
+
+/* A cache of keys and values: `slots` sequences of up to `capacity` tokens
+ * (at most 65,536), kv_heads heads of `dim` (at most 128) i16, in a resident
+ * buffer of volta_mi355x_fixed_cache_bytes bytes (0: invalid sizes) at a byte
+ * offset that is a multiple of 16. */
+typedef struct VoltaFixedCache {
+    uint64_t id;
+    size_t off_bytes;
+    size_t slots, kv_heads, dim, capacity;
+} VoltaFixedCache;
+/* Rows row .. row + count of packed tensors: the last `count` of the `length`
+ * tokens of the sequence in `slot`. */
+typedef struct VoltaFixedSequence {
+    uint64_t slot, row, count, length;
+} VoltaFixedSequence;
+size_t volta_mi355x_fixed_cache_bytes(size_t slots, size_t kv_heads, size_t dim, size_t capacity);
+/* Writes k and v rows (kv_heads x dim each, rows k_stride and v_stride apart)
+ * to places length - count .. length of their slots.  A slot may occur once. */
+int volta_mi355x_fixed_kv_append_device(void* ctx, const VoltaFixedCache* cache, uint64_t k_id, size_t k_off,
+                                        size_t k_stride, uint64_t v_id, size_t v_off, size_t v_stride,
+                                        const VoltaFixedSequence* sequences, size_t count);
+
+/* For every row and head (heads a multiple of kv_heads; head h reads key head
+ * h / (heads / kv_heads)) over the keys j it may see (causal: places up to its
+ * own; otherwise all of `length`):
+ *   z_j = (q . k_j) >> shift, e_j = table[min(max z - z_j, entries - 1)],
+ *   out = sum e_j v_j / sum e_j, rounded to nearest, halves up;
+ * zeros where it sees none or all e are 0.  table: 1 .. 8,192 u16, at most
+ * 2^14 each (larger entries count as 2^14); 8 <= shift <= 24.  Rows are heads x
+ * dim; the output may not overlap the queries, and rows of two sequences may
+ * not overlap.  Only without `causal` may count exceed length. */
+typedef struct VoltaFixedAttention {
+    uint64_t q_id;
+    size_t q_off, q_stride;
+    uint64_t table_id;
+    size_t table_off, entries;
+    uint64_t out_id;
+    size_t out_off, out_stride;
+    size_t heads;
+    uint32_t shift, causal;
+} VoltaFixedAttention;
+int volta_mi355x_fixed_attention_device(void* ctx, const VoltaFixedCache* cache, const VoltaFixedAttention* args,
+                                        const VoltaFixedSequence* sequences, size_t count);
+
+/* h = sat(x + residual); n = cols, S = sum h (0 for rms), V = n sum h^2 - S^2,
+ * R = floor(sqrt(V + eps)):
+ *   out = sat((n h - S) gain / (R 2^shift), rounded to nearest, halves up, + bias),
+ *   sum = h, where asked for.
+ * cols <= 65,536, shift <= 15, 1 <= eps <= 2^40.  The sum may be x or the
+ * residual itself (same place and stride); no other output may overlap a tensor. */
+typedef struct VoltaFixedNorm {
+    uint64_t x_id;
+    size_t x_off, x_stride;
+    uint64_t residual_id;
+    size_t residual_off, residual_stride;
+    uint64_t sum_id;
+    size_t sum_off, sum_stride;
+    uint64_t gain_id;
+    size_t gain_off;
+    uint64_t bias_id;
+    size_t bias_off;
+    uint64_t out_id;
+    size_t out_off, out_stride;
+    size_t rows, cols;
+    uint64_t eps;
+    uint32_t shift, rms;
+} VoltaFixedNorm;
+int volta_mi355x_fixed_norm_device(void* ctx, const VoltaFixedNorm* args);
+
+/* out[i] = sat(rs(table[tokens[i]] scale, shift) + position_table[positions[i]]);
+ * tokens and positions are i32, and one outside its table adds nothing.
+ * shift <= 46. */
+typedef struct VoltaFixedEmbed {
+    uint64_t tokens_id;
+    size_t tokens_off;
+    uint64_t table_id;
+    size_t table_off, table_stride, vocab;
+    uint64_t positions_id;
+    size_t positions_off;
+    uint64_t position_table_id;
+    size_t position_table_off, position_stride, position_rows;
+    uint64_t out_id;
+    size_t out_off, out_stride;
+    size_t rows, cols;
+    int32_t scale;
+    uint32_t shift;
+} VoltaFixedEmbed;
+int volta_mi355x_fixed_embed_device(void* ctx, const VoltaFixedEmbed* args);
+
 /* Measurement probes: a 16-byte streaming copy (achievable HBM bandwidth)
  * and the reference's Fp2-multiply stream (rounds == 0) / chain kernels
  * (cuda/p7_goldilocks_roofline.cu:74-89).  Not timed or accounted in stats. */

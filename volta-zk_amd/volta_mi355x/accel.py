@@ -83,6 +83,55 @@ class Fp2C(ctypes.Structure):
     _fields_ = [("c0", ctypes.c_uint64), ("c1", ctypes.c_uint64)]
 
 
+class _FixedLinear(ctypes.Structure):
+    _fields_ = [("x_id", ctypes.c_uint64), ("x_off", ctypes.c_size_t), ("x_stride", ctypes.c_size_t),
+                ("weights_id", ctypes.c_uint64), ("weights_off_bytes", ctypes.c_size_t),
+                ("bias_id", ctypes.c_uint64), ("bias_off", ctypes.c_size_t),
+                ("table_id", ctypes.c_uint64), ("table_off", ctypes.c_size_t),
+                ("residual_id", ctypes.c_uint64), ("residual_off", ctypes.c_size_t),
+                ("residual_stride", ctypes.c_size_t),
+                ("out_id", ctypes.c_uint64), ("out_off", ctypes.c_size_t), ("out_stride", ctypes.c_size_t),
+                ("rows", ctypes.c_size_t), ("k", ctypes.c_size_t), ("n", ctypes.c_size_t),
+                ("bias_shift", ctypes.c_uint32), ("shift", ctypes.c_uint32),
+                ("raw", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
+class _FixedCache(ctypes.Structure):
+    _fields_ = [("id", ctypes.c_uint64), ("off_bytes", ctypes.c_size_t), ("slots", ctypes.c_size_t),
+                ("kv_heads", ctypes.c_size_t), ("dim", ctypes.c_size_t), ("capacity", ctypes.c_size_t)]
+
+
+class _FixedAttention(ctypes.Structure):
+    _fields_ = [("q_id", ctypes.c_uint64), ("q_off", ctypes.c_size_t), ("q_stride", ctypes.c_size_t),
+                ("table_id", ctypes.c_uint64), ("table_off", ctypes.c_size_t), ("entries", ctypes.c_size_t),
+                ("out_id", ctypes.c_uint64), ("out_off", ctypes.c_size_t), ("out_stride", ctypes.c_size_t),
+                ("heads", ctypes.c_size_t), ("shift", ctypes.c_uint32), ("causal", ctypes.c_uint32)]
+
+
+class _FixedNorm(ctypes.Structure):
+    _fields_ = [("x_id", ctypes.c_uint64), ("x_off", ctypes.c_size_t), ("x_stride", ctypes.c_size_t),
+                ("residual_id", ctypes.c_uint64), ("residual_off", ctypes.c_size_t),
+                ("residual_stride", ctypes.c_size_t),
+                ("sum_id", ctypes.c_uint64), ("sum_off", ctypes.c_size_t), ("sum_stride", ctypes.c_size_t),
+                ("gain_id", ctypes.c_uint64), ("gain_off", ctypes.c_size_t),
+                ("bias_id", ctypes.c_uint64), ("bias_off", ctypes.c_size_t),
+                ("out_id", ctypes.c_uint64), ("out_off", ctypes.c_size_t), ("out_stride", ctypes.c_size_t),
+                ("rows", ctypes.c_size_t), ("cols", ctypes.c_size_t), ("eps", ctypes.c_uint64),
+                ("shift", ctypes.c_uint32), ("rms", ctypes.c_uint32)]
+
+
+class _FixedEmbed(ctypes.Structure):
+    _fields_ = [("tokens_id", ctypes.c_uint64), ("tokens_off", ctypes.c_size_t),
+                ("table_id", ctypes.c_uint64), ("table_off", ctypes.c_size_t), ("table_stride", ctypes.c_size_t),
+                ("vocab", ctypes.c_size_t),
+                ("positions_id", ctypes.c_uint64), ("positions_off", ctypes.c_size_t),
+                ("position_table_id", ctypes.c_uint64), ("position_table_off", ctypes.c_size_t),
+                ("position_stride", ctypes.c_size_t), ("position_rows", ctypes.c_size_t),
+                ("out_id", ctypes.c_uint64), ("out_off", ctypes.c_size_t), ("out_stride", ctypes.c_size_t),
+                ("rows", ctypes.c_size_t), ("cols", ctypes.c_size_t),
+                ("scale", ctypes.c_int32), ("shift", ctypes.c_uint32)]
+
+
 def abi_symbols(header: pathlib.Path = HEADER) -> list[str]:
     """The reference-ABI symbol names declared in include/volta_cuda_abi.h."""
     text = header.read_text()
@@ -155,6 +204,16 @@ _SIGS = {
     "volta_mi355x_resident_device_ptr": (_int, [_vp, _u64, _sz, _sz, ctypes.POINTER(_vp)]),
     "volta_mi355x_stream": (_int, [_vp, ctypes.POINTER(_vp)]),
     "volta_mi355x_synchronize": (_int, [_vp]),
+    "volta_mi355x_fixed_weights_bytes": (_sz, [_sz, _sz]),
+    "volta_mi355x_fixed_weights_device": (_int, [_vp, _u64, _sz, _sz, _sz, _sz, _int, _u64, _sz]),
+    "volta_mi355x_fixed_linear_device": (_int, [_vp, ctypes.POINTER(_FixedLinear)]),
+    "volta_mi355x_fixed_cache_bytes": (_sz, [_sz, _sz, _sz, _sz]),
+    "volta_mi355x_fixed_kv_append_device": (_int, [_vp, ctypes.POINTER(_FixedCache), _u64, _sz, _sz, _u64, _sz, _sz,
+                                                   _vp, _sz]),
+    "volta_mi355x_fixed_attention_device": (_int, [_vp, ctypes.POINTER(_FixedCache), ctypes.POINTER(_FixedAttention),
+                                                   _vp, _sz]),
+    "volta_mi355x_fixed_norm_device": (_int, [_vp, ctypes.POINTER(_FixedNorm)]),
+    "volta_mi355x_fixed_embed_device": (_int, [_vp, ctypes.POINTER(_FixedEmbed)]),
     "volta_mi355x_probe_copy_device": (_int, [_vp, _u64, _u64, _sz]),
     "volta_mi355x_probe_expand_device": (_int, [_vp, _u64, _u64, _sz]),
     "volta_mi355x_probe_fp2_device": (_int, [_vp, _u64, _u64, _u64, _sz, _int]),
@@ -209,6 +268,27 @@ class DeviceMerkleTree:
     storage holds (2 leaves - 1) 32-byte hashes, leaves first, root last."""
     storage: DeviceBuffer
     leaves: int
+
+
+@dataclass
+class FixedWeights:
+    """A k x n weight matrix packed for fixed_linear_device (it holds the values; the source may be freed)."""
+    storage: DeviceBuffer
+    k: int
+    n: int
+
+
+@dataclass
+class FixedKvCache:
+    """Keys and values of `slots` sequences of up to `capacity` tokens, for fixed_attention_device."""
+    storage: DeviceBuffer
+    slots: int
+    kv_heads: int
+    dim: int
+    capacity: int
+
+    def _args(self) -> _FixedCache:
+        return _FixedCache(self.storage.id, 0, self.slots, self.kv_heads, self.dim, self.capacity)
 
 
 def _as_fp2(a) -> np.ndarray:
@@ -723,6 +803,211 @@ class Backend:
             raise InvalidInput("invalid resident Fp2 Mobius inverse")
         self._region(values, offset, n)
         self._check(self.lib.volta_cuda_fp2_mobius_inverse_inplace_device(self.raw, values.id, offset, n))
+
+    # ---- fixed-point model operators (MI355X extensions; no reference counterpart) ---------
+    def _typed(self, buf: DeviceBuffer, dtype, what: str) -> DeviceBuffer:
+        self._own(buf)
+        if buf.dtype != np.dtype(dtype):
+            raise InvalidInput(f"{what} must hold {np.dtype(dtype).name}, not {buf.dtype}")
+        return buf
+
+    def _matrix(self, buf: DeviceBuffer, offset: int, stride: int, rows: int, cols: int, dtype, what: str) -> int:
+        """Checks a strided matrix inside a buffer and gives the buffer's id."""
+        self._typed(buf, dtype, what)
+        if stride < cols:
+            raise InvalidInput(f"{what}: row stride {stride} is shorter than a row of {cols}")
+        self._region(buf, offset, (rows - 1) * stride + cols)
+        return buf.id
+
+    def fixed_weights_device(self, weights: DeviceBuffer, k: int, n: int, *, offset: int = 0, stride: int | None = None,
+                             transposed: bool = False) -> FixedWeights:
+        """Packs k x n i16 weights (transposed: n rows of k) for fixed_linear_device."""
+        size = self.lib.volta_mi355x_fixed_weights_bytes(max(k, 0), max(n, 0))
+        if size == 0:
+            raise InvalidInput("invalid fixed-point weight geometry")
+        rows, cols = (n, k) if transposed else (k, n)
+        stride = cols if stride is None else stride
+        wid = self._matrix(weights, offset, stride, rows, cols, np.int16, "weights")
+        out = self.alloc_device(size, np.uint8)
+        self._call_or_free(out, self.lib.volta_mi355x_fixed_weights_device, wid, offset, k, n, stride,
+                           1 if transposed else 0, out.id, 0)
+        return FixedWeights(out, k, n)
+
+    def free_fixed_weights(self, weights: FixedWeights) -> None:
+        self.free_device(weights.storage)
+
+    def fixed_linear_device(self, x: DeviceBuffer, rows: int, weights: FixedWeights, shift: int = 0, *,
+                            x_offset: int = 0, x_stride: int | None = None, bias: DeviceBuffer | None = None,
+                            bias_offset: int = 0, bias_shift: int = 0, table: DeviceBuffer | None = None,
+                            table_offset: int = 0, residual: DeviceBuffer | None = None, residual_offset: int = 0,
+                            residual_stride: int | None = None, raw: bool = False, out: DeviceBuffer | None = None,
+                            out_offset: int = 0, out_stride: int | None = None) -> DeviceBuffer:
+        """x w with its epilogue: h = sat(rs(x w + (bias << bias_shift), shift)), then the
+        65,536-entry table at h + 2^15, then sat(h + residual).  raw: the i64 sums
+        x w + (bias << bias_shift) alone (shift is not used)."""
+        k, n = weights.k, weights.n
+        if rows <= 0 or not 0 <= bias_shift <= 46 or (not raw and not 0 <= shift <= 62):
+            raise InvalidInput("invalid fixed-point linear geometry")
+        if raw and (table is not None or residual is not None):
+            raise InvalidInput("raw fixed-point sums take neither a table nor a residual")
+        a = _FixedLinear(x_off=x_offset, x_stride=k if x_stride is None else x_stride, bias_off=bias_offset,
+                         table_off=table_offset, residual_off=residual_offset,
+                         residual_stride=n if residual_stride is None else residual_stride, out_off=out_offset,
+                         out_stride=n if out_stride is None else out_stride, rows=rows, k=k, n=n,
+                         bias_shift=bias_shift, shift=0 if raw else shift, raw=1 if raw else 0)
+        a.x_id = self._matrix(x, x_offset, a.x_stride, rows, k, np.int16, "x")
+        self._own(weights.storage)
+        a.weights_id = weights.storage.id
+        if bias is not None:
+            a.bias_id = self._matrix(bias, bias_offset, n, 1, n, np.int16, "bias")
+        if table is not None:
+            a.table_id = self._matrix(table, table_offset, 65536, 1, 65536, np.int16, "table")
+        if residual is not None:
+            a.residual_id = self._matrix(residual, residual_offset, a.residual_stride, rows, n, np.int16, "residual")
+        return self._into(out, a, rows, n, np.int64 if raw else np.int16,
+                          lambda: self.lib.volta_mi355x_fixed_linear_device(self.raw, ctypes.byref(a)))
+
+    def _into(self, out: DeviceBuffer | None, a, rows: int, cols: int, dtype, call) -> DeviceBuffer:
+        """Runs `call` with a's output set to `out`, or to a new buffer that a failure frees."""
+        made = out is None
+        if made:
+            if a.out_off:
+                raise InvalidInput("an output offset needs an output buffer")
+            if a.out_stride < cols:
+                raise InvalidInput(f"output: row stride {a.out_stride} is shorter than a row of {cols}")
+            out = self.alloc_device((rows - 1) * a.out_stride + cols, dtype)
+            a.out_id = out.id
+        else:
+            a.out_id = self._matrix(out, a.out_off, a.out_stride, rows, cols, dtype, "output")
+        if call() != 0:
+            msg = self.last_error()
+            if made:
+                self.free_device(out)
+            raise GpuError(msg or "fixed-point operator failed")
+        return out
+
+    def fixed_kv_cache(self, slots: int, kv_heads: int, dim: int, capacity: int) -> FixedKvCache:
+        """An empty cache for `slots` sequences: its tokens are those that appends have written."""
+        size = 0
+        if min(slots, kv_heads, dim, capacity) > 0:
+            size = self.lib.volta_mi355x_fixed_cache_bytes(slots, kv_heads, dim, capacity)
+        if size == 0:
+            raise InvalidInput("invalid fixed-point cache geometry")
+        return FixedKvCache(self.alloc_device(size, np.uint8), slots, kv_heads, dim, capacity)
+
+    def free_fixed_kv_cache(self, cache: FixedKvCache) -> None:
+        self.free_device(cache.storage)
+
+    @staticmethod
+    def _sequences(sequences) -> tuple[np.ndarray, int]:
+        """(n x 4 array, rows): slot, first row, rows, tokens in all, of each sequence."""
+        s = np.ascontiguousarray(sequences, dtype=np.int64).reshape(-1, 4)
+        if s.size and s.min() < 0:
+            raise InvalidInput("sequences hold whole numbers from 0 on")
+        return s, int((s[:, 1] + s[:, 2])[s[:, 2] > 0].max(initial=0))
+
+    def fixed_kv_append_device(self, cache: FixedKvCache, k: DeviceBuffer, v: DeviceBuffer, sequences, *,
+                               k_offset: int = 0, k_stride: int | None = None, v_offset: int = 0,
+                               v_stride: int | None = None) -> None:
+        """Writes new tokens' keys and values (rows of kv_heads x dim) to the cache.  sequences: rows of
+        (slot, first row, new tokens, tokens in all); the new ones are the last."""
+        s, rows = self._sequences(sequences)
+        cols = cache.kv_heads * cache.dim
+        k_stride, v_stride = (cols if x is None else x for x in (k_stride, v_stride))
+        self._own(cache.storage)
+        if rows:
+            self._matrix(k, k_offset, k_stride, rows, cols, np.int16, "keys")
+            self._matrix(v, v_offset, v_stride, rows, cols, np.int16, "values")
+        c = cache._args()
+        self._check(self.lib.volta_mi355x_fixed_kv_append_device(self.raw, ctypes.byref(c), k.id, k_offset, k_stride,
+                                                                 v.id, v_offset, v_stride, s.ctypes.data, len(s)))
+
+    def fixed_attention_device(self, q: DeviceBuffer, cache: FixedKvCache, sequences, heads: int, table: DeviceBuffer,
+                               shift: int, *, causal: bool = True, q_offset: int = 0, q_stride: int | None = None,
+                               table_offset: int = 0, entries: int | None = None, out: DeviceBuffer | None = None,
+                               out_offset: int = 0, out_stride: int | None = None) -> DeviceBuffer:
+        """Attention of packed rows (heads x dim) over the cache: z = (q . k) >> shift, e =
+        table[min(max z - z, entries - 1)], out = sum e v / sum e to the nearest integer.  sequences as for
+        fixed_kv_append_device; causal rows see the tokens up to their own, others all of their sequence."""
+        s, rows = self._sequences(sequences)
+        cols = heads * cache.dim
+        entries = table.len - table_offset if entries is None else entries
+        if heads <= 0 or heads % cache.kv_heads:
+            raise InvalidInput("attention heads are not a multiple of the cache's")
+        if not 8 <= shift <= 24 or not 0 < entries <= 8192:
+            raise InvalidInput("invalid fixed-point attention shift or table")
+        if rows == 0 and out is None:
+            raise InvalidInput("attention without rows needs an output buffer")
+        a = _FixedAttention(q_off=q_offset, q_stride=cols if q_stride is None else q_stride, table_off=table_offset,
+                            entries=entries, out_off=out_offset, out_stride=cols if out_stride is None else out_stride,
+                            heads=heads, shift=shift, causal=1 if causal else 0)
+        self._own(cache.storage)
+        a.table_id = self._matrix(table, table_offset, entries, 1, entries, table.dtype, "table")
+        if table.dtype.itemsize != 2 or table.dtype.kind not in "iu":
+            raise InvalidInput("the exponential table must hold 16-bit integers")
+        if rows:
+            a.q_id = self._matrix(q, q_offset, a.q_stride, rows, cols, np.int16, "queries")
+        c = cache._args()
+        call = lambda: self.lib.volta_mi355x_fixed_attention_device(  # noqa: E731
+            self.raw, ctypes.byref(c), ctypes.byref(a), s.ctypes.data, len(s))
+        if rows == 0:
+            self._check(call())
+            return out
+        return self._into(out, a, rows, cols, np.int16, call)
+
+    def fixed_norm_device(self, x: DeviceBuffer, rows: int, cols: int, gain: DeviceBuffer, shift: int, eps: int, *,
+                          bias: DeviceBuffer | None = None, rms: bool = False, x_offset: int = 0,
+                          x_stride: int | None = None, residual: DeviceBuffer | None = None, residual_offset: int = 0,
+                          residual_stride: int | None = None, sum_out: DeviceBuffer | None = None, sum_offset: int = 0,
+                          sum_stride: int | None = None, gain_offset: int = 0, bias_offset: int = 0,
+                          out: DeviceBuffer | None = None, out_offset: int = 0,
+                          out_stride: int | None = None) -> DeviceBuffer:
+        """The norm of h = sat(x + residual) along rows; sum_out keeps h.  With S = sum h (0 for rms) and
+        R = floor(sqrt(cols sum h^2 - S^2 + eps)): sat((cols h - S) gain / (R 2^shift) to the nearest integer + bias)."""
+        if rows <= 0 or not 0 < cols <= 65536 or not 0 <= shift <= 15 or not 0 < eps <= 1 << 40:
+            raise InvalidInput("invalid fixed-point norm geometry")
+        strides = [cols if st is None else st for st in (x_stride, residual_stride, sum_stride, out_stride)]
+        a = _FixedNorm(x_off=x_offset, x_stride=strides[0], residual_off=residual_offset, residual_stride=strides[1],
+                       sum_off=sum_offset, sum_stride=strides[2], gain_off=gain_offset, bias_off=bias_offset,
+                       out_off=out_offset, out_stride=strides[3], rows=rows, cols=cols, eps=eps, shift=shift,
+                       rms=1 if rms else 0)
+        a.x_id = self._matrix(x, x_offset, a.x_stride, rows, cols, np.int16, "x")
+        a.gain_id = self._matrix(gain, gain_offset, cols, 1, cols, np.int16, "gain")
+        if bias is not None:
+            a.bias_id = self._matrix(bias, bias_offset, cols, 1, cols, np.int16, "bias")
+        if residual is not None:
+            a.residual_id = self._matrix(residual, residual_offset, a.residual_stride, rows, cols, np.int16, "residual")
+        if sum_out is not None:
+            a.sum_id = self._matrix(sum_out, sum_offset, a.sum_stride, rows, cols, np.int16, "sum")
+        return self._into(out, a, rows, cols, np.int16,
+                          lambda: self.lib.volta_mi355x_fixed_norm_device(self.raw, ctypes.byref(a)))
+
+    def fixed_embed_device(self, tokens: DeviceBuffer, rows: int, table: DeviceBuffer, vocab: int, cols: int, *,
+                           scale: int = 1, shift: int = 0, tokens_offset: int = 0, table_offset: int = 0,
+                           table_stride: int | None = None, positions: DeviceBuffer | None = None,
+                           positions_offset: int = 0, position_table: DeviceBuffer | None = None,
+                           position_rows: int = 0, position_offset: int = 0, position_stride: int | None = None,
+                           out: DeviceBuffer | None = None, out_offset: int = 0,
+                           out_stride: int | None = None) -> DeviceBuffer:
+        """sat(rs(table[token] scale, shift) + position_table[position]) for i32 tokens (and positions); one
+        outside its table adds nothing."""
+        if rows <= 0 or cols <= 0 or vocab <= 0 or not 0 <= shift <= 46 or not -(1 << 31) <= scale < 1 << 31:
+            raise InvalidInput("invalid fixed-point embedding geometry")
+        if (positions is None) != (position_table is None) or (positions is not None and position_rows <= 0):
+            raise InvalidInput("positions and their table come together")
+        strides = [cols if st is None else st for st in (table_stride, position_stride, out_stride)]
+        a = _FixedEmbed(tokens_off=tokens_offset, table_off=table_offset, table_stride=strides[0], vocab=vocab,
+                        positions_off=positions_offset, position_table_off=position_offset, position_stride=strides[1],
+                        position_rows=position_rows, out_off=out_offset, out_stride=strides[2], rows=rows, cols=cols,
+                        scale=scale, shift=shift)
+        a.tokens_id = self._matrix(tokens, tokens_offset, rows, 1, rows, np.int32, "tokens")
+        a.table_id = self._matrix(table, table_offset, a.table_stride, vocab, cols, np.int16, "table")
+        if positions is not None:
+            a.positions_id = self._matrix(positions, positions_offset, rows, 1, rows, np.int32, "positions")
+            a.position_table_id = self._matrix(position_table, position_offset, a.position_stride, position_rows, cols,
+                                               np.int16, "position table")
+        return self._into(out, a, rows, cols, np.int16,
+                          lambda: self.lib.volta_mi355x_fixed_embed_device(self.raw, ctypes.byref(a)))
 
     def _call_or_free(self, out: DeviceBuffer, fn, *args) -> None:
         rc = fn(self.raw, *args)
