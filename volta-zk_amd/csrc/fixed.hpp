@@ -84,6 +84,21 @@ __device__ inline void load16(const int16_t* p, int at, int len, v4i* lo, v4i* h
     *hi = u.v[1];
 }
 
+// Sixteen bytes a lane from base + off (off a lane's own, base the wave's) to
+// LDS at `to` (the wave's) + 16 lane, without registers between.  The compiler
+// does not see the copy: lds_copies_done() waits for a wave's own ones, and a
+// barrier after it covers the workgroup's.  (Through the builtin it would wait
+// for all of them before every read of LDS, the buffers in use among them.)
+__device__ inline void copy_to_lds(const void* base, uint32_t off, void* to) {
+    const uint32_t at = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)to));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+__device__ inline void lds_copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 __device__ inline v4i mfma(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
 __device__ inline int64_t join(int hh, int mid, int ll) {
