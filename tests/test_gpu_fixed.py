@@ -149,6 +149,20 @@ def test_linear_longest_sums_of_equal_values(backend, rows, a, b_):
     assert (got == k * a * b_).all()
 
 
+@pytest.mark.parametrize("rows", [3, 70, 200])
+@pytest.mark.parametrize("top", [32639, 32640, 32767])
+@pytest.mark.parametrize("cols", [[0], [37], [149], [16, 17, 140]])
+def test_linear_few_large_weights(backend, rows, top, cols):
+    """Columns whose weights need the offset of their low byte beside columns that do not."""
+    g = gen(top + rows)
+    x, w = full(g, (rows, 130)), normal(g, (130, 150), 2000)
+    for c in cols:
+        w[g.integers(0, 130), c] = top
+    kw = dict(shift=13, bias=full(g, 150), bias_shift=11)
+    assert np.array_equal(run_linear(backend, x, w, raw=True), ref.linear(x, w, raw=True))
+    assert np.array_equal(run_linear(backend, x, w, **kw), ref.linear(x, w, **kw))
+
+
 def test_linear_transposed_weights_and_stride(backend):
     g = gen(3)
     x, w = full(g, (9, 70)), full(g, (70, 41))

@@ -6,10 +6,12 @@
 // joined: split axes and atomic additions give the same bits every time.
 //
 // 16-bit products on the matrix cores.  A 16-bit x is 256 h + l + 128 with
-// h = x >> 8 and l = (x & 255) - 128, both signed bytes, so with X = x - 128
-// and W = w - 128 a product of 16-bit vectors is four products of 8-bit ones:
+// h = x >> 8 and l = (x & 255) - 128, both signed bytes.  A w of at most 32,639
+// is 256 h + l with signed bytes itself (l the low byte's own sign, h the rest);
+// larger ones need the 128 as well.  So with X = x - 128 and W = w - o, o = 0 or
+// 128, a product of 16-bit vectors is four products of 8-bit ones:
 //   sum X W = 2^16 sum xh wh + 2^8 (sum xh wl + sum xl wh) + sum xl wl,
-//   sum x w = sum X W + 128 sum_k W + 128 sum_k x.
+//   sum x w = sum X W + 128 sum_k W + o sum_k x.
 // The two middle products share an accumulator: three i32 sums per result,
 // which hold rows of 2^16 - 1 elements (2 * 2^14 a place in the middle one).
 // Padding places hold x = 0 and w = 0, which the same identity covers.
@@ -25,6 +27,7 @@
 namespace vmx {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 typedef short v2s __attribute__((ext_vector_type(2)));
 
 namespace fx {
@@ -86,7 +89,7 @@ __device__ inline void load16(const int16_t* p, int at, int len, v4i* lo, v4i* h
 
 // Sixteen bytes a lane from base + off (off a lane's own, base the wave's) to
 // LDS at `to` (the wave's) + 16 lane, without registers between.  The compiler
-// does not see the copy: lds_copies_done() waits for a wave's own ones, and a
+// does not see the copy: lds_copies_done waits for a wave's own ones, and a
 // barrier after it covers the workgroup's.  (Through the builtin it would wait
 // for all of them before every read of LDS, the buffers in use among them.)
 __device__ inline void copy_to_lds(const void* base, uint32_t off, void* to) {
@@ -97,9 +100,26 @@ __device__ inline void copy_to_lds(const void* base, uint32_t off, void* to) {
                  : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(base)
                  : "memory", "m0");
 }
-__device__ inline void lds_copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits until at most `Left` of the wave's copies are under way.
+template <int Left>
+__device__ inline void lds_copies_done() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(Left) : "memory");
+}
 
+// Both shapes take 16 places of one row (column) per lane, in the same order on
+// both sides; results: row 4 (lane >> 4) + r, column lane & 15 of 16 x 16, and
+// row 8 (r >> 2) + 4 (lane >> 5) + (r & 3), column lane & 31 of 32 x 32.
 __device__ inline v4i mfma(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+__device__ inline v16i mfma32(v4i a, v4i b, v16i c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+}
+
+// A 16-bit w, less its offset, as its two signed bytes (high in bits 15..8 of the result).
+__device__ inline int halves(int w) {
+    const int l = static_cast<int8_t>(w);
+    return ((w - l) & 0xff00) | (l & 0xff);
+}
+constexpr int HALVES_MAX = 32639;  // the largest w that needs no offset
 
 __device__ inline int64_t join(int hh, int mid, int ll) {
     return (static_cast<int64_t>(hh) << 16) + (static_cast<int64_t>(mid) << 8) + ll;
@@ -126,12 +146,12 @@ __device__ inline double floor_div(double a, double b, double inv) {
 // ---- matrix product --------------------------------------------------------------
 // Packed weights: for each block of 16 columns, each step of 64 rows of w, the
 // high and the low plane in the order a wave's lanes read them (lane l: column
-// l & 15, rows 16 (l >> 4) .. + 15), 1 KiB each; then 128 sum_k (w - 128) of
-// every column, i64.
+// l & 15, rows 16 (l >> 4) .. + 15), 1 KiB each; then 128 sum_k W of every
+// column, i64; then o of every block, i32.
 constexpr size_t FX_K_MAX = 65535;
 inline size_t fx_blocks(size_t n) { return (n + 15) / 16; }
 inline size_t fx_steps(size_t k) { return (k + 63) / 64; }
-inline size_t fx_weight_bytes(size_t k, size_t n) { return fx_blocks(n) * (fx_steps(k) * 2048 + 128); }
+inline size_t fx_weight_bytes(size_t k, size_t n) { return fx_blocks(n) * (fx_steps(k) * 2048 + 128 + 4); }
 
 struct FxLinear {
     const int16_t* x;

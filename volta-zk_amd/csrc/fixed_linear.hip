@@ -1,6 +1,8 @@
 // fixed_linear.hip -- out = epilogue(x w): 16-bit integer matrix product on the
 // i8 matrix cores (fixed.hpp has the identity) with bias, rounding shift,
 // activation table and residual applied to the sums in registers.
+#include <algorithm>
+
 #include "fixed.hpp"
 
 namespace vmx {
@@ -9,7 +11,8 @@ namespace {
 using namespace fx;
 
 // ---- packing -------------------------------------------------------------------------
-// One workgroup per 16 columns; its waves take the steps of 64 rows in turn.
+// One workgroup per 16 columns: once for their largest value, then its waves
+// take the steps of 64 rows in turn.
 __global__ __launch_bounds__(256) void fx_pack_weights_kernel(const int16_t* w, int k, int n, size_t stride,
                                                               bool transposed, unsigned char* out, size_t blocks) {
     __shared__ int part[4][64];
@@ -17,26 +20,32 @@ __global__ __launch_bounds__(256) void fx_pack_weights_kernel(const int16_t* w, 
     const size_t block = blockIdx.x;
     const int col = static_cast<int>(block * 16) + (lane & 15);
     const int steps = (k + 63) / 64;
-    v4i* dst = reinterpret_cast<v4i*>(out + block * steps * 2048) + lane;
+    auto at = [&](int row) -> int {
+        return col < n && row < k ? (transposed ? w[col * stride + row] : w[row * stride + col]) : 0;
+    };
+    int most = 0;
+    for (int row = threadIdx.x >> 4; row < k; row += 16) most = max(most, at(row));
+    part[wave][lane] = most;
+    __syncthreads();
+    for (int i = 0; i < 256; ++i) most = max(most, part[i >> 6][i & 63]);
+    const int off = most > HALVES_MAX ? 128 : 0;
+    __syncthreads();
+    unsigned char* dst = out + block * steps * 2048 + lane * 16;
     int sum = 0;
     for (int s = wave; s < steps; s += 4) {
-        const int at = s * 64 + 16 * (lane >> 4);
         union {
-            v4i v[2];
-            int16_t e[16];
-        } u;
-        u.v[0] = v4i{0, 0, 0, 0};
-        u.v[1] = v4i{0, 0, 0, 0};
-        if (col < n) {
+            v4i v;
+            uint8_t b[16];
+        } h, l;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (at + i < k) u.e[i] = transposed ? w[col * stride + at + i] : w[(at + i) * stride + col];
+        for (int i = 0; i < 16; ++i) {
+            const int v = at(s * 64 + 16 * (lane >> 4) + i) - off, p = halves(v);
+            sum += v;
+            h.b[i] = static_cast<uint8_t>(p >> 8);
+            l.b[i] = static_cast<uint8_t>(p);
         }
-        sum = sum8(u.v[1], sum8(u.v[0], sum));
-        v4i h, l;
-        split16(u.v[0], u.v[1], &h, &l);
-        dst[s * 128] = h;
-        dst[s * 128 + 64] = l;
+        *reinterpret_cast<v4i*>(dst + s * 2048) = h.v;
+        *reinterpret_cast<v4i*>(dst + s * 2048 + 1024) = l.v;
     }
     part[wave][lane] = sum;
     __syncthreads();
@@ -44,8 +53,9 @@ __global__ __launch_bounds__(256) void fx_pack_weights_kernel(const int16_t* w, 
         int64_t total = 0;
         for (int g = 0; g < 4; ++g)
             for (int v = 0; v < 4; ++v) total += part[v][g * 16 + lane];
-        int64_t* offs = reinterpret_cast<int64_t*>(out + blocks * steps * 2048);
-        offs[block * 16 + lane] = 128 * (total - int64_t{128} * 64 * steps);
+        int64_t* sums = reinterpret_cast<int64_t*>(out + blocks * steps * 2048);
+        sums[block * 16 + lane] = 128 * total;
+        if (threadIdx.x == 0) reinterpret_cast<int*>(sums + blocks * 16)[block] = off;
     }
 }
 
@@ -63,87 +73,72 @@ __device__ inline void finish(const FxLinear& a, size_t row, int col, int64_t su
 }
 
 // ---- few rows ------------------------------------------------------------------------
-// A workgroup computes MB * 16 rows of 16 columns; its waves take the steps of
-// 64 along k in turn, each streaming its part of the packed weights once, and
-// add their i64 sums in LDS.
-template <int MB>
+// A workgroup computes 16 rows of 16 columns; its waves take the steps of 64
+// along k in turn, each streaming its part of the packed weights once, and add
+// their i64 sums in LDS.
 __global__ __launch_bounds__(1024) void fx_linear_rows_kernel(FxLinear a) {
-    __shared__ unsigned long long total[MB * 256];
-    __shared__ int x_sum[MB * 16];
+    __shared__ unsigned long long total[256];
+    __shared__ int x_sum[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int steps = (a.k + 63) / 64, col0 = blockIdx.x * 16;
-    const size_t row0 = static_cast<size_t>(blockIdx.y) * (MB * 16);
-    for (int i = threadIdx.x; i < MB * 256; i += blockDim.x) total[i] = 0;
-    for (int i = threadIdx.x; i < MB * 16; i += blockDim.x) x_sum[i] = 0;
+    const size_t row0 = static_cast<size_t>(blockIdx.y) * 16, row = row0 + (lane & 15);
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) total[i] = 0;
+    if (threadIdx.x < 16) x_sum[threadIdx.x] = 0;
     __syncthreads();
     const v4i* w = reinterpret_cast<const v4i*>(a.weights + static_cast<size_t>(blockIdx.x) * steps * 2048) + lane;
-    v4i hh[MB] = {}, mid[MB] = {}, ll[MB] = {};
-    int sums[MB] = {};
+    v4i hh = {}, mid = {}, ll = {};
+    int sum = 0;
     for (int s = wave; s < steps; s += waves) {
         const v4i wh = w[s * 128], wl = w[s * 128 + 64];
-#pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            const size_t row = row0 + b * 16 + (lane & 15);
-            v4i x0 = {}, x1 = {}, xh, xl;
-            if (row < a.rows) load16(a.x + row * a.x_stride, s * 64 + 16 * (lane >> 4), a.k, &x0, &x1);
-            sums[b] = sum8(x1, sum8(x0, sums[b]));
-            split16(x0, x1, &xh, &xl);
-            hh[b] = mfma(xh, wh, hh[b]);
-            mid[b] = mfma(xh, wl, mid[b]);
-            ll[b] = mfma(xl, wl, ll[b]);
-            mid[b] = mfma(xl, wh, mid[b]);
-        }
+        v4i x0 = {}, x1 = {}, xh, xl;
+        if (row < a.rows) load16(a.x + row * a.x_stride, s * 64 + 16 * (lane >> 4), a.k, &x0, &x1);
+        sum = sum8(x1, sum8(x0, sum));
+        split16(x0, x1, &xh, &xl);
+        hh = mfma(xh, wh, hh);
+        mid = mfma(xh, wl, mid);
+        ll = mfma(xl, wl, ll);
+        mid = mfma(xl, wh, mid);
     }
+    atomicAdd(&x_sum[lane & 15], sum);
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        atomicAdd(&x_sum[b * 16 + (lane & 15)], sums[b]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            atomicAdd(&total[b * 256 + (4 * (lane >> 4) + r) * 16 + (lane & 15)],
-                      static_cast<unsigned long long>(join(hh[b][r], mid[b][r], ll[b][r])));
-    }
+    for (int r = 0; r < 4; ++r)
+        atomicAdd(&total[(4 * (lane >> 4) + r) * 16 + (lane & 15)],
+                  static_cast<unsigned long long>(join(hh[r], mid[r], ll[r])));
     __syncthreads();
-    const int64_t* offs =
-        reinterpret_cast<const int64_t*>(a.weights + static_cast<size_t>(gridDim.x) * steps * 2048) + col0;
-    for (int i = threadIdx.x; i < MB * 256; i += blockDim.x) {
-        const size_t row = row0 + (i >> 4);
+    const int64_t* offs = reinterpret_cast<const int64_t*>(a.weights + static_cast<size_t>(gridDim.x) * steps * 2048);
+    const int64_t off = reinterpret_cast<const int*>(offs + static_cast<size_t>(gridDim.x) * 16)[blockIdx.x];
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) {
         const int col = col0 + (i & 15);
-        if (row < a.rows && col < a.n)
-            finish(a, row, col,
-                   static_cast<int64_t>(total[i]) + offs[i & 15] + 128 * static_cast<int64_t>(x_sum[i >> 4]));
+        if (row0 + (i >> 4) < a.rows && col < a.n)
+            finish(a, row0 + (i >> 4), col, static_cast<int64_t>(total[i]) + offs[col] + off * x_sum[i >> 4]);
     }
 }
 
 // ---- many rows -----------------------------------------------------------------------
-// A workgroup of 2 x 2 waves computes a tile of 32 I rows x 32 J columns, each
-// wave I x J blocks of 16 x 16.  Along k it takes steps of 64: the step's x rows
-// (raw i16) and packed weights go from memory to LDS without passing through
-// registers, two steps deep, and a wave splits its x fragments into planes as
-// it reads them.  Fragments lie in LDS in the order the lanes read them.
+// A workgroup of WM x WN waves computes a tile of 32 WM I rows x 32 WN J
+// columns, each wave I x J blocks of 32 x 32.  Along k it takes steps of 64: the
+// step's x rows (raw i16) and packed weights go from memory to LDS without
+// passing through registers, STAGES - 1 steps ahead, and a wave splits its x
+// fragments into planes as it reads them.  Fragments lie in LDS in the order the
+// lanes read them.
 //
 // x is copied in pieces of 8 elements when every piece is 16-byte aligned
 // (`Aligned`), else through registers.  Places past k of a row's last piece may
 // then hold anything: their weights are 0, and the identity of fixed.hpp holds
 // for whatever x they have, as the same bytes feed products and sums.
-// One 64-bit sum after its rounding shift (whose half is already in it), in 16 bits.
-__device__ inline int shifted_sat(int64_t sum, uint32_t shift) {
-    const int64_t v = sum >> shift;
-    const int lo = static_cast<int>(v), hi = static_cast<int>(v >> 32);
-    const int fit = hi == (lo >> 31) ? lo : (hi >> 31) ^ 0x7fffffff;
-    return min(max(fit, -32768), 32767);
-}
-
-template <int I, int J, bool Aligned>
-__global__ __launch_bounds__(256, 2) void fx_linear_tile_kernel(FxLinear a, unsigned row_tiles, unsigned col_tiles) {
-    constexpr int BM = 32 * I, BN = 32 * J;
+template <int WM, int WN, int I, int J, int STAGES, bool Aligned>
+__global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinear a, unsigned row_tiles,
+                                                                         unsigned col_tiles) {
+    constexpr int BM = 32 * WM * I, BN = 32 * WN * J, WAVES = WM * WN;
     constexpr int XP = BM / 8, WP = BN / 8;  // KiB pieces of a step
+    static_assert(XP % WAVES == 0 && WP % WAVES == 0 && WAVES % 2 == 0, "equal shares of copies");
     constexpr int OUT_STRIDE = BN + 8;       // i16 of a row of finished values in LDS
     constexpr int STAGE = (XP + WP) * 1024;
     __shared__ __attribute__((aligned(1024)))
-    unsigned char lds[2 * STAGE > BM * OUT_STRIDE * 2 ? 2 * STAGE : BM * OUT_STRIDE * 2];
+    unsigned char lds[STAGES * STAGE > BM * OUT_STRIDE * 2 ? STAGES * STAGE : BM * OUT_STRIDE * 2];
     __shared__ int x_sum[BM];
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
     const int steps = (a.k + 63) / 64, blocks = (a.n + 15) / 16;
     // Workgroups go to the XCDs in turn: each XCD takes a run of neighbouring
     // tiles, so that their rows and columns meet in its L2.
@@ -158,16 +153,16 @@ __global__ __launch_bounds__(256, 2) void fx_linear_tile_kernel(FxLinear a, unsi
 
     // The pieces a wave copies: x piece p holds, of rows 16 (p >> 1) .., half p & 1
     // of each lane's 16 places; weight piece p is block p >> 1's plane p & 1.
-    uint32_t x_at[XP / 4];
+    uint32_t x_at[XP / WAVES];
 #pragma unroll
-    for (int i = 0; i < XP / 4; ++i)
-        x_at[i] = static_cast<uint32_t>(min(((i * 4 + wave) >> 1) * 16 + (lane & 15), rows - 1) * a.x_stride);
+    for (int i = 0; i < XP / WAVES; ++i)
+        x_at[i] = static_cast<uint32_t>(min(((i * WAVES + wave) >> 1) * 16 + (lane & 15), rows - 1) * a.x_stride);
     const uint32_t k_at = 16 * (lane >> 4) + 8 * (wave & 1), k_last = (a.k - 1) & ~7;
     auto stage = [&](int s, unsigned char* to) {
         const uint32_t at = s * 64 + k_at;
 #pragma unroll
-        for (int i = 0; i < XP / 4; ++i) {
-            unsigned char* place = to + (i * 4 + wave) * 1024;
+        for (int i = 0; i < XP / WAVES; ++i) {
+            unsigned char* place = to + (i * WAVES + wave) * 1024;
             if constexpr (Aligned) {
                 copy_to_lds(x, 2 * (x_at[i] + min(at, k_last)), place);
             } else {
@@ -176,7 +171,7 @@ __global__ __launch_bounds__(256, 2) void fx_linear_tile_kernel(FxLinear a, unsi
                     int16_t e[8];
                 } u;
                 u.v = v4i{0, 0, 0, 0};
-                const int16_t* from = x + min(((i * 4 + wave) >> 1) * 16 + (lane & 15), rows - 1) * a.x_stride + at;
+                const int16_t* from = x + min(((i * WAVES + wave) >> 1) * 16 + (lane & 15), rows - 1) * a.x_stride + at;
                 if (at + 8 <= static_cast<uint32_t>(a.k)) {
                     u.v = load8(from);
                 } else {
@@ -188,88 +183,123 @@ __global__ __launch_bounds__(256, 2) void fx_linear_tile_kernel(FxLinear a, unsi
             }
         }
 #pragma unroll
-        for (int i = 0; i < WP / 4; ++i) {
-            const int p = i * 4 + wave, b = min(block0 + (p >> 1), blocks - 1);
+        for (int i = 0; i < WP / WAVES; ++i) {
+            const int p = i * WAVES + wave, b = min(block0 + (p >> 1), blocks - 1);
             copy_to_lds(a.weights + (static_cast<size_t>(b) * steps + s) * 2048 + (p & 1) * 1024, lane * 16,
                         to + (XP + p) * 1024);
         }
     };
 
-    v4i hh[I][J] = {}, mid[I][J] = {}, ll[I][J] = {};
+    const int64_t* offs = reinterpret_cast<const int64_t*>(a.weights + static_cast<size_t>(blocks) * steps * 2048);
+    // Row sums of x are needed where a weight of the tile needed its offset.
+    const int* o = reinterpret_cast<const int*>(offs + static_cast<size_t>(blocks) * 16);
+    bool offset = false;
+    for (int b = block0; b < min(block0 + BN / 16, blocks); ++b) offset |= o[b] != 0;
+
+    v16i hh[I][J] = {}, mid[I][J] = {}, ll[I][J] = {};
     int sums[I] = {};
-    stage(0, lds);
+    // A lane's fragment of 32 rows (or columns) and half u of the step: its row is
+    // lane & 31, its 16 places start at 32 u + 16 (lane >> 5).
+    const int in_block = ((lane >> 4) & 1) * 128 + (lane >> 5) * 16 + (lane & 15);
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+        if (s < steps) stage(s, lds + s * STAGE);
+    int now_at = 0, next_at = (STAGES - 1) * STAGE;
     for (int s = 0; s < steps; ++s) {
-        lds_copies_done();
-        __syncthreads();  // this step's copies have landed for all waves, and all have left the other buffer
-        if (s + 1 < steps) stage(s + 1, lds + ((s + 1) & 1) * STAGE);
-        const unsigned char* now = lds + (s & 1) * STAGE;
-        const v4i* xs = reinterpret_cast<const v4i*>(now) + wm * I * 128 + lane;
-        const v4i* ws = reinterpret_cast<const v4i*>(now + XP * 1024) + wn * J * 128 + lane;
-        v4i wh[J], wl[J];
+        // This step's copies have landed for all waves, and all have left the
+        // buffer of the step before.
+        if (Aligned && s + STAGES - 2 < steps)
+            lds_copies_done<(STAGES - 2) * (XP + WP) / WAVES>();
+        else
+            lds_copies_done<0>();
+        __syncthreads();
+        if (s + STAGES - 1 < steps) stage(s + STAGES - 1, lds + next_at);
+        const unsigned char* now = lds + now_at;
+        next_at = now_at;
+        now_at = now_at + STAGE == STAGES * STAGE ? 0 : now_at + STAGE;
+        const v4i* xs = reinterpret_cast<const v4i*>(now) + wm * I * 256 + in_block;
+        const v4i* ws = reinterpret_cast<const v4i*>(now + XP * 1024) + wn * J * 256 + in_block;
 #pragma unroll
-        for (int j = 0; j < J; ++j) wh[j] = ws[j * 128], wl[j] = ws[j * 128 + 64];
+        for (int u = 0; u < 2; ++u) {
+            v4i wh[J], wl[J];
 #pragma unroll
-        for (int i = 0; i < I; ++i) {
-            const v4i x0 = xs[i * 128], x1 = xs[i * 128 + 64];
-            sums[i] = sum8(x1, sum8(x0, sums[i]));
-            v4i xh, xl;
-            split16(x0, x1, &xh, &xl);
+            for (int j = 0; j < J; ++j) wh[j] = ws[j * 256 + u * 32], wl[j] = ws[j * 256 + 64 + u * 32];
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
-                hh[i][j] = mfma(xh, wh[j], hh[i][j]);
-                mid[i][j] = mfma(xh, wl[j], mid[i][j]);
-                ll[i][j] = mfma(xl, wl[j], ll[i][j]);
+            for (int i = 0; i < I; ++i) {
+                const v4i x0 = xs[i * 256 + u * 32], x1 = xs[i * 256 + 64 + u * 32];
+                if (offset) sums[i] = sum8(x1, sum8(x0, sums[i]));
+                v4i xh, xl;
+                split16(x0, x1, &xh, &xl);
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    hh[i][j] = mfma32(xh, wh[j], hh[i][j]);
+                    mid[i][j] = mfma32(xh, wl[j], mid[i][j]);
+                    ll[i][j] = mfma32(xl, wl[j], ll[i][j]);
+                }
+#pragma unroll
+                for (int j = 0; j < J; ++j) mid[i][j] = mfma32(xl, wh[j], mid[i][j]);
             }
-#pragma unroll
-            for (int j = 0; j < J; ++j) mid[i][j] = mfma(xl, wh[j], mid[i][j]);
         }
     }
     if (wn == 0) {
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            int t = sums[i];
-            t += __shfl_xor(t, 16);
-            t += __shfl_xor(t, 32);
-            if (lane < 16) x_sum[(wm * I + i) * 16 + lane] = t;
+            const int t = sums[i] + __shfl_xor(sums[i], 32);
+            if (lane < 32) x_sum[(wm * I + i) * 32 + lane] = t;
         }
     }
     __syncthreads();  // and the last step's buffer is free
 
-    const int64_t* offs = reinterpret_cast<const int64_t*>(a.weights + static_cast<size_t>(blocks) * steps * 2048);
     int16_t* done = reinterpret_cast<int16_t*>(lds);
-    // The sums of every place, with the column's constant and the row's.
+    // Every place with its three sums, its column's constant and its row's sum of x.
     auto each = [&](auto&& use) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int col = (block0 + wn * J + j) * 16 + (lane & 15);
+            const int place = (wn * J + j) * 32 + (lane & 31), col = block0 * 16 + place;
             int64_t off = col < a.n ? offs[col] : 0;
             if (a.bias && col < a.n) off += static_cast<int64_t>(a.bias[col]) << a.bias_shift;
             if (!a.raw && a.shift) off += int64_t{1} << (a.shift - 1);
+            const int64_t more = offset && col < a.n ? o[col >> 4] : 0;
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                const int at = (wm * I + i) * 16 + 4 * (lane >> 4);
-                const v4i xs = *reinterpret_cast<const v4i*>(x_sum + at);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    use(at + r, (wn * J + j) * 16 + (lane & 15),
-                        join(hh[i][j][r], mid[i][j][r], ll[i][j][r]) + off + (static_cast<int64_t>(xs[r]) << 7));
+                for (int r = 0; r < 16; ++r) {
+                    const int row = (wm * I + i) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                    use(row, place, hh[i][j][r], mid[i][j][r], ll[i][j][r],
+                        offset ? off + more * x_sum[row] : off);
+                }
             }
         }
     };
     if (a.raw) {
         int64_t* out = static_cast<int64_t*>(a.out) + row0 * a.out_stride + block0 * 16;
         const int cols = a.n - block0 * 16;
-        each([&](int row, int col, int64_t sum) {
-            if (row < rows && col < cols) out[row * a.out_stride + col] = sum;
+        each([&](int row, int col, int h, int m, int l, int64_t off) {
+            if (row < rows && col < cols) out[row * a.out_stride + col] = join(h, m, l) + off;
         });
         return;
     }
-    each([&](int row, int col, int64_t sum) {
-        done[row * OUT_STRIDE + col] = static_cast<int16_t>(shifted_sat(sum, a.shift));
-    });
+    if (a.shift <= 45 && a.bias_shift <= 29) {
+        // Constants below 2^45: with off = 2^16 A + B the sum is 2^16 high + low,
+        // 0 <= low < 2^16 and high in 32 bits, and its shift needs no 64-bit
+        // arithmetic (under a shift below 16, high is clamped first: past 15 bits
+        // the result is clamped whatever they are).
+        const int up = a.shift < 16 ? 16 - a.shift : 0, down = a.shift < 16 ? a.shift : 16,
+                  more = a.shift < 16 ? 0 : a.shift - 16;
+        each([&](int row, int col, int h, int m, int l, int64_t off) {
+            const int t = ((m & 255) << 8) + l + static_cast<int>(off & 0xffff);
+            int high = h + (m >> 8) + static_cast<int>(off >> 16) + (t >> 16);
+            high = up ? (min(max(high, -32768), 32767) << up) + ((t & 0xffff) >> down) : high >> more;
+            done[row * OUT_STRIDE + col] = static_cast<int16_t>(min(max(high, -32768), 32767));
+        });
+    } else {
+        each([&](int row, int col, int h, int m, int l, int64_t off) {
+            done[row * OUT_STRIDE + col] = static_cast<int16_t>(sat16((join(h, m, l) + off) >> a.shift));
+        });
+    }
     __syncthreads();
     // Rows of finished values, eight columns a thread.
-    for (int i = threadIdx.x; i < BM * (BN / 8); i += 256) {
+    for (int i = threadIdx.x; i < BM * (BN / 8); i += 64 * WAVES) {
         const int row = i / (BN / 8), at = i % (BN / 8) * 8, col = block0 * 16 + at;
         if (row >= rows || col >= a.n) continue;
         union {
@@ -300,18 +330,18 @@ __global__ __launch_bounds__(256, 2) void fx_linear_tile_kernel(FxLinear a, unsi
     }
 }
 
-template <int I, int J>
+template <int WM, int WN, int I, int J, int STAGES>
 void launch_tile(Context* c, const FxLinear& a) {
     // Aligned also needs a tile's offsets to fit 32 bits.
     const bool aligned =
-        reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0 && a.x_stride < (size_t{1} << 23);
-    const unsigned rt = static_cast<unsigned>((a.rows + 32 * I - 1) / (32 * I));
-    const unsigned ct = static_cast<unsigned>((a.n + 32 * J - 1) / (32 * J));
-    const dim3 grid((rt * ct + 7) / 8 * 8);
+        reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0 && a.x_stride < (size_t{1} << 22);
+    constexpr int BM = 32 * WM * I, BN = 32 * WN * J;
+    const unsigned rt = static_cast<unsigned>((a.rows + BM - 1) / BM), ct = static_cast<unsigned>((a.n + BN - 1) / BN);
+    const dim3 grid((rt * ct + 7) / 8 * 8), threads(64 * WM * WN);
     if (aligned)
-        hipLaunchKernelGGL((fx_linear_tile_kernel<I, J, true>), grid, dim3(256), 0, c->stream, a, rt, ct);
+        hipLaunchKernelGGL((fx_linear_tile_kernel<WM, WN, I, J, STAGES, true>), grid, threads, 0, c->stream, a, rt, ct);
     else
-        hipLaunchKernelGGL((fx_linear_tile_kernel<I, J, false>), grid, dim3(256), 0, c->stream, a, rt, ct);
+        hipLaunchKernelGGL((fx_linear_tile_kernel<WM, WN, I, J, STAGES, false>), grid, threads, 0, c->stream, a, rt, ct);
 }
 
 }  // namespace
@@ -325,23 +355,44 @@ int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t str
     return 0;
 }
 
+// Which kernel.  us for k x n on the rows given, in a loop (6 us of them the call):
+//                          16-row    64 x 64,  64 x 64,  128 x 128,  128 x 128,
+//                                    4 stages  2 stages  8 waves, 4  4 waves, 2
+//   3072 x 768, 200 rows   13.7      20.9      24.5      42.3        56.4
+//   768 x 4096, 200        16.1      9.7       10.3      16.8        20.8
+//   768 x 50257, 48        37.4      23.3      20.4      33.0        30.3
+//   768 x 4096, 800        49.6      23.6      21.5      19.4        22.9
+//   768 x 768, 6,000       66.0      27.7      25.6      32.9        28.9
+//   3072 x 768, 1,600      67.4      34.1      34.3      42.8        57.2
+//   768 x 4096, 6,000      325       118       106       111         89.9
+//   768 x 50257, 1,600               372       348       357         292
+// The 16-row kernel reads the packed weights once for 16 rows and splits k over
+// its waves: it wins while its workgroups are few, and always for 16 rows.  Few
+// tiles want depth of prefetch, a tile a CU wants eight waves on it, and past
+// that two workgroups a CU hide each other's waits.  The costs are those of a
+// step (in 1/120 us), by tiles on 256 CUs, that the measurements above show.
 int fx_linear(Context* c, const FxLinear& a) {
-    if (a.rows > 64) {
-        launch_tile<4, 4>(c, a);
-        VMX_HIP(c, hipGetLastError());
-        return 0;
+    const size_t blocks = fx_blocks(a.n), steps = fx_steps(a.k), row_blocks = (a.rows + 15) / 16;
+    const size_t small = ((blocks + 3) / 4) * ((row_blocks + 3) / 4), large = ((blocks + 7) / 8) * ((row_blocks + 7) / 8);
+    const size_t cus = c->cu_count;
+    const size_t deep = small <= cus ? 33 : small <= 2 * cus ? 80 : SIZE_MAX;
+    const size_t pairs = std::max<size_t>(43, 46 * small / cus);
+    const size_t waves8 = large <= cus ? 133 : 170 * ((large + cus - 1) / cus);
+    const size_t two = large <= cus ? 140 : 270 * ((large + 2 * cus - 1) / (2 * cus));
+    const size_t least = std::min(std::min(deep, pairs), std::min(waves8, two));
+    if (row_blocks == 1 || (row_blocks <= 1024 && blocks * row_blocks <= 1400 * std::max<size_t>(1, small / (2 * cus)))) {
+        const unsigned waves = static_cast<unsigned>(std::min<size_t>(steps, blocks * row_blocks < cus ? 16 : 4));
+        hipLaunchKernelGGL(fx_linear_rows_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(row_blocks)),
+                           dim3(64 * waves), 0, c->stream, a);
+    } else if (deep == least) {
+        launch_tile<2, 2, 1, 1, 4>(c, a);
+    } else if (pairs == least) {
+        launch_tile<2, 2, 1, 1, 2>(c, a);
+    } else if (waves8 == least) {
+        launch_tile<4, 2, 1, 2, 4>(c, a);
+    } else {
+        launch_tile<2, 2, 2, 2, 2>(c, a);
     }
-    const size_t blocks = fx_blocks(a.n), steps = fx_steps(a.k);
-    const unsigned waves = static_cast<unsigned>(steps < 16 ? steps : 16);
-    const int mb = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((a.rows + 16 * mb - 1) / (16 * mb)));
-    const dim3 threads(64 * waves);
-    if (mb == 1)
-        hipLaunchKernelGGL(fx_linear_rows_kernel<1>, grid, threads, 0, c->stream, a);
-    else if (mb == 2)
-        hipLaunchKernelGGL(fx_linear_rows_kernel<2>, grid, threads, 0, c->stream, a);
-    else
-        hipLaunchKernelGGL(fx_linear_rows_kernel<4>, grid, threads, 0, c->stream, a);
     VMX_HIP(c, hipGetLastError());
     return 0;
 }
