@@ -173,13 +173,15 @@ int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t str
 int fx_linear(Context* c, const FxLinear& a);
 
 // ---- attention over a cache ---------------------------------------------------------
-// One record per (slot, key head, 64 tokens), heads padded to 64 or 128 places:
-//   keys     16 tokens a subtile x 64 places a step x plane, 1 KiB each in the
-//            order a wave reads them (lane l: token l & 15, places 16 (l >> 4) .. + 15)
-//   values   16 places a block x plane, 1 KiB each (lane l: place l & 15, byte
-//            4 t + r of token 16 t + 4 (l >> 4) + r: the order in which a wave
-//            holds the scores of 64 tokens)
-//   offsets  128 sum_d k of each token, i32
+// One record per (slot, key head, 64 tokens), heads padded to 64 or 128 places,
+// in pieces of 1 KiB in the order a wave reads them:
+//   keys    32-token block x 32 places x plane (lane l: token l & 31, places
+//           16 (l >> 5) .. + 15), split as weights are, with an offset for
+//           tokens that hold a value over 32,639
+//   values  32-token block x 32 places x plane (lane l: place l & 31, byte
+//           4 q + r of token 8 q + 4 (l >> 5) + r: the order in which a wave holds
+//           the scores of 32 tokens), split with the offset always
+//   extras  256 sum_d k + the key's offset, of each token, i32
 constexpr int FX_TILE = 64;
 constexpr size_t FX_HEAD_MAX = 128;
 constexpr size_t FX_CACHE_MAX = 65536;  // tokens a slot: the i32 sums of e v hold 87,000

@@ -6,19 +6,21 @@
 // runs over the keys a query may see, and a query without any gives zeros.
 //
 // Rows of a launch are the pairs (token, query head) of one key head's group,
-// so grouped heads share the keys and values that a wave reads.  Scores are
+// so grouped heads share the keys and values that a workgroup reads.  Scores are
 // computed transposed, S^T = K Q^T: a lane then holds scores of one query only,
 // its statistics are one register, and the exponentials are already in the
 // layout in which O^T = V^T E^T reads them.
 //
-// 16-bit scores from four i8 products, as in fixed.hpp; s - 2^16 sum qh kh fits
-// 32 bits for heads of up to 128, so z = (hh << 16 - s1) + (c >> s1) >> s2 with
+// 16-bit scores from four i8 products, as in fixed.hpp, with offsets only for
+// keys and queries that hold a value over 32,639; s - 2^16 sum qh kh fits 32 bits
+// for heads of up to 128, so z = ((hh << 16 - s1) + (c >> s1)) >> s2 with
 // s1 = min(shift, 16) never needs 64-bit arithmetic.  e (at most 2^14) is
-// 256 h + l with signed bytes, so sum e v needs no correction but
-// 128 sum e for the values' low bytes.
-#include "fixed.hpp"
-
+// 256 h + l with signed bytes; values keep the constant offset of 128, whose
+// correction is 128 sum e.
+#include <algorithm>
 #include <climits>
+
+#include "fixed.hpp"
 
 namespace vmx {
 namespace {
@@ -44,8 +46,40 @@ __device__ inline uint32_t sequence_of(const Seqs& q, uint32_t at) {
     return lo;
 }
 
+// Parts of a record (fixed.hpp), in bytes.
 template <int DC>
-constexpr size_t RECORD = DC * 16384 + 256;
+struct Record {
+    static constexpr int VALUES = DC * 8192, EXTRA = DC * 16384, BYTES = DC * 16384 + 256;
+};
+
+// Sixteen i16 less o (0 or 128) as their signed high and low bytes.
+__device__ inline void split16(v4i lo, v4i hi, int o, v4i* h, v4i* l) {
+    const int up = o ? 0 : 0x00800080, flip = o ? 0x80808080 : 0;
+    v4i a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int x = lo[i], y = hi[i];
+        a[i] = __builtin_bit_cast(int, __builtin_bit_cast(v2s, x) + __builtin_bit_cast(v2s, up));
+        b[i] = __builtin_bit_cast(int, __builtin_bit_cast(v2s, y) + __builtin_bit_cast(v2s, up));
+    }
+    const uint32_t top = 0x07050301u, bottom = 0x06040200u;
+    *h = v4i{static_cast<int>(__builtin_amdgcn_perm(a[1], a[0], top)),
+             static_cast<int>(__builtin_amdgcn_perm(a[3], a[2], top)),
+             static_cast<int>(__builtin_amdgcn_perm(b[1], b[0], top)),
+             static_cast<int>(__builtin_amdgcn_perm(b[3], b[2], top))};
+    *l = v4i{static_cast<int>(__builtin_amdgcn_perm(lo[1], lo[0], bottom)) ^ flip,
+             static_cast<int>(__builtin_amdgcn_perm(lo[3], lo[2], bottom)) ^ flip,
+             static_cast<int>(__builtin_amdgcn_perm(hi[1], hi[0], bottom)) ^ flip,
+             static_cast<int>(__builtin_amdgcn_perm(hi[3], hi[2], bottom)) ^ flip};
+}
+
+// Whether one of eight i16 is over HALVES_MAX.
+__device__ inline bool large8(v4i v) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= static_cast<int16_t>(v[i]) > HALVES_MAX || (v[i] >> 16) > HALVES_MAX;
+    return any;
+}
 
 // ---- append ---------------------------------------------------------------------------
 // One workgroup per (key head, 64-token tile that new tokens touch).
@@ -59,37 +93,97 @@ struct AppendArgs {
 
 template <int DC>
 __global__ __launch_bounds__(256) void fx_append_kernel(AppendArgs a, Seqs q) {
-    constexpr int DP = DC * 64;
+    __shared__ int sums[64], large[64];
     const uint32_t at = sequence_of(q, blockIdx.x);
     const FxSeq s = q.s[at];
     const int past = static_cast<int>(s.length - s.count);
     const int tile = past / FX_TILE + static_cast<int>(blockIdx.x - q.first[at]);
     const int head = blockIdx.y;
-    unsigned char* rec = a.data + ((static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles + tile) * RECORD<DC>;
-    unsigned char* keys = rec;
-    unsigned char* values = rec + DP * 128;
-    int* offs = reinterpret_cast<int*>(rec + DP * 256);
+    unsigned char* rec =
+        a.data + ((static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles + tile) * Record<DC>::BYTES;
+    unsigned char* values = rec + Record<DC>::VALUES;
+    int* extra = reinterpret_cast<int*>(rec + Record<DC>::EXTRA);
     const int from = max(past - tile * FX_TILE, 0), to = min(static_cast<int>(s.length) - tile * FX_TILE, FX_TILE);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // row of token j of this tile
+    const size_t row0 = static_cast<size_t>(s.row) + tile * FX_TILE - past;
+    const int16_t* k0 = a.k + static_cast<size_t>(head) * a.dim;
+    const int16_t* v0 = a.v + static_cast<size_t>(head) * a.dim;
+    if (from == 0) {
+        // A tile from its first token on: whole pieces of 16 bytes; what they
+        // hold of tokens past the last is never used.
+        if (threadIdx.x < 64) sums[threadIdx.x] = large[threadIdx.x] = 0;
+        __syncthreads();
+        const int j = threadIdx.x & 63;
+        v4i lo[DC], hi[DC];
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+            lo[c] = hi[c] = v4i{0, 0, 0, 0};
+            if (j < to) {
+                load16(k0 + (row0 + j) * a.k_stride, (c * 4 + wave) * 16, a.dim, &lo[c], &hi[c]);
+                atomicAdd(&sums[j], sum8(hi[c], sum8(lo[c], 0)));
+                if (large8(lo[c]) || large8(hi[c])) large[j] = 128;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+            const int piece = c * 4 + wave;  // places 16 piece ..
+            v4i h, l;
+            split16(lo[c], hi[c], large[j], &h, &l);
+            v4i* p = reinterpret_cast<v4i*>(rec) + ((j >> 5) * 2 * DC + (piece >> 1)) * 128 + (j & 31) + 32 * (piece & 1);
+            p[0] = h;
+            p[64] = l;
+        }
+        if (threadIdx.x < 64) extra[j] = sums[j] * 256 + large[j];
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+            // piece (32-token block, half of it, place)
+            const int i = c * 256 + threadIdx.x, d = i % (64 * DC), part = i / (64 * DC), block = part >> 1, half = part & 1;
+            union {
+                v4i v;
+                uint8_t b[16];
+            } h, l;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int t = block * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+                const int x = t < to && d < a.dim ? v0[(row0 + t) * a.v_stride + d] : 0;
+                h.b[e] = static_cast<uint8_t>(x >> 8);
+                l.b[e] = static_cast<uint8_t>(x ^ 0x80);
+            }
+            v4i* p = reinterpret_cast<v4i*>(values) + (block * 2 * DC + (d >> 5)) * 128 + (d & 31) + 32 * half;
+            p[0] = h.v;
+            p[64] = l.v;
+        }
+        return;
+    }
+    // Tokens after others of their tile: their own bytes, a token a wave.
     for (int j = from + wave; j < to; j += 4) {
-        const size_t row = s.row + (tile * FX_TILE + j - past);
-        const int16_t* k = a.k + row * a.k_stride + static_cast<size_t>(head) * a.dim;
-        const int16_t* v = a.v + row * a.v_stride + static_cast<size_t>(head) * a.dim;
         int sum = 0;
+        bool over = false;
+        int kd[DC], vd[DC];
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
             const int d = c * 64 + lane;
-            const int kd = d < a.dim ? k[d] : 0, vd = d < a.dim ? v[d] : 0;
-            sum += kd;
-            unsigned char* pk = keys + (((j >> 4) * DC + c) * 2) * 1024 + ((j & 15) + 16 * (lane >> 4)) * 16 + (lane & 15);
-            pk[0] = static_cast<unsigned char>(kd >> 8);
-            pk[1024] = static_cast<unsigned char>(kd ^ 0x80);
-            unsigned char* pv = values + (d >> 4) * 2048 + ((d & 15) + 16 * ((j & 15) >> 2)) * 16 + (j >> 4) * 4 + (j & 3);
-            pv[0] = static_cast<unsigned char>(vd >> 8);
-            pv[1024] = static_cast<unsigned char>(vd ^ 0x80);
+            kd[c] = d < a.dim ? k0[(row0 + j) * a.k_stride + d] : 0;
+            vd[c] = d < a.dim ? v0[(row0 + j) * a.v_stride + d] : 0;
+            sum += kd[c];
+            over |= kd[c] > HALVES_MAX;
         }
+        const int o = __any(over) ? 128 : 0;
         for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
-        if (lane == 0) offs[j] = 128 * sum;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+            const int d = c * 64 + lane, kk = halves(kd[c] - o);
+            unsigned char* pk = rec + (((j >> 5) * 2 * DC + (d >> 5)) * 128 + (j & 31) + 32 * ((d >> 4) & 1)) * 16 + (d & 15);
+            pk[0] = static_cast<unsigned char>(kk >> 8);
+            pk[1024] = static_cast<unsigned char>(kk);
+            unsigned char* pv = values + (((j >> 5) * 2 * DC + (d >> 5)) * 128 + (d & 31) + 32 * ((j >> 2) & 1)) * 16 +
+                                ((j >> 3) & 3) * 4 + (j & 3);
+            pv[0] = static_cast<unsigned char>(vd[c] >> 8);
+            pv[1024] = static_cast<unsigned char>(vd[c] ^ 0x80);
+        }
+        if (lane == 0) extra[j] = sum * 256 + o;
     }
 }
 
@@ -108,146 +202,254 @@ struct AttentionArgs {
     bool causal;
 };
 
-// A lane's query: its planes along d and 128 sum_d (q - 128).
+// Keys that row `row` of a sequence may see.
+__device__ inline int limit_of(const AttentionArgs& a, const FxSeq& s, int row) {
+    return static_cast<int>(s.length) - (a.causal ? static_cast<int>(s.count) - row / a.group - 1 : 0);
+}
+
+// A lane's query: its planes (32 places a step) and sum_d (q - o) and o.
 template <int DC>
 struct Query {
-    v4i h[DC], l[DC];
-    int offset;
-    int limit;  // keys it may see
+    v4i h[2 * DC], l[2 * DC];
+    int sum, o;
 };
 
+// The 16 places of a step that lane holds start at 16 (lane >> 5).
 template <int DC>
 __device__ inline void load_query(const AttentionArgs& a, const FxSeq& s, int head, int row, int lane, Query<DC>* q) {
-    const int rows = static_cast<int>(s.count) * a.group;
-    const bool live = row < rows;
+    const bool live = row < static_cast<int>(s.count) * a.group;
     const int token = live ? row / a.group : 0, member = live ? row - token * a.group : 0;
     const int16_t* p = a.q + (static_cast<size_t>(s.row) + token) * a.q_stride +
                        (static_cast<size_t>(head) * a.group + member) * a.dim;
-    int sum = 0;
+    v4i lo[2 * DC], hi[2 * DC];
+    int sum = 0, large = 0;
 #pragma unroll
-    for (int c = 0; c < DC; ++c) {
-        v4i x0 = {}, x1 = {};
-        if (live) load16(p, c * 64 + 16 * (lane >> 4), a.dim, &x0, &x1);
-        sum = sum8(x1, sum8(x0, sum));
-        split16(x0, x1, &q->h[c], &q->l[c]);
+    for (int u = 0; u < 2 * DC; ++u) {
+        lo[u] = hi[u] = v4i{0, 0, 0, 0};
+        if (live) load16(p, u * 32 + 16 * (lane >> 5), a.dim, &lo[u], &hi[u]);
+        sum = sum8(hi[u], sum8(lo[u], sum));
+        large |= large8(lo[u]) || large8(hi[u]);
     }
-    sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    q->offset = 128 * sum - 16384 * 64 * DC;
-    const int length = static_cast<int>(s.length);
-    q->limit = !live ? 0 : a.causal ? length - static_cast<int>(s.count) + token + 1 : length;
+    large |= __shfl_xor(large, 32);
+    q->o = large ? 128 : 0;
+    q->sum = sum - q->o * 64 * DC;
+#pragma unroll
+    for (int u = 0; u < 2 * DC; ++u) split16(lo[u], hi[u], q->o, &q->h[u], &q->l[u]);
 }
 
-// Scores z of the 16 tokens of a subtile (this lane: tokens 4 (lane >> 4) .. + 3).
+// Scores z of 32 tokens (block `block` of the record's keys and extras), this
+// lane's query: token 8 (r >> 2) + 4 (lane >> 5) + (r & 3) in place r.  `plain`:
+// neither a key of the tile nor a query of the wave has an offset.
 template <int DC>
-__device__ inline v4i scores(const v4i* keys, const int* offs, const Query<DC>& q, int sub, int lane, uint32_t s1,
-                             uint32_t s2) {
-    v4i hh = {}, mid = {}, ll = *reinterpret_cast<const v4i*>(offs + sub * 16 + 4 * (lane >> 4));
+__device__ inline v16i scores(const unsigned char* keys, const int* extra, const Query<DC>& q, int block, int lane,
+                              uint32_t s1, uint32_t s2, bool plain) {
+    v16i hh = {}, mid = {}, ll = {};
+    const v4i* p = reinterpret_cast<const v4i*>(keys) + block * 2 * DC * 128 + lane;
 #pragma unroll
-    for (int c = 0; c < DC; ++c) {
-        const v4i kh = keys[(sub * DC + c) * 128 + lane], kl = keys[(sub * DC + c) * 128 + 64 + lane];
-        hh = mfma(kh, q.h[c], hh);
-        mid = mfma(kh, q.l[c], mid);
-        ll = mfma(kl, q.l[c], ll);
-        mid = mfma(kl, q.h[c], mid);
+    for (int u = 0; u < 2 * DC; ++u) {
+        const v4i kh = p[u * 128], kl = p[u * 128 + 64];
+        hh = mfma32(kh, q.h[u], hh);
+        mid = mfma32(kh, q.l[u], mid);
+        ll = mfma32(kl, q.l[u], ll);
+        mid = mfma32(kl, q.h[u], mid);
     }
-    v4i z;
+    if (!plain) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        z[r] = ((hh[r] << (16 - s1)) + ((static_cast<int>((static_cast<uint32_t>(mid[r]) << 8) + ll[r] + q.offset)) >> s1)) >> s2;
+        for (int r = 0; r < 16; ++r) {
+            const int x = extra[block * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)];
+            ll[r] = static_cast<int>(static_cast<uint32_t>(ll[r]) + static_cast<uint32_t>((x & 128) * q.sum) +
+                                     static_cast<uint32_t>((x >> 8) * q.o));
+        }
+    }
+    v16i z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        z[r] = (hh[r] << (16 - s1)) + (static_cast<int>((static_cast<uint32_t>(mid[r]) << 8) + ll[r]) >> s1);
+    if (s2) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] >>= s2;
+    }
     return z;
 }
 
 // e (at most 2^14) as its two signed bytes: high in bits 15..8, low in bits 7..0.
-__device__ inline uint32_t encoded(uint32_t e) { return (min(e, 16384u) + 128) ^ 128; }
+__device__ inline uint32_t encoded(uint32_t e) { return halves(static_cast<int>(min(e, 16384u))); }
 
-template <int DC>
-__device__ inline void store_out(const AttentionArgs& a, const FxSeq& s, int head, int row, int d, const int64_t* sums,
-                                 int64_t total) {
-    if (row >= static_cast<int>(s.count) * a.group) return;
-    const int token = row / a.group, member = row - token * a.group;
-    int16_t* p = a.out + (static_cast<size_t>(s.row) + token) * a.out_stride +
-                 (static_cast<size_t>(head) * a.group + member) * a.dim + d;
+// out[d .. d + 3] of a row from sum e (v - 128) and sum e.
+__device__ inline void store4(int16_t* p, int live, const int64_t* sums, int64_t total) {
     const double below = 2.0 * static_cast<double>(total), inv = total ? 1.0 / below : 0.0;
+    union {
+        uint2 v;
+        int16_t e[4];
+    } u;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        if (d + r >= a.dim) break;
         const double num = static_cast<double>(2 * (sums[r] + 128 * total) + total);
-        p[r] = total ? static_cast<int16_t>(floor_div(num, below, inv)) : 0;
+        u.e[r] = total ? static_cast<int16_t>(floor_div(num, below, inv)) : 0;
+    }
+    if (live >= 4) {
+        reinterpret_cast<Row8*>(p)->v = u.v;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < live) p[r] = u.e[r];
     }
 }
 
-// One wave per 16 rows, one pass for the maximum and one for the sums.
+// Many rows: a workgroup takes 128 rows of a sequence and key head, 32 for each
+// group of DC waves, and goes over the tiles of 64 tokens twice: for the
+// maximum, then for the sums.  Records come to LDS by direct copies, one tile
+// ahead.  With heads over 64 (DC = 2) the two waves of a group take 32 tokens of
+// a tile each, exchange the exponentials through LDS, and keep half of the
+// result's places each: 96 accumulators a lane either way.
 template <int DC>
-__global__ __launch_bounds__(256) void fx_attention_kernel(AttentionArgs a, Seqs q) {
+__global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs a, Seqs q) {
+    constexpr int WAVES = 4 * DC, STAGE = Record<DC>::BYTES;
+    __shared__ __attribute__((aligned(1024))) unsigned char stages[2][(STAGE + 1023) / 1024 * 1024];
+    __shared__ __attribute__((aligned(16))) uint16_t table[FX_TABLE_MAX];
+    __shared__ __attribute__((aligned(16))) v4i swap[DC == 2 ? WAVES * 128 : 1];
+    __shared__ int share[WAVES][32];
     const uint32_t at = sequence_of(q, blockIdx.x);
     const FxSeq s = q.s[at];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.y;
-    const int row = static_cast<int>(blockIdx.x - q.first[at]) * 64 + wave * 16 + (lane & 15);
-    const unsigned char* base = a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles * RECORD<DC>;
+    const int lane = threadIdx.x & 63, head = blockIdx.y;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave / DC, part = wave % DC;
+    const int rows = static_cast<int>(s.count) * a.group;
+    // the longest tiles first
+    const int row0 = static_cast<int>(q.first[at + 1] - 1 - blockIdx.x) * 128;
+    const int row = row0 + group * 32 + (lane & 31);
+    const unsigned char* base =
+        a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles * static_cast<size_t>(STAGE);
     Query<DC> mine;
     load_query<DC>(a, s, head, row, lane, &mine);
-    int last = mine.limit;
-    for (int m = 32; m; m >>= 1) last = max(last, __shfl_xor(last, m));
-    const int tiles = (last + FX_TILE - 1) / FX_TILE;
+    const bool no_offset = !__any(mine.o);
+    const int limit = limit_of(a, s, min(row, rows - 1));
+    // what all rows of the wave see, and what one of the workgroup's sees
+    const int all = limit_of(a, s, min(row0 + group * 32, rows - 1));
+    const int tiles = (limit_of(a, s, min(row0 + 127, rows - 1)) + FX_TILE - 1) / FX_TILE;
+    for (uint32_t i = threadIdx.x; i < a.entries; i += 64 * WAVES)
+        table[i] = static_cast<uint16_t>(encoded(a.table[i]));
+    const uint32_t last = a.entries - 1;
+
+    auto stage = [&](int t, int pieces, unsigned char* to) {
+        const unsigned char* rec = base + static_cast<size_t>(t) * STAGE;
+        for (int p = wave; p < pieces; p += WAVES) copy_to_lds(rec + p * 1024, lane * 16, to + p * 1024);
+        if (wave == 0 && lane < 16) copy_to_lds(rec + Record<DC>::EXTRA, lane * 16, to + Record<DC>::EXTRA);
+    };
+    // Runs `use` on every tile's record in LDS, `pieces` KiB of it and its extras.
+    auto over_tiles = [&](int pieces, auto&& use) {
+        if (tiles > 0) stage(0, pieces, stages[0]);
+        for (int t = 0; t < tiles; ++t) {
+            lds_copies_done<0>();
+            __syncthreads();  // this tile has landed for all waves, and all have left the other buffer
+            if (t + 1 < tiles) stage(t + 1, pieces, stages[(t + 1) & 1]);
+            const unsigned char* rec = stages[t & 1];
+            const int* extra = reinterpret_cast<const int*>(rec + Record<DC>::EXTRA);
+            const bool offset = lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128);
+            use(t, rec, extra, no_offset && !__any(offset));
+        }
+        __syncthreads();
+    };
 
     int top = INT_MIN;
-    for (int t = 0; t < tiles; ++t) {
-        const unsigned char* rec = base + static_cast<size_t>(t) * RECORD<DC>;
+    over_tiles(8 * DC, [&](int t, const unsigned char* rec, const int* extra, bool plain) {
 #pragma unroll
-        for (int sub = 0; sub < 4; ++sub) {
-            const v4i z = scores<DC>(reinterpret_cast<const v4i*>(rec), reinterpret_cast<const int*>(rec + DC * 16384),
-                                     mine, sub, lane, a.s1, a.s2);
+        for (int b = 0; b < 2 / DC; ++b) {
+            const int block = DC == 2 ? part : b, token = t * FX_TILE + block * 32;
+            const v16i z = scores<DC>(rec, extra, mine, block, lane, a.s1, a.s2, plain);
+            if (token + 32 <= all) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (t * FX_TILE + sub * 16 + 4 * (lane >> 4) + r < mine.limit) top = max(top, z[r]);
-        }
-    }
-    top = max(top, __shfl_xor(top, 16));
-    top = max(top, __shfl_xor(top, 32));
-
-    v4i hh[DC * 4] = {}, mid[DC * 4] = {}, ll[DC * 4] = {};
-    int sum_h = 0, sum_l = 0;
-    for (int t = 0; t < tiles; ++t) {
-        const unsigned char* rec = base + static_cast<size_t>(t) * RECORD<DC>;
-        v4i eh, el;
+                for (int r = 0; r < 16; ++r) top = max(top, z[r]);
+            } else {
 #pragma unroll
-        for (int sub = 0; sub < 4; ++sub) {
-            const v4i z = scores<DC>(reinterpret_cast<const v4i*>(rec), reinterpret_cast<const int*>(rec + DC * 16384),
-                                     mine, sub, lane, a.s1, a.s2);
-            uint32_t e[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool seen = t * FX_TILE + sub * 16 + 4 * (lane >> 4) + r < mine.limit;
-                const uint32_t d = min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[r]), a.entries - 1);
-                e[r] = seen ? encoded(a.table[d]) : 0;
+                for (int r = 0; r < 16; ++r)
+                    if (token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) < limit) top = max(top, z[r]);
             }
-            const uint32_t a01 = e[0] | e[1] << 16, a23 = e[2] | e[3] << 16;
-            eh[sub] = __builtin_amdgcn_perm(a23, a01, 0x07050301u);
-            el[sub] = __builtin_amdgcn_perm(a23, a01, 0x06040200u);
-            sum_h = __builtin_amdgcn_sdot4(eh[sub], 0x01010101, sum_h, false);
-            sum_l = __builtin_amdgcn_sdot4(el[sub], 0x01010101, sum_l, false);
         }
-        const v4i* values = reinterpret_cast<const v4i*>(rec + DC * 8192) + lane;
-#pragma unroll
-        for (int b = 0; b < DC * 4; ++b) {
-            const v4i vh = values[b * 128], vl = values[b * 128 + 64];
-            hh[b] = mfma(vh, eh, hh[b]);
-            mid[b] = mfma(vh, el, mid[b]);
-            ll[b] = mfma(vl, el, ll[b]);
-            mid[b] = mfma(vl, eh, mid[b]);
-        }
+    });
+    top = max(top, __shfl_xor(top, 32));
+    if constexpr (DC == 2) {
+        if (lane < 32) share[wave][lane] = top;
+        __syncthreads();
+        top = max(top, share[wave ^ 1][lane & 31]);
+        __syncthreads();
     }
+
+    v16i hh[2] = {}, mid[2] = {}, ll[2] = {};  // 32 places each, of this wave's 64
+    int sum_h = 0, sum_l = 0;
+    over_tiles(16 * DC, [&](int t, const unsigned char* rec, const int* extra, bool plain) {
+        const v4i* values = reinterpret_cast<const v4i*>(rec + Record<DC>::VALUES) + lane;
+        auto add = [&](int block, v4i eh, v4i el) {
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const v4i* p = values + (block * 2 * DC + part * 2 + d) * 128;
+                const v4i vh = p[0], vl = p[64];
+                hh[d] = mfma32(vh, eh, hh[d]);
+                mid[d] = mfma32(vh, el, mid[d]);
+                ll[d] = mfma32(vl, el, ll[d]);
+                mid[d] = mfma32(vl, eh, mid[d]);
+            }
+        };
+#pragma unroll
+        for (int b = 0; b < 2 / DC; ++b) {
+            const int block = DC == 2 ? part : b, token = t * FX_TILE + block * 32;
+            const v16i z = scores<DC>(rec, extra, mine, block, lane, a.s1, a.s2, plain);
+            v4i eh, el;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t e[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[4 * g + r]), last)];
+                if (token + 32 > all) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (token + 8 * g + 4 * (lane >> 5) + r >= limit) e[r] = 0;
+                }
+                const uint32_t a01 = e[0] | e[1] << 16, a23 = e[2] | e[3] << 16;
+                eh[g] = __builtin_amdgcn_perm(a23, a01, 0x07050301u);
+                el[g] = __builtin_amdgcn_perm(a23, a01, 0x06040200u);
+                sum_h = __builtin_amdgcn_sdot4(eh[g], 0x01010101, sum_h, false);
+                sum_l = __builtin_amdgcn_sdot4(el[g], 0x01010101, sum_l, false);
+            }
+            if constexpr (DC == 1) {
+                add(block, eh, el);
+            } else {
+                swap[wave * 128 + lane] = eh;
+                swap[wave * 128 + 64 + lane] = el;
+            }
+        }
+        if constexpr (DC == 2) {
+            __syncthreads();
+#pragma unroll
+            for (int block = 0; block < 2; ++block) {
+                const v4i* p = swap + (group * 2 + block) * 128 + lane;
+                add(block, p[0], p[64]);
+            }
+        }
+    });
     int total = 256 * sum_h + sum_l;
-    total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);
-#pragma unroll
-    for (int b = 0; b < DC * 4; ++b) {
-        int64_t sums[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sums[r] = join(hh[b][r], mid[b][r], ll[b][r]);
-        store_out<DC>(a, s, head, row, b * 16 + 4 * (lane >> 4), sums, total);
+    if constexpr (DC == 2) {
+        if (lane < 32) share[wave][lane] = total;
+        __syncthreads();
+        total += share[wave ^ 1][lane & 31];
     }
+    if (row >= rows) return;
+    const int token = row / a.group, member = row - token * a.group;
+    int16_t* out = a.out + (static_cast<size_t>(s.row) + token) * a.out_stride +
+                   (static_cast<size_t>(head) * a.group + member) * a.dim;
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int place = part * 64 + d * 32 + 8 * g + 4 * (lane >> 5);
+            if (place >= a.dim) continue;
+            int64_t sums[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[r] = join(hh[d][4 * g + r], mid[d][4 * g + r], ll[d][4 * g + r]);
+            store4(out + place, a.dim - place, sums, total);
+        }
 }
 
 // Sequences in groups of FX_SEQS with work items counted by `items`; one launch each.
@@ -305,13 +507,13 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
                           t.shift - s1,
                           t.causal};
     return each_group(
-        c, seqs, count, [&](const FxSeq& s) { return (s.count * group + 63) / 64; },
+        c, seqs, count, [&](const FxSeq& s) { return (s.count * group + 127) / 128; },
         [&](const Seqs& q, uint32_t total) {
             const dim3 grid(total, static_cast<unsigned>(cache.kv_heads));
             if (cache.dim <= 64)
                 hipLaunchKernelGGL(fx_attention_kernel<1>, grid, dim3(256), 0, c->stream, a, q);
             else
-                hipLaunchKernelGGL(fx_attention_kernel<2>, grid, dim3(256), 0, c->stream, a, q);
+                hipLaunchKernelGGL(fx_attention_kernel<2>, grid, dim3(512), 0, c->stream, a, q);
         });
 }
 
