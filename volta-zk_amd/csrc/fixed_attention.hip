@@ -19,6 +19,7 @@
 // correction is 128 sum e.
 #include <algorithm>
 #include <climits>
+#include <vector>
 
 #include "fixed.hpp"
 
@@ -452,6 +453,237 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
         }
 }
 
+// ---- few rows ----------------------------------------------------------------------------
+// A workgroup takes 16 rows of a sequence and key head and a run of its tiles;
+// its eight waves take the tiles in turn, straight from memory, and add their
+// sums in LDS.  Scores are computed once and kept for the second pass, which
+// needs the maximum over the whole run:
+//   FUSED   one workgroup has all tiles: kept in LDS, one launch;
+//   SCORES, VALUES   the tiles are split over `splits` workgroups: kept in memory,
+//           with a maximum per split, between two launches.  The second adds its
+//           sums to the unit's (integers: any order gives the same), and the last
+//           workgroup of a unit to arrive divides.  The first clears them.
+enum Pass { FUSED, SCORES, VALUES };
+constexpr int FEW = 16, FEW_WAVES = 8;
+
+struct FewArgs {
+    int cols;       // rows of a unit that scores are kept for, at most FEW
+    int max_tiles;  // of a sequence
+    int splits;
+    int* z;                   // units x max_tiles x cols x 64
+    int* tops;                // units x splits x FEW
+    unsigned long long* sums;  // units x (FEW x head, FEW totals, arrivals)
+};
+
+template <int DC>
+constexpr int FEW_SUMS = FEW * (64 * DC + 1) + 1;
+
+// A lane's query for 16 x 16 products: row lane & 15, 16 of 64 places from 16 (lane >> 4).
+template <int DC>
+struct FewQuery {
+    v4i h[DC], l[DC];
+    int sum, o;
+};
+
+template <int DC, Pass PASS>
+__global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(AttentionArgs a, FewArgs f, Seqs q) {
+    extern __shared__ __attribute__((aligned(16))) int kept[];  // FUSED: scores
+    __shared__ unsigned long long sums[PASS == SCORES ? 1 : FEW * 64 * DC];
+    __shared__ unsigned long long totals[FEW];
+    __shared__ int tops[FEW_WAVES][FEW];
+    __shared__ bool final;
+    const uint32_t at = sequence_of(q, blockIdx.x);
+    const FxSeq s = q.s[at];
+    const int lane = threadIdx.x & 63, head = blockIdx.y, split = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rows = static_cast<int>(s.count) * a.group;
+    const int row0 = static_cast<int>(blockIdx.x - q.first[at]) * FEW, row = row0 + (lane & 15);
+    const int cols = min(rows - row0, FEW);  // at most f.cols
+    const bool mine = (lane & 15) < cols;
+    const size_t unit = static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+    const unsigned char* base =
+        a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles * static_cast<size_t>(Record<DC>::BYTES);
+    const int limit = limit_of(a, s, min(row, rows - 1)), all = limit_of(a, s, row0);
+    const int tiles = (limit_of(a, s, min(row0 + FEW, rows) - 1) + FX_TILE - 1) / FX_TILE;
+    const int each = (f.max_tiles + f.splits - 1) / f.splits;
+    const int from = split * each, to = min(from + each, tiles);
+    int* z_of = PASS == FUSED ? kept : f.z + unit * f.max_tiles * f.cols * 64;
+    // this lane's token in place r of its quarter t of a tile: first + 8 t + r
+    const int first = 32 * (lane >> 5) + 4 * ((lane >> 4) & 1);
+    unsigned long long* unit_sums = f.sums + unit * FEW_SUMS<DC>;
+
+    int top = INT_MIN;
+    if constexpr (PASS != VALUES) {
+        if constexpr (PASS == SCORES) {
+            if (split == 0)
+                for (int i = threadIdx.x; i < FEW_SUMS<DC>; i += 64 * FEW_WAVES) unit_sums[i] = 0;
+        }
+        FewQuery<DC> mq;
+        {
+            const int token = mine ? row / a.group : 0, member = mine ? row - token * a.group : 0;
+            const int16_t* p = a.q + (static_cast<size_t>(s.row) + token) * a.q_stride +
+                               (static_cast<size_t>(head) * a.group + member) * a.dim;
+            v4i lo[DC], hi[DC];
+            int sum = 0, large = 0;
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                lo[c] = hi[c] = v4i{0, 0, 0, 0};
+                if (mine) load16(p, c * 64 + 16 * (lane >> 4), a.dim, &lo[c], &hi[c]);
+                sum = sum8(hi[c], sum8(lo[c], sum));
+                large |= large8(lo[c]) || large8(hi[c]);
+            }
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            large |= __shfl_xor(large, 16);
+            large |= __shfl_xor(large, 32);
+            mq.o = large ? 128 : 0;
+            mq.sum = sum - mq.o * 64 * DC;
+#pragma unroll
+            for (int c = 0; c < DC; ++c) split16(lo[c], hi[c], mq.o, &mq.h[c], &mq.l[c]);
+        }
+        const bool no_offset = !__any(mq.o);
+        // the key that this lane reads for row i = lane & 15 of quarter t: 8 t past
+        // token 32 (i >> 3) + 4 ((i >> 2) & 1) + (i & 3)
+        const int in_tile = (((lane >> 3) & 1) * 2 * DC + (lane >> 5)) * 128 + (lane & 7) + 32 * ((lane >> 4) & 1);
+        for (int t = from + wave; t < to; t += FEW_WAVES) {
+            const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES;
+            const v4i* keys = reinterpret_cast<const v4i*>(rec) + in_tile;
+            const int* extra = reinterpret_cast<const int*>(rec + Record<DC>::EXTRA);
+            const bool offset = lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128);
+            v4i hh[4] = {}, mid[4] = {}, ll[4] = {};
+#pragma unroll
+            for (int c = 0; c < DC; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const v4i kh = keys[c * 256 + k * 8], kl = keys[c * 256 + 64 + k * 8];
+                    hh[k] = mfma(kh, mq.h[c], hh[k]);
+                    mid[k] = mfma(kh, mq.l[c], mid[k]);
+                    ll[k] = mfma(kl, mq.l[c], ll[k]);
+                    mid[k] = mfma(kl, mq.h[c], mid[k]);
+                }
+            if (!no_offset || __any(offset)) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int x = extra[first + 8 * k + r];
+                        ll[k][r] = static_cast<int>(static_cast<uint32_t>(ll[k][r]) +
+                                                    static_cast<uint32_t>((x & 128) * mq.sum) +
+                                                    static_cast<uint32_t>((x >> 8) * mq.o));
+                    }
+            }
+            int* zt = z_of + ((PASS == FUSED ? t - from : t) * f.cols + (lane & 15)) * 64 + 4 * (lane >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v4i z;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int low = static_cast<int>((static_cast<uint32_t>(mid[k][r]) << 8) + ll[k][r]);
+                    z[r] = ((hh[k][r] << (16 - a.s1)) + (low >> a.s1)) >> a.s2;
+                    if (t * FX_TILE + first + 8 * k + r < limit) top = max(top, z[r]);
+                }
+                if (mine) *reinterpret_cast<v4i*>(zt + 16 * k) = z;
+            }
+        }
+        top = max(top, __shfl_xor(top, 16));
+        top = max(top, __shfl_xor(top, 32));
+        if (lane < FEW) tops[wave][lane] = top;
+        __syncthreads();
+        if constexpr (PASS == SCORES) {
+            if (threadIdx.x < FEW) {
+                for (int w = 0; w < FEW_WAVES; ++w) top = max(top, tops[w][threadIdx.x]);
+                f.tops[(unit * f.splits + split) * FEW + threadIdx.x] = top;
+            }
+            return;
+        }
+        for (int w = 0; w < FEW_WAVES; ++w) top = max(top, tops[w][lane & 15]);
+    } else {
+        for (int i = 0; i < f.splits; ++i) top = max(top, f.tops[(unit * f.splits + i) * FEW + (lane & 15)]);
+    }
+
+    if constexpr (PASS != SCORES) {
+        for (int i = threadIdx.x; i < FEW * 64 * DC; i += 64 * FEW_WAVES) sums[i] = 0;
+        if (threadIdx.x < FEW) totals[threadIdx.x] = 0;
+        __syncthreads();
+        v4i hh[4 * DC] = {}, mid[4 * DC] = {}, ll[4 * DC] = {};
+        int sum_h = 0, sum_l = 0;
+        const int in_values = ((lane >> 5) * 2 * DC) * 128 + (lane & 15) + 32 * ((lane >> 4) & 1);
+        const uint32_t last = a.entries - 1;
+        for (int t = from + wave; t < to; t += FEW_WAVES) {
+            const v4i* values = reinterpret_cast<const v4i*>(base + static_cast<size_t>(t) * Record<DC>::BYTES +
+                                                             Record<DC>::VALUES) +
+                                in_values;
+            const int* zt = z_of + ((PASS == FUSED ? t - from : t) * f.cols + (lane & 15)) * 64 + 4 * (lane >> 4);
+            v4i eh, el;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t e[4] = {};
+                if (mine) {
+                    const v4i z = *reinterpret_cast<const v4i*>(zt + 16 * k);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (t * FX_TILE + first + 8 * k + r < limit)
+                            e[r] = encoded(a.table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[r]), last)]);
+                }
+                const uint32_t a01 = e[0] | e[1] << 16, a23 = e[2] | e[3] << 16;
+                eh[k] = __builtin_amdgcn_perm(a23, a01, 0x07050301u);
+                el[k] = __builtin_amdgcn_perm(a23, a01, 0x06040200u);
+                sum_h = __builtin_amdgcn_sdot4(eh[k], 0x01010101, sum_h, false);
+                sum_l = __builtin_amdgcn_sdot4(el[k], 0x01010101, sum_l, false);
+            }
+#pragma unroll
+            for (int b = 0; b < 4 * DC; ++b) {
+                const v4i vh = values[(b >> 1) * 128 + (b & 1) * 16], vl = values[(b >> 1) * 128 + (b & 1) * 16 + 64];
+                hh[b] = mfma(vh, eh, hh[b]);
+                mid[b] = mfma(vh, el, mid[b]);
+                ll[b] = mfma(vl, el, ll[b]);
+                mid[b] = mfma(vl, eh, mid[b]);
+            }
+        }
+        if (mine) {
+            atomicAdd(&totals[lane & 15], static_cast<unsigned long long>(static_cast<int64_t>(256 * sum_h + sum_l)));
+#pragma unroll
+            for (int b = 0; b < 4 * DC; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    atomicAdd(&sums[(lane & 15) * 64 * DC + 16 * b + 4 * (lane >> 4) + r],
+                              static_cast<unsigned long long>(join(hh[b][r], mid[b][r], ll[b][r])));
+        }
+        __syncthreads();
+        if constexpr (PASS == VALUES) {
+            if (from < to) {
+                for (int i = threadIdx.x; i < cols * 64 * DC; i += 64 * FEW_WAVES) atomicAdd(unit_sums + i, sums[i]);
+                if (threadIdx.x < cols) atomicAdd(unit_sums + FEW * 64 * DC + threadIdx.x, totals[threadIdx.x]);
+            }
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0)
+                final = atomicAdd(unit_sums + FEW * (64 * DC + 1), 1ull) == static_cast<unsigned>(f.splits) - 1;
+            __syncthreads();
+            if (!final) return;
+            __threadfence();
+            for (int i = threadIdx.x; i < cols * 64 * DC; i += 64 * FEW_WAVES)
+                sums[i] = __hip_atomic_load(unit_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (threadIdx.x < cols)
+                totals[threadIdx.x] = __hip_atomic_load(unit_sums + FEW * 64 * DC + threadIdx.x, __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+        }
+        // four places a thread
+        for (int i = threadIdx.x; i < cols * 16 * DC; i += 64 * FEW_WAVES) {
+            const int col = i / (16 * DC), place = i % (16 * DC) * 4;
+            if (place >= a.dim) continue;
+            const int token = (row0 + col) / a.group, member = row0 + col - token * a.group;
+            int64_t four[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) four[r] = static_cast<int64_t>(sums[col * 64 * DC + place + r]);
+            store4(a.out + (static_cast<size_t>(s.row) + token) * a.out_stride +
+                       (static_cast<size_t>(head) * a.group + member) * a.dim + place,
+                   a.dim - place, four, static_cast<int64_t>(totals[col]));
+        }
+    }
+}
+
 // Sequences in groups of FX_SEQS with work items counted by `items`; one launch each.
 template <class Items, class Launch>
 int each_group(Context* c, const FxSeq* seqs, size_t count, Items&& items, Launch&& launch) {
@@ -469,6 +701,46 @@ int each_group(Context* c, const FxSeq* seqs, size_t count, Items&& items, Launc
         VMX_HIP(c, hipGetLastError());
     }
     return 0;
+}
+
+template <int DC>
+int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::vector<FxSeq>& seqs, bool fused) {
+    return each_group(
+        c, seqs.data(), seqs.size(), [&](const FxSeq& s) { return (s.count * a.group + FEW - 1) / FEW; },
+        [&](const Seqs& q, uint32_t total) {
+            const dim3 grid(total, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(f.splits));
+            const dim3 threads(64 * FEW_WAVES);
+            if (fused) {
+                hipLaunchKernelGGL((fx_attention_few_kernel<DC, FUSED>), grid, threads,
+                                   static_cast<unsigned>(f.max_tiles * f.cols * 256), c->stream, a, f, q);
+            } else {
+                hipLaunchKernelGGL((fx_attention_few_kernel<DC, SCORES>), grid, threads, 0, c->stream, a, f, q);
+                hipLaunchKernelGGL((fx_attention_few_kernel<DC, VALUES>), grid, threads, 0, c->stream, a, f, q);
+            }
+        });
+}
+
+// 1 where its space may not grow: the other kernel needs none.
+int few_rows(Context* c, const AttentionArgs& a, const std::vector<FxSeq>& seqs, size_t tiles, size_t cols,
+             size_t units) {
+    FewArgs f{};
+    f.cols = static_cast<int>(cols);
+    f.max_tiles = static_cast<int>(std::max<size_t>(tiles, 1));
+    f.splits = 1;
+    const size_t score_bytes = f.max_tiles * cols * 256;
+    const bool fused = score_bytes <= 65536 && (tiles <= 2 * FEW_WAVES || units >= static_cast<size_t>(c->cu_count));
+    if (!fused) {
+        const size_t want = (2 * c->cu_count + units - 1) / units, most = (tiles + FEW_WAVES - 1) / FEW_WAVES;
+        f.splits = static_cast<int>(std::max<size_t>(1, std::min(want, most)));
+        // every group of sequences reuses the space: its launches are in order
+        const size_t z = units * score_bytes, tops = units * f.splits * FEW * 4;
+        const size_t sums = units * static_cast<size_t>(a.dim <= 64 ? FEW_SUMS<1> : FEW_SUMS<2>) * 8;
+        if (!try_ws(c, WS_FIXED, sums + 16 + z + tops)) return 1;
+        f.sums = ws<unsigned long long>(c, WS_FIXED);
+        f.z = reinterpret_cast<int*>(ws<unsigned char>(c, WS_FIXED) + (sums + 15) / 16 * 16);
+        f.tops = f.z + z / 4;
+    }
+    return a.dim <= 64 ? launch_few<1>(c, a, f, seqs, fused) : launch_few<2>(c, a, f, seqs, fused);
 }
 
 }  // namespace
@@ -506,8 +778,26 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
                           s1,
                           t.shift - s1,
                           t.causal};
+    std::vector<FxSeq> many, few;
+    size_t tiles = 0, cols = 0, units = 0;
+    for (size_t i = 0; i < count; ++i) {
+        const FxSeq& s = seqs[i];
+        if (s.count * group > FEW) {
+            many.push_back(s);
+            continue;
+        }
+        few.push_back(s);
+        tiles = std::max<size_t>(tiles, (s.length + FX_TILE - 1) / FX_TILE);
+        cols = std::max<size_t>(cols, std::min<size_t>(s.count * group, FEW));
+        units += (s.count * group + FEW - 1) / FEW * cache.kv_heads;
+    }
+    if (!few.empty()) {
+        const int rc = few_rows(c, a, few, tiles, cols, units);
+        if (rc < 0) return -1;
+        if (rc) many.assign(seqs, seqs + count);
+    }
     return each_group(
-        c, seqs, count, [&](const FxSeq& s) { return (s.count * group + 127) / 128; },
+        c, many.data(), many.size(), [&](const FxSeq& s) { return (s.count * group + 127) / 128; },
         [&](const Seqs& q, uint32_t total) {
             const dim3 grid(total, static_cast<unsigned>(cache.kv_heads));
             if (cache.dim <= 64)
