@@ -247,13 +247,16 @@ __device__ inline v16i scores(const unsigned char* keys, const int* extra, const
                               uint32_t s1, uint32_t s2, bool plain) {
     v16i hh = {}, mid = {}, ll = {};
     const v4i* p = reinterpret_cast<const v4i*>(keys) + block * 2 * DC * 128 + lane;
+    v4i kh[2 * DC], kl[2 * DC];
+#pragma unroll
+    for (int u = 0; u < 2 * DC; ++u) kh[u] = p[u * 128], kl[u] = p[u * 128 + 64];
+    __builtin_amdgcn_sched_barrier(0);  // all reads first: one wait for LDS, not one a step
 #pragma unroll
     for (int u = 0; u < 2 * DC; ++u) {
-        const v4i kh = p[u * 128], kl = p[u * 128 + 64];
-        hh = mfma32(kh, q.h[u], hh);
-        mid = mfma32(kh, q.l[u], mid);
-        ll = mfma32(kl, q.l[u], ll);
-        mid = mfma32(kl, q.h[u], mid);
+        hh = mfma32(kh[u], q.h[u], hh);
+        mid = mfma32(kh[u], q.l[u], mid);
+        ll = mfma32(kl[u], q.l[u], ll);
+        mid = mfma32(kl[u], q.h[u], mid);
     }
     if (!plain) {
 #pragma unroll
@@ -277,87 +280,132 @@ __device__ inline v16i scores(const unsigned char* keys, const int* extra, const
 // e (at most 2^14) as its two signed bytes: high in bits 15..8, low in bits 7..0.
 __device__ inline uint32_t encoded(uint32_t e) { return halves(static_cast<int>(min(e, 16384u))); }
 
-// out[d .. d + 3] of a row from sum e (v - 128) and sum e.
-__device__ inline void store4(int16_t* p, int live, const int64_t* sums, int64_t total) {
-    const double below = 2.0 * static_cast<double>(total), inv = total ? 1.0 / below : 0.0;
-    union {
-        uint2 v;
-        int16_t e[4];
-    } u;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const double num = static_cast<double>(2 * (sums[r] + 128 * total) + total);
-        u.e[r] = total ? static_cast<int16_t>(floor_div(num, below, inv)) : 0;
+// Results of a row from its sums, 0 where sum e is 0: a = 2 sum e (v - 128), less
+// than 2^50 and so exact in a double.
+struct Divide {
+    double below, inv, add;
+    __device__ explicit Divide(int64_t total)
+        : below(2.0 * static_cast<double>(total)), inv(total ? 1.0 / below : 0.0), add(257.0 * static_cast<double>(total)) {}
+    __device__ int operator()(double a) const {
+        return inv == 0.0 ? 0 : static_cast<int>(floor_div(a + add, below, inv));
     }
+};
+
+__device__ inline double twice(int hh, int mid, int ll) {
+    return __builtin_fma(hh, 131072.0, __builtin_fma(mid, 512.0, 2.0 * ll));
+}
+
+__device__ inline void store4(int16_t* p, int live, const int* v) {
     if (live >= 4) {
-        reinterpret_cast<Row8*>(p)->v = u.v;
+        reinterpret_cast<Row8*>(p)->v =
+            make_uint2((v[0] & 0xffff) | v[1] << 16, (v[2] & 0xffff) | v[3] << 16);
     } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (r < live) p[r] = u.e[r];
+            if (r < live) p[r] = static_cast<int16_t>(v[r]);
+    }
+}
+
+// Entries of the exponential table to LDS, encoded; the rest of it is not read.
+__device__ inline void load_table(const uint16_t* from, int entries, uint16_t* to, int thread, int threads) {
+    typedef unsigned short v2u __attribute__((ext_vector_type(2)));
+    for (int i = thread * 8; i < entries; i += threads * 8) {
+        if (i + 8 <= entries) {
+            v4i v = load8(reinterpret_cast<const int16_t*>(from) + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int pair = v[k];
+                const v2u e = __builtin_elementwise_min(__builtin_bit_cast(v2u, pair), v2u{16384, 16384});
+                const v2u up = e + v2u{128, 128};
+                v[k] = (__builtin_bit_cast(int, up) & 0xff00ff00) | (__builtin_bit_cast(int, e) & 0x00ff00ff);
+            }
+            *reinterpret_cast<v4i*>(to + i) = v;
+        } else {
+            for (int k = i; k < entries; ++k) to[k] = static_cast<uint16_t>(encoded(from[k]));
+        }
     }
 }
 
 // Many rows: a workgroup takes 128 rows of a sequence and key head, 32 for each
 // group of DC waves, and goes over the tiles of 64 tokens twice: for the
-// maximum, then for the sums.  Records come to LDS by direct copies, one tile
-// ahead.  With heads over 64 (DC = 2) the two waves of a group take 32 tokens of
-// a tile each, exchange the exponentials through LDS, and keep half of the
-// result's places each: 96 accumulators a lane either way.
+// maximum, then for the sums.  Keys and values come to LDS by direct copies,
+// three tiles ahead in the first pass, two (DC = 1) or two phases (DC = 2) in the
+// second.
+//
+// With heads over 64 (DC = 2) the two waves of a group take 32 tokens of a tile
+// each, exchange the exponentials through LDS, and keep half of the result's
+// places each: 96 accumulators a lane either way.  The second pass then has two
+// phases a tile, scores with exponentials and the sums; the two halves of the
+// workgroup run one phase apart, so that a SIMD's two waves are never both at
+// the vector work.
 template <int DC>
 __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs a, Seqs q) {
-    constexpr int WAVES = 4 * DC, STAGE = Record<DC>::BYTES;
-    __shared__ __attribute__((aligned(1024))) unsigned char stages[2][(STAGE + 1023) / 1024 * 1024];
+    constexpr int WAVES = 4 * DC, PART = Record<DC>::VALUES;  // bytes of a tile's keys, and of its values
+    constexpr int PARTS = DC == 1 ? 6 : 4, RING = 4;
+    __shared__ __attribute__((aligned(1024))) unsigned char parts[PARTS][PART];
+    __shared__ __attribute__((aligned(16))) int extras[RING][64];
     __shared__ __attribute__((aligned(16))) uint16_t table[FX_TABLE_MAX];
     __shared__ __attribute__((aligned(16))) v4i swap[DC == 2 ? WAVES * 128 : 1];
     __shared__ int share[WAVES][32];
-    const uint32_t at = sequence_of(q, blockIdx.x);
+    // heads vary fastest: an XCD gets few of them, and their keys stay in its L2
+    const uint32_t item = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
+    const uint32_t at = sequence_of(q, item);
     const FxSeq s = q.s[at];
-    const int lane = threadIdx.x & 63, head = blockIdx.y;
+    const int lane = threadIdx.x & 63, head = static_cast<int>(blockIdx.x - item * static_cast<uint32_t>(a.kv_heads));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave / DC, part = wave % DC;
     const int rows = static_cast<int>(s.count) * a.group;
     // the longest tiles first
-    const int row0 = static_cast<int>(q.first[at + 1] - 1 - blockIdx.x) * 128;
+    const int row0 = static_cast<int>(q.first[at + 1] - 1 - item) * 128;
     const int row = row0 + group * 32 + (lane & 31);
-    const unsigned char* base =
-        a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles * static_cast<size_t>(STAGE);
+    const unsigned char* base = a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles *
+                                             static_cast<size_t>(Record<DC>::BYTES);
+    const int limit = limit_of(a, s, min(row, rows - 1));
+    // what all rows of the wave see, what any of them does, and any of the workgroup's
+    const int all = limit_of(a, s, min(row0 + group * 32, rows - 1));
+    const int some = row0 + group * 32 < rows ? limit_of(a, s, min(row0 + group * 32 + 31, rows - 1)) : 0;
+    const int tiles = (limit_of(a, s, min(row0 + 127, rows - 1)) + FX_TILE - 1) / FX_TILE;
+
+    // A wave's share of a tile's keys with its extras (KEYS instructions), or of its values (VALUES).
+    constexpr int VALUES_COPIES = 2, KEYS_COPIES = 3;
+    auto stage_keys = [&](int t, unsigned char* to, int* extra) {
+        const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES;
+        copy_to_lds(rec + wave * 1024, lane * 16, to + wave * 1024);
+        copy_to_lds(rec + (WAVES + wave) * 1024, lane * 16, to + (WAVES + wave) * 1024);
+        if (lane < 16) copy_to_lds(rec + Record<DC>::EXTRA, lane * 16, extra);  // every wave the same
+    };
+    auto stage_values = [&](int t, unsigned char* to) {
+        const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES + Record<DC>::VALUES;
+        copy_to_lds(rec + wave * 1024, lane * 16, to + wave * 1024);
+        copy_to_lds(rec + (WAVES + wave) * 1024, lane * 16, to + (WAVES + wave) * 1024);
+    };
+#pragma unroll
+    for (int t = 0; t < RING - 1; ++t)
+        if (t < tiles) stage_keys(t, parts[t], extras[t]);
     Query<DC> mine;
     load_query<DC>(a, s, head, row, lane, &mine);
     const bool no_offset = !__any(mine.o);
-    const int limit = limit_of(a, s, min(row, rows - 1));
-    // what all rows of the wave see, and what one of the workgroup's sees
-    const int all = limit_of(a, s, min(row0 + group * 32, rows - 1));
-    const int tiles = (limit_of(a, s, min(row0 + 127, rows - 1)) + FX_TILE - 1) / FX_TILE;
-    for (uint32_t i = threadIdx.x; i < a.entries; i += 64 * WAVES)
-        table[i] = static_cast<uint16_t>(encoded(a.table[i]));
+    load_table(a.table, static_cast<int>(a.entries), table, threadIdx.x, 64 * WAVES);
     const uint32_t last = a.entries - 1;
-
-    auto stage = [&](int t, int pieces, unsigned char* to) {
-        const unsigned char* rec = base + static_cast<size_t>(t) * STAGE;
-        for (int p = wave; p < pieces; p += WAVES) copy_to_lds(rec + p * 1024, lane * 16, to + p * 1024);
-        if (wave == 0 && lane < 16) copy_to_lds(rec + Record<DC>::EXTRA, lane * 16, to + Record<DC>::EXTRA);
-    };
-    // Runs `use` on every tile's record in LDS, `pieces` KiB of it and its extras.
-    auto over_tiles = [&](int pieces, auto&& use) {
-        if (tiles > 0) stage(0, pieces, stages[0]);
-        for (int t = 0; t < tiles; ++t) {
-            lds_copies_done<0>();
-            __syncthreads();  // this tile has landed for all waves, and all have left the other buffer
-            if (t + 1 < tiles) stage(t + 1, pieces, stages[(t + 1) & 1]);
-            const unsigned char* rec = stages[t & 1];
-            const int* extra = reinterpret_cast<const int*>(rec + Record<DC>::EXTRA);
-            const bool offset = lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128);
-            use(t, rec, extra, no_offset && !__any(offset));
-        }
-        __syncthreads();
+    auto is_plain = [&](int t, const int* extra) {
+        return no_offset && !__any(lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128));
     };
 
     int top = INT_MIN;
-    over_tiles(8 * DC, [&](int t, const unsigned char* rec, const int* extra, bool plain) {
+    for (int t = 0; t < tiles; ++t) {
+        if (t + RING - 2 < tiles)
+            lds_copies_done<(RING - 2) * KEYS_COPIES>();
+        else
+            lds_copies_done<0>();
+        __syncthreads();  // this tile has landed for all waves, and all have left the one before
+        if (t + RING - 1 < tiles) stage_keys(t + RING - 1, parts[(t + RING - 1) % RING], extras[(t + RING - 1) % RING]);
+        const unsigned char* keys = parts[t % RING];
+        const int* extra = extras[t % RING];
+        const bool plain = is_plain(t, extra);
 #pragma unroll
         for (int b = 0; b < 2 / DC; ++b) {
             const int block = DC == 2 ? part : b, token = t * FX_TILE + block * 32;
-            const v16i z = scores<DC>(rec, extra, mine, block, lane, a.s1, a.s2, plain);
+            if (token >= some) continue;
+            const v16i z = scores<DC>(keys, extra, mine, block, lane, a.s1, a.s2, plain);
             if (token + 32 <= all) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = max(top, z[r]);
@@ -367,71 +415,139 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
                     if (token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) < limit) top = max(top, z[r]);
             }
         }
-    });
+    }
     top = max(top, __shfl_xor(top, 32));
     if constexpr (DC == 2) {
         if (lane < 32) share[wave][lane] = top;
         __syncthreads();
         top = max(top, share[wave ^ 1][lane & 31]);
-        __syncthreads();
     }
+    __syncthreads();  // the first pass's buffers are free
 
     v16i hh[2] = {}, mid[2] = {}, ll[2] = {};  // 32 places each, of this wave's 64
     int sum_h = 0, sum_l = 0;
-    over_tiles(16 * DC, [&](int t, const unsigned char* rec, const int* extra, bool plain) {
-        const v4i* values = reinterpret_cast<const v4i*>(rec + Record<DC>::VALUES) + lane;
-        auto add = [&](int block, v4i eh, v4i el) {
+    // exponentials of 32 tokens
+    auto exponentials = [&](const unsigned char* keys, const int* extra, int block, int token, bool plain, v4i* eh,
+                            v4i* el) {
+        const v16i z = scores<DC>(keys, extra, mine, block, lane, a.s1, a.s2, plain);
+        uint32_t e[16];
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                const v4i* p = values + (block * 2 * DC + part * 2 + d) * 128;
-                const v4i vh = p[0], vl = p[64];
-                hh[d] = mfma32(vh, eh, hh[d]);
-                mid[d] = mfma32(vh, el, mid[d]);
-                ll[d] = mfma32(vl, el, ll[d]);
-                mid[d] = mfma32(vl, eh, mid[d]);
-            }
-        };
+        for (int r = 0; r < 16; ++r) e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[r]), last)];
+        if (token + 32 > all) {
 #pragma unroll
-        for (int b = 0; b < 2 / DC; ++b) {
-            const int block = DC == 2 ? part : b, token = t * FX_TILE + block * 32;
-            const v16i z = scores<DC>(rec, extra, mine, block, lane, a.s1, a.s2, plain);
-            v4i eh, el;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                uint32_t e[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[4 * g + r]), last)];
-                if (token + 32 > all) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (token + 8 * g + 4 * (lane >> 5) + r >= limit) e[r] = 0;
-                }
-                const uint32_t a01 = e[0] | e[1] << 16, a23 = e[2] | e[3] << 16;
-                eh[g] = __builtin_amdgcn_perm(a23, a01, 0x07050301u);
-                el[g] = __builtin_amdgcn_perm(a23, a01, 0x06040200u);
-                sum_h = __builtin_amdgcn_sdot4(eh[g], 0x01010101, sum_h, false);
-                sum_l = __builtin_amdgcn_sdot4(el[g], 0x01010101, sum_l, false);
-            }
-            if constexpr (DC == 1) {
-                add(block, eh, el);
-            } else {
-                swap[wave * 128 + lane] = eh;
-                swap[wave * 128 + 64 + lane] = el;
-            }
+            for (int r = 0; r < 16; ++r)
+                if (token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= limit) e[r] = 0;
         }
-        if constexpr (DC == 2) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const uint32_t a01 = e[4 * g] | e[4 * g + 1] << 16, a23 = e[4 * g + 2] | e[4 * g + 3] << 16;
+            (*eh)[g] = __builtin_amdgcn_perm(a23, a01, 0x07050301u);
+            (*el)[g] = __builtin_amdgcn_perm(a23, a01, 0x06040200u);
+            sum_h = __builtin_amdgcn_sdot4((*eh)[g], 0x01010101, sum_h, false);
+            sum_l = __builtin_amdgcn_sdot4((*el)[g], 0x01010101, sum_l, false);
+        }
+    };
+    // the 64 places' values of a block of 32 tokens
+    struct Values {
+        v4i h[2], l[2];
+    };
+    auto read = [&](const unsigned char* values, int block) {
+        Values v;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const v4i* p = reinterpret_cast<const v4i*>(values) + (block * 2 * DC + part * 2 + d) * 128 + lane;
+            v.h[d] = p[0];
+            v.l[d] = p[64];
+        }
+        return v;
+    };
+    auto add = [&](const Values& v, v4i eh, v4i el) {
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            hh[d] = mfma32(v.h[d], eh, hh[d]);
+            mid[d] = mfma32(v.h[d], el, mid[d]);
+            ll[d] = mfma32(v.l[d], el, ll[d]);
+            mid[d] = mfma32(v.l[d], eh, mid[d]);
+        }
+    };
+    if constexpr (DC == 1) {
+        constexpr int AHEAD = 2;  // tiles, of three in LDS
+#pragma unroll
+        for (int t = 0; t < AHEAD; ++t)
+            if (t < tiles) stage_keys(t, parts[2 * t], extras[t]), stage_values(t, parts[2 * t + 1]);
+        int now = 0;
+        for (int t = 0; t < tiles; ++t) {
+            if (t + 1 < tiles)
+                lds_copies_done<KEYS_COPIES + VALUES_COPIES>();
+            else
+                lds_copies_done<0>();
             __syncthreads();
+            if (t + AHEAD < tiles) {
+                const int next = now == 0 ? 2 : now - 1;
+                stage_keys(t + AHEAD, parts[2 * next], extras[next]);
+                stage_values(t + AHEAD, parts[2 * next + 1]);
+            }
+            const bool plain = is_plain(t, extras[now]);
 #pragma unroll
             for (int block = 0; block < 2; ++block) {
-                const v4i* p = swap + (group * 2 + block) * 128 + lane;
-                add(block, p[0], p[64]);
+                const int token = t * FX_TILE + block * 32;
+                if (token >= some) continue;
+                v4i eh, el;
+                exponentials(parts[2 * now], extras[now], block, token, plain, &eh, &el);
+                add(read(parts[2 * now + 1], block), eh, el);
             }
+            now = now == 2 ? 0 : now + 1;
         }
-    });
+    } else {
+        // Keys in parts 0 and 1, values in parts 2 and 3.  Phase 2 t has the first
+        // half's scores of tile t and the second half's sums of tile t - 1, phase
+        // 2 t + 1 the other way round.  At its start keys (even) or values (odd) of
+        // tile t + 1 go where those of t - 1 were, which all have left by then;
+        // they are waited for two phases later.
+        constexpr int COPIES = 3;
+        auto stage = [&](int t, int odd) {
+            const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES;
+            const unsigned char* from = rec + (odd ? Record<DC>::VALUES : 0) + wave * 1024;
+            unsigned char* to = parts[2 * odd + (t & 1)] + wave * 1024;
+            copy_to_lds(from, lane * 16, to);
+            copy_to_lds(from + WAVES * 1024, lane * 16, to + WAVES * 1024);
+            if (lane < 16) copy_to_lds(rec + Record<DC>::EXTRA, lane * 16, extras[t & 1]);
+        };
+        auto begin = [&](int phase) {
+            const int t = phase >> 1, odd = phase & 1;
+            if (t + odd < tiles)
+                lds_copies_done<COPIES>();
+            else
+                lds_copies_done<0>();
+            __syncthreads();
+            if (t + 1 < tiles) stage(t + 1, odd);
+        };
+        if (tiles > 0) stage(0, 0), stage(0, 1);
+        const int behind = group >> 1;
+        int phase = 0;
+        if (behind) begin(phase++);
+        for (int t = 0; t < tiles; ++t) {
+            begin(phase++);
+            const int token = t * FX_TILE + part * 32;
+            v4i eh = {}, el = {};
+            if (token < some)
+                exponentials(parts[t & 1], extras[t & 1], part, token, is_plain(t, extras[t & 1]), &eh, &el);
+            swap[wave * 128 + lane] = eh;
+            swap[wave * 128 + 64 + lane] = el;
+            begin(phase++);
+            const v4i* p = swap + group * 256 + lane;
+            const v4i e0h = p[0], e0l = p[64], e1h = p[128], e1l = p[192];
+            const Values v0 = read(parts[2 + (t & 1)], 0), v1 = read(parts[2 + (t & 1)], 1);
+            __builtin_amdgcn_sched_barrier(0);
+            add(v0, e0h, e0l);
+            add(v1, e1h, e1l);
+        }
+        if (!behind) begin(phase++);
+    }
     int total = 256 * sum_h + sum_l;
     total += __shfl_xor(total, 32);
     if constexpr (DC == 2) {
+        __syncthreads();
         if (lane < 32) share[wave][lane] = total;
         __syncthreads();
         total += share[wave ^ 1][lane & 31];
@@ -440,16 +556,17 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
     const int token = row / a.group, member = row - token * a.group;
     int16_t* out = a.out + (static_cast<size_t>(s.row) + token) * a.out_stride +
                    (static_cast<size_t>(head) * a.group + member) * a.dim;
+    const Divide divide(total);
 #pragma unroll
     for (int d = 0; d < 2; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int place = part * 64 + d * 32 + 8 * g + 4 * (lane >> 5);
             if (place >= a.dim) continue;
-            int64_t sums[4];
+            int v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sums[r] = join(hh[d][4 * g + r], mid[d][4 * g + r], ll[d][4 * g + r]);
-            store4(out + place, a.dim - place, sums, total);
+            for (int r = 0; r < 4; ++r) v[r] = divide(twice(hh[d][4 * g + r], mid[d][4 * g + r], ll[d][4 * g + r]));
+            store4(out + place, a.dim - place, v);
         }
 }
 
@@ -674,12 +791,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
             const int col = i / (16 * DC), place = i % (16 * DC) * 4;
             if (place >= a.dim) continue;
             const int token = (row0 + col) / a.group, member = row0 + col - token * a.group;
-            int64_t four[4];
+            int v[4];
+            const Divide divide(static_cast<int64_t>(totals[col]));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) four[r] = static_cast<int64_t>(sums[col * 64 * DC + place + r]);
+            for (int r = 0; r < 4; ++r)
+                v[r] = divide(2.0 * static_cast<double>(static_cast<int64_t>(sums[col * 64 * DC + place + r])));
             store4(a.out + (static_cast<size_t>(s.row) + token) * a.out_stride +
                        (static_cast<size_t>(head) * a.group + member) * a.dim + place,
-                   a.dim - place, four, static_cast<int64_t>(totals[col]));
+                   a.dim - place, v);
         }
     }
 }
@@ -799,7 +918,7 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
     return each_group(
         c, many.data(), many.size(), [&](const FxSeq& s) { return (s.count * group + 127) / 128; },
         [&](const Seqs& q, uint32_t total) {
-            const dim3 grid(total, static_cast<unsigned>(cache.kv_heads));
+            const dim3 grid(total * static_cast<unsigned>(cache.kv_heads));
             if (cache.dim <= 64)
                 hipLaunchKernelGGL(fx_attention_kernel<1>, grid, dim3(256), 0, c->stream, a, q);
             else
