@@ -30,7 +30,7 @@ using namespace fx;
 
 struct Seqs {
     FxSeq s[FX_SEQS];
-    uint32_t first[FX_SEQS + 1];  // work items before each sequence
+    uint32_t first[FX_SEQS + 1];  // work items before each sequence (of each, for many rows)
     uint32_t count;
 };
 
@@ -348,14 +348,22 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
     __shared__ __attribute__((aligned(16))) v4i swap[DC == 2 ? WAVES * 128 : 1];
     __shared__ int share[WAVES][32];
     // heads vary fastest: an XCD gets few of them, and their keys stay in its L2
-    const uint32_t item = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
-    const uint32_t at = sequence_of(q, item);
-    const FxSeq s = q.s[at];
+    uint32_t item = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
     const int lane = threadIdx.x & 63, head = static_cast<int>(blockIdx.x - item * static_cast<uint32_t>(a.kv_heads));
+    // The longest work first: first[] holds the sequences' counts of 128 rows,
+    // falling; the last such place of all sequences comes first, then the one
+    // before it, each with the sequences that reach it.
+    uint32_t reach = 0, place = 0;
+    for (;; ++reach) {
+        const uint32_t here = (q.first[reach] - q.first[reach + 1]) * (reach + 1);
+        if (item < here) break;
+        item -= here;
+    }
+    place = q.first[reach] - 1 - item / (reach + 1);
+    const FxSeq s = q.s[item % (reach + 1)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave / DC, part = wave % DC;
     const int rows = static_cast<int>(s.count) * a.group;
-    // the longest tiles first
-    const int row0 = static_cast<int>(q.first[at + 1] - 1 - item) * 128;
+    const int row0 = static_cast<int>(place) * 128;
     const int row = row0 + group * 32 + (lane & 31);
     const unsigned char* base = a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles *
                                              static_cast<size_t>(Record<DC>::BYTES);
@@ -915,9 +923,12 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
         if (rc < 0) return -1;
         if (rc) many.assign(seqs, seqs + count);
     }
+    auto items = [&](const FxSeq& s) { return (s.count * group + 127) / 128; };
+    std::sort(many.begin(), many.end(), [&](const FxSeq& x, const FxSeq& y) { return items(x) > items(y); });
     return each_group(
-        c, many.data(), many.size(), [&](const FxSeq& s) { return (s.count * group + 127) / 128; },
-        [&](const Seqs& q, uint32_t total) {
+        c, many.data(), many.size(), items, [&](Seqs& q, uint32_t total) {
+            for (uint32_t i = 0; i < q.count; ++i) q.first[i] = items(q.s[i]);
+            q.first[q.count] = 0;
             const dim3 grid(total * static_cast<unsigned>(cache.kv_heads));
             if (cache.dim <= 64)
                 hipLaunchKernelGGL(fx_attention_kernel<1>, grid, dim3(256), 0, c->stream, a, q);
