@@ -585,9 +585,8 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
 // needs the maximum over the whole run:
 //   FUSED   one workgroup has all tiles: kept in LDS, one launch;
 //   SCORES, VALUES   the tiles are split over `splits` workgroups: kept in memory,
-//           with a maximum per split, between two launches.  The second adds its
-//           sums to the unit's (integers: any order gives the same), and the last
-//           workgroup of a unit to arrive divides.  The first clears them.
+//           with a maximum per split, between two launches; a third adds the
+//           splits' sums (integers: any order gives the same) and divides.
 enum Pass { FUSED, SCORES, VALUES };
 constexpr int FEW = 16, FEW_WAVES = 8;
 
@@ -595,13 +594,10 @@ struct FewArgs {
     int cols;       // rows of a unit that scores are kept for, at most FEW
     int max_tiles;  // of a sequence
     int splits;
-    int* z;                   // units x max_tiles x cols x 64
-    int* tops;                // units x splits x FEW
-    unsigned long long* sums;  // units x (FEW x head, FEW totals, arrivals)
+    int* z;        // units x max_tiles x cols x 64
+    int* tops;     // units x splits x FEW
+    int64_t* sums;  // units x splits x cols x (head + 1): sum e (v - 128), sum e
 };
-
-template <int DC>
-constexpr int FEW_SUMS = FEW * (64 * DC + 1) + 1;
 
 // A lane's query for 16 x 16 products: row lane & 15, 16 of 64 places from 16 (lane >> 4).
 template <int DC>
@@ -616,16 +612,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
     __shared__ unsigned long long sums[PASS == SCORES ? 1 : FEW * 64 * DC];
     __shared__ unsigned long long totals[FEW];
     __shared__ int tops[FEW_WAVES][FEW];
-    __shared__ bool final;
-    const uint32_t at = sequence_of(q, blockIdx.x);
+    const uint32_t item = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
+    const uint32_t at = sequence_of(q, item);
     const FxSeq s = q.s[at];
-    const int lane = threadIdx.x & 63, head = blockIdx.y, split = blockIdx.z;
+    const int lane = threadIdx.x & 63, head = static_cast<int>(blockIdx.x - item * static_cast<uint32_t>(a.kv_heads));
+    const int split = blockIdx.y;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rows = static_cast<int>(s.count) * a.group;
-    const int row0 = static_cast<int>(blockIdx.x - q.first[at]) * FEW, row = row0 + (lane & 15);
+    const int row0 = static_cast<int>(item - q.first[at]) * FEW, row = row0 + (lane & 15);
     const int cols = min(rows - row0, FEW);  // at most f.cols
     const bool mine = (lane & 15) < cols;
-    const size_t unit = static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+    const size_t unit = blockIdx.x;
     const unsigned char* base =
         a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles * static_cast<size_t>(Record<DC>::BYTES);
     const int limit = limit_of(a, s, min(row, rows - 1)), all = limit_of(a, s, row0);
@@ -635,14 +632,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
     int* z_of = PASS == FUSED ? kept : f.z + unit * f.max_tiles * f.cols * 64;
     // this lane's token in place r of its quarter t of a tile: first + 8 t + r
     const int first = 32 * (lane >> 5) + 4 * ((lane >> 4) & 1);
-    unsigned long long* unit_sums = f.sums + unit * FEW_SUMS<DC>;
 
     int top = INT_MIN;
     if constexpr (PASS != VALUES) {
-        if constexpr (PASS == SCORES) {
-            if (split == 0)
-                for (int i = threadIdx.x; i < FEW_SUMS<DC>; i += 64 * FEW_WAVES) unit_sums[i] = 0;
-        }
         FewQuery<DC> mq;
         {
             const int token = mine ? row / a.group : 0, member = mine ? row - token * a.group : 0;
@@ -776,23 +768,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
         }
         __syncthreads();
         if constexpr (PASS == VALUES) {
-            if (from < to) {
-                for (int i = threadIdx.x; i < cols * 64 * DC; i += 64 * FEW_WAVES) atomicAdd(unit_sums + i, sums[i]);
-                if (threadIdx.x < cols) atomicAdd(unit_sums + FEW * 64 * DC + threadIdx.x, totals[threadIdx.x]);
-            }
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0)
-                final = atomicAdd(unit_sums + FEW * (64 * DC + 1), 1ull) == static_cast<unsigned>(f.splits) - 1;
-            __syncthreads();
-            if (!final) return;
-            __threadfence();
+            constexpr int WIDTH = 64 * DC + 1;
+            int64_t* kept_sums = f.sums + (unit * f.splits + split) * f.cols * WIDTH;
             for (int i = threadIdx.x; i < cols * 64 * DC; i += 64 * FEW_WAVES)
-                sums[i] = __hip_atomic_load(unit_sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                kept_sums[i / (64 * DC) * WIDTH + i % (64 * DC)] = static_cast<int64_t>(sums[i]);
             if (threadIdx.x < cols)
-                totals[threadIdx.x] = __hip_atomic_load(unit_sums + FEW * 64 * DC + threadIdx.x, __ATOMIC_RELAXED,
-                                                        __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
+                kept_sums[threadIdx.x * WIDTH + 64 * DC] = static_cast<int64_t>(totals[threadIdx.x]);
+            return;
         }
         // four places a thread
         for (int i = threadIdx.x; i < cols * 16 * DC; i += 64 * FEW_WAVES) {
@@ -808,6 +790,37 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
                        (static_cast<size_t>(head) * a.group + member) * a.dim + place,
                    a.dim - place, v);
         }
+    }
+}
+
+// The splits' sums of a unit, added and divided: a workgroup a unit, four places a thread.
+template <int DC>
+__global__ __launch_bounds__(256) void fx_attention_join_kernel(AttentionArgs a, FewArgs f, Seqs q) {
+    constexpr int WIDTH = 64 * DC + 1;
+    const uint32_t item = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
+    const uint32_t at = sequence_of(q, item);
+    const FxSeq s = q.s[at];
+    const int head = static_cast<int>(blockIdx.x - item * static_cast<uint32_t>(a.kv_heads));
+    const int row0 = static_cast<int>(item - q.first[at]) * FEW;
+    const int cols = min(static_cast<int>(s.count) * a.group - row0, FEW);
+    for (int i = threadIdx.x; i < cols * 16 * DC; i += 256) {
+        const int col = i / (16 * DC), place = i % (16 * DC) * 4;
+        if (place >= a.dim) continue;
+        const int64_t* p = f.sums + (static_cast<size_t>(blockIdx.x) * f.splits * f.cols + col) * WIDTH;
+        int64_t total = 0, sums[4] = {};
+        for (int k = 0; k < f.splits; ++k, p += f.cols * WIDTH) {
+            total += p[64 * DC];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[r] += p[place + r];
+        }
+        const Divide divide(total);
+        int v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = divide(2.0 * static_cast<double>(sums[r]));
+        const int token = (row0 + col) / a.group, member = row0 + col - token * a.group;
+        store4(a.out + (static_cast<size_t>(s.row) + token) * a.out_stride +
+                   (static_cast<size_t>(head) * a.group + member) * a.dim + place,
+               a.dim - place, v);
     }
 }
 
@@ -835,7 +848,7 @@ int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::
     return each_group(
         c, seqs.data(), seqs.size(), [&](const FxSeq& s) { return (s.count * a.group + FEW - 1) / FEW; },
         [&](const Seqs& q, uint32_t total) {
-            const dim3 grid(total, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(f.splits));
+            const dim3 grid(total * static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(f.splits));
             const dim3 threads(64 * FEW_WAVES);
             if (fused) {
                 hipLaunchKernelGGL((fx_attention_few_kernel<DC, FUSED>), grid, threads,
@@ -843,13 +856,14 @@ int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::
             } else {
                 hipLaunchKernelGGL((fx_attention_few_kernel<DC, SCORES>), grid, threads, 0, c->stream, a, f, q);
                 hipLaunchKernelGGL((fx_attention_few_kernel<DC, VALUES>), grid, threads, 0, c->stream, a, f, q);
+                hipLaunchKernelGGL(fx_attention_join_kernel<DC>, dim3(grid.x), dim3(256), 0, c->stream, a, f, q);
             }
         });
 }
 
 // 1 where its space may not grow: the other kernel needs none.
-int few_rows(Context* c, const AttentionArgs& a, const std::vector<FxSeq>& seqs, size_t tiles, size_t cols,
-             size_t units) {
+int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_t tiles, size_t cols, size_t units) {
+    std::sort(seqs.begin(), seqs.end(), [](const FxSeq& x, const FxSeq& y) { return x.length > y.length; });
     FewArgs f{};
     f.cols = static_cast<int>(cols);
     f.max_tiles = static_cast<int>(std::max<size_t>(tiles, 1));
@@ -861,11 +875,11 @@ int few_rows(Context* c, const AttentionArgs& a, const std::vector<FxSeq>& seqs,
         f.splits = static_cast<int>(std::max<size_t>(1, std::min(want, most)));
         // every group of sequences reuses the space: its launches are in order
         const size_t z = units * score_bytes, tops = units * f.splits * FEW * 4;
-        const size_t sums = units * static_cast<size_t>(a.dim <= 64 ? FEW_SUMS<1> : FEW_SUMS<2>) * 8;
-        if (!try_ws(c, WS_FIXED, sums + 16 + z + tops)) return 1;
-        f.sums = ws<unsigned long long>(c, WS_FIXED);
-        f.z = reinterpret_cast<int*>(ws<unsigned char>(c, WS_FIXED) + (sums + 15) / 16 * 16);
-        f.tops = f.z + z / 4;
+        const size_t sums = units * f.splits * cols * (a.dim <= 64 ? 65 : 129) * 8;
+        if (!try_ws(c, WS_FIXED, z + sums + tops)) return 1;
+        f.z = ws<int>(c, WS_FIXED);
+        f.sums = reinterpret_cast<int64_t*>(ws<unsigned char>(c, WS_FIXED) + z);
+        f.tops = reinterpret_cast<int*>(ws<unsigned char>(c, WS_FIXED) + z + sums);
     }
     return a.dim <= 64 ? launch_few<1>(c, a, f, seqs, fused) : launch_few<2>(c, a, f, seqs, fused);
 }
