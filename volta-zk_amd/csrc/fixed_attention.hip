@@ -306,23 +306,26 @@ __device__ inline void store4(int16_t* p, int live, const int* v) {
     }
 }
 
-// Entries of the exponential table to LDS, encoded; the rest of it is not read.
-__device__ inline void load_table(const uint16_t* from, int entries, uint16_t* to, int thread, int threads) {
+// Eight entries of the exponential table, encoded.
+__device__ inline v4i encoded8(v4i v) {
     typedef unsigned short v2u __attribute__((ext_vector_type(2)));
-    for (int i = thread * 8; i < entries; i += threads * 8) {
-        if (i + 8 <= entries) {
-            v4i v = load8(reinterpret_cast<const int16_t*>(from) + i);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int pair = v[k];
-                const v2u e = __builtin_elementwise_min(__builtin_bit_cast(v2u, pair), v2u{16384, 16384});
-                const v2u up = e + v2u{128, 128};
-                v[k] = (__builtin_bit_cast(int, up) & 0xff00ff00) | (__builtin_bit_cast(int, e) & 0x00ff00ff);
-            }
-            *reinterpret_cast<v4i*>(to + i) = v;
-        } else {
+    for (int k = 0; k < 4; ++k) {
+        const int pair = v[k];
+        const v2u e = __builtin_elementwise_min(__builtin_bit_cast(v2u, pair), v2u{16384, 16384});
+        const v2u up = e + v2u{128, 128};
+        v[k] = (__builtin_bit_cast(int, up) & 0xff00ff00) | (__builtin_bit_cast(int, e) & 0x00ff00ff);
+    }
+    return v;
+}
+
+// The table to LDS, encoded; the rest of the space is not read.
+__device__ inline void load_table(const uint16_t* from, int entries, uint16_t* to, int thread, int threads) {
+    for (int i = thread * 8; i < entries; i += threads * 8) {
+        if (i + 8 <= entries)
+            *reinterpret_cast<v4i*>(to + i) = encoded8(load8(reinterpret_cast<const int16_t*>(from) + i));
+        else
             for (int k = i; k < entries; ++k) to[k] = static_cast<uint16_t>(encoded(from[k]));
-        }
     }
 }
 
@@ -580,15 +583,21 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
 
 // ---- few rows ----------------------------------------------------------------------------
 // A workgroup takes 16 rows of a sequence and key head and a run of its tiles;
-// its eight waves take the tiles in turn, straight from memory, and add their
-// sums in LDS.  Scores are computed once and kept for the second pass, which
-// needs the maximum over the whole run:
+// its waves take the tiles in turn, straight from memory, and add their sums in
+// LDS.  Scores are computed once and kept for the second pass, which needs the
+// maximum over the whole run:
+//   ONE     a tile a wave at most: kept in registers, with the wave's values
+//           and the table under way while the scores are computed;
 //   FUSED   one workgroup has all tiles: kept in LDS, one launch;
 //   SCORES, VALUES   the tiles are split over `splits` workgroups: kept in memory,
 //           with a maximum per split, between two launches; a third adds the
 //           splits' sums (integers: any order gives the same) and divides.
-enum Pass { FUSED, SCORES, VALUES };
-constexpr int FEW = 16, FEW_WAVES = 8;
+enum Pass { ONE, FUSED, SCORES, VALUES };
+constexpr int FEW = 16;
+
+// Waves of a workgroup: ONE has room for 16 with heads up to 64 (128 registers a lane).
+template <int DC, Pass PASS>
+constexpr int FEW_WAVES = PASS == ONE && DC == 1 ? 16 : 8;
 
 struct FewArgs {
     int cols;       // rows of a unit that scores are kept for, at most FEW
@@ -607,11 +616,13 @@ struct FewQuery {
 };
 
 template <int DC, Pass PASS>
-__global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(AttentionArgs a, FewArgs f, Seqs q) {
+__global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_kernel(AttentionArgs a, FewArgs f, Seqs q) {
+    constexpr int WAVES = FEW_WAVES<DC, PASS>, THREADS = 64 * WAVES;
     extern __shared__ __attribute__((aligned(16))) int kept[];  // FUSED: scores
+    __shared__ __attribute__((aligned(16))) uint16_t table[PASS == ONE ? FX_TABLE_MAX : 8];
     __shared__ unsigned long long sums[PASS == SCORES ? 1 : FEW * 64 * DC];
     __shared__ unsigned long long totals[FEW];
-    __shared__ int tops[FEW_WAVES][FEW];
+    __shared__ int tops[WAVES][FEW];
     const uint32_t item = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
     const uint32_t at = sequence_of(q, item);
     const FxSeq s = q.s[at];
@@ -625,15 +636,44 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
     const size_t unit = blockIdx.x;
     const unsigned char* base =
         a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles * static_cast<size_t>(Record<DC>::BYTES);
-    const int limit = limit_of(a, s, min(row, rows - 1)), all = limit_of(a, s, row0);
+    const int limit = limit_of(a, s, min(row, rows - 1));
     const int tiles = (limit_of(a, s, min(row0 + FEW, rows) - 1) + FX_TILE - 1) / FX_TILE;
     const int each = (f.max_tiles + f.splits - 1) / f.splits;
     const int from = split * each, to = min(from + each, tiles);
+    const uint32_t last = a.entries - 1;
     int* z_of = PASS == FUSED ? kept : f.z + unit * f.max_tiles * f.cols * 64;
     // this lane's token in place r of its quarter t of a tile: first + 8 t + r
     const int first = 32 * (lane >> 5) + 4 * ((lane >> 4) & 1);
+    // where its scores of tile t are kept
+    auto z_at = [&](int t) {
+        return z_of + ((PASS == FUSED ? t - from : t) * f.cols + (lane & 15)) * 64 + 4 * (lane >> 4);
+    };
+
+    // values of a tile: places 16 b + (lane & 15), half (lane >> 4) & 1 of 32-token block lane >> 5
+    const int in_values = ((lane >> 5) * 2 * DC) * 128 + (lane & 15) + 32 * ((lane >> 4) & 1);
+    struct Values {
+        v4i h[4 * DC], l[4 * DC];
+    };
+    auto read_values = [&](int t, Values* v) {
+        const v4i* p = reinterpret_cast<const v4i*>(base + static_cast<size_t>(t) * Record<DC>::BYTES + Record<DC>::VALUES) +
+                       in_values;
+#pragma unroll
+        for (int b = 0; b < 4 * DC; ++b) {
+            v->h[b] = p[(b >> 1) * 128 + (b & 1) * 16];
+            v->l[b] = p[(b >> 1) * 128 + (b & 1) * 16 + 64];
+        }
+    };
 
     int top = INT_MIN;
+    v4i z[4] = {};
+    Values ahead;
+    v4i entries = {};
+    if constexpr (PASS == ONE) {
+        if (wave < to) read_values(wave, &ahead);
+        const int i = threadIdx.x * 8;
+        if (THREADS * 8 >= static_cast<int>(FX_TABLE_MAX) && i + 8 <= static_cast<int>(a.entries))
+            entries = load8(reinterpret_cast<const int16_t*>(a.table) + i);
+    }
     if constexpr (PASS != VALUES) {
         FewQuery<DC> mq;
         {
@@ -662,7 +702,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
         // the key that this lane reads for row i = lane & 15 of quarter t: 8 t past
         // token 32 (i >> 3) + 4 ((i >> 2) & 1) + (i & 3)
         const int in_tile = (((lane >> 3) & 1) * 2 * DC + (lane >> 5)) * 128 + (lane & 7) + 32 * ((lane >> 4) & 1);
-        for (int t = from + wave; t < to; t += FEW_WAVES) {
+        for (int t = from + wave; t < to; t += WAVES) {
             const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES;
             const v4i* keys = reinterpret_cast<const v4i*>(rec) + in_tile;
             const int* extra = reinterpret_cast<const int*>(rec + Record<DC>::EXTRA);
@@ -689,58 +729,63 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
                                                     static_cast<uint32_t>((x >> 8) * mq.o));
                     }
             }
-            int* zt = z_of + ((PASS == FUSED ? t - from : t) * f.cols + (lane & 15)) * 64 + 4 * (lane >> 4);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                v4i z;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int low = static_cast<int>((static_cast<uint32_t>(mid[k][r]) << 8) + ll[k][r]);
-                    z[r] = ((hh[k][r] << (16 - a.s1)) + (low >> a.s1)) >> a.s2;
-                    if (t * FX_TILE + first + 8 * k + r < limit) top = max(top, z[r]);
+                    z[k][r] = ((hh[k][r] << (16 - a.s1)) + (low >> a.s1)) >> a.s2;
+                    if (t * FX_TILE + first + 8 * k + r < limit) top = max(top, z[k][r]);
                 }
-                if (mine) *reinterpret_cast<v4i*>(zt + 16 * k) = z;
+                if (PASS != ONE && mine) *reinterpret_cast<v4i*>(z_at(t) + 16 * k) = z[k];
             }
         }
         top = max(top, __shfl_xor(top, 16));
         top = max(top, __shfl_xor(top, 32));
         if (lane < FEW) tops[wave][lane] = top;
-        __syncthreads();
+        if constexpr (PASS == ONE) {
+            if constexpr (THREADS * 8 >= static_cast<int>(FX_TABLE_MAX)) {
+                const int i = threadIdx.x * 8;
+                if (i + 8 <= static_cast<int>(a.entries))
+                    *reinterpret_cast<v4i*>(table + i) = encoded8(entries);
+                else
+                    for (int k = i; k < static_cast<int>(a.entries); ++k) table[k] = static_cast<uint16_t>(encoded(a.table[k]));
+            } else {
+                load_table(a.table, static_cast<int>(a.entries), table, threadIdx.x, THREADS);
+            }
+        }
         if constexpr (PASS == SCORES) {
+            __syncthreads();
             if (threadIdx.x < FEW) {
-                for (int w = 0; w < FEW_WAVES; ++w) top = max(top, tops[w][threadIdx.x]);
+                for (int w = 0; w < WAVES; ++w) top = max(top, tops[w][threadIdx.x]);
                 f.tops[(unit * f.splits + split) * FEW + threadIdx.x] = top;
             }
             return;
         }
-        for (int w = 0; w < FEW_WAVES; ++w) top = max(top, tops[w][lane & 15]);
     } else {
         for (int i = 0; i < f.splits; ++i) top = max(top, f.tops[(unit * f.splits + i) * FEW + (lane & 15)]);
     }
 
     if constexpr (PASS != SCORES) {
-        for (int i = threadIdx.x; i < FEW * 64 * DC; i += 64 * FEW_WAVES) sums[i] = 0;
+        for (int i = threadIdx.x; i < FEW * 64 * DC; i += THREADS) sums[i] = 0;
         if (threadIdx.x < FEW) totals[threadIdx.x] = 0;
         __syncthreads();
+        if constexpr (PASS != VALUES)
+            for (int w = 0; w < WAVES; ++w) top = max(top, tops[w][lane & 15]);
         v4i hh[4 * DC] = {}, mid[4 * DC] = {}, ll[4 * DC] = {};
         int sum_h = 0, sum_l = 0;
-        const int in_values = ((lane >> 5) * 2 * DC) * 128 + (lane & 15) + 32 * ((lane >> 4) & 1);
-        const uint32_t last = a.entries - 1;
-        for (int t = from + wave; t < to; t += FEW_WAVES) {
-            const v4i* values = reinterpret_cast<const v4i*>(base + static_cast<size_t>(t) * Record<DC>::BYTES +
-                                                             Record<DC>::VALUES) +
-                                in_values;
-            const int* zt = z_of + ((PASS == FUSED ? t - from : t) * f.cols + (lane & 15)) * 64 + 4 * (lane >> 4);
+        auto use = [&](int t, const Values& v) {
             v4i eh, el;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 uint32_t e[4] = {};
                 if (mine) {
-                    const v4i z = *reinterpret_cast<const v4i*>(zt + 16 * k);
+                    const v4i zk = PASS == ONE ? z[k] : *reinterpret_cast<const v4i*>(z_at(t) + 16 * k);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (t * FX_TILE + first + 8 * k + r < limit)
-                            e[r] = encoded(a.table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[r]), last)]);
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t d = min(static_cast<uint32_t>(top) - static_cast<uint32_t>(zk[r]), last);
+                        if (t * FX_TILE + first + 8 * k + r < limit) e[r] = PASS == ONE ? table[d] : encoded(a.table[d]);
+                    }
                 }
                 const uint32_t a01 = e[0] | e[1] << 16, a23 = e[2] | e[3] << 16;
                 eh[k] = __builtin_amdgcn_perm(a23, a01, 0x07050301u);
@@ -750,11 +795,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
             }
 #pragma unroll
             for (int b = 0; b < 4 * DC; ++b) {
-                const v4i vh = values[(b >> 1) * 128 + (b & 1) * 16], vl = values[(b >> 1) * 128 + (b & 1) * 16 + 64];
-                hh[b] = mfma(vh, eh, hh[b]);
-                mid[b] = mfma(vh, el, mid[b]);
-                ll[b] = mfma(vl, el, ll[b]);
-                mid[b] = mfma(vl, eh, mid[b]);
+                hh[b] = mfma(v.h[b], eh, hh[b]);
+                mid[b] = mfma(v.h[b], el, mid[b]);
+                ll[b] = mfma(v.l[b], el, ll[b]);
+                mid[b] = mfma(v.l[b], eh, mid[b]);
+            }
+        };
+        if constexpr (PASS == ONE) {
+            if (wave < to) use(wave, ahead);
+        } else {
+            for (int t = from + wave; t < to; t += WAVES) {
+                Values v;
+                read_values(t, &v);
+                use(t, v);
             }
         }
         if (mine) {
@@ -770,14 +823,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fx_attention_few_kernel(Attent
         if constexpr (PASS == VALUES) {
             constexpr int WIDTH = 64 * DC + 1;
             int64_t* kept_sums = f.sums + (unit * f.splits + split) * f.cols * WIDTH;
-            for (int i = threadIdx.x; i < cols * 64 * DC; i += 64 * FEW_WAVES)
+            for (int i = threadIdx.x; i < cols * 64 * DC; i += THREADS)
                 kept_sums[i / (64 * DC) * WIDTH + i % (64 * DC)] = static_cast<int64_t>(sums[i]);
             if (threadIdx.x < cols)
                 kept_sums[threadIdx.x * WIDTH + 64 * DC] = static_cast<int64_t>(totals[threadIdx.x]);
             return;
         }
         // four places a thread
-        for (int i = threadIdx.x; i < cols * 16 * DC; i += 64 * FEW_WAVES) {
+        for (int i = threadIdx.x; i < cols * 16 * DC; i += THREADS) {
             const int col = i / (16 * DC), place = i % (16 * DC) * 4;
             if (place >= a.dim) continue;
             const int token = (row0 + col) / a.group, member = row0 + col - token * a.group;
@@ -844,18 +897,22 @@ int each_group(Context* c, const FxSeq* seqs, size_t count, Items&& items, Launc
 }
 
 template <int DC>
-int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::vector<FxSeq>& seqs, bool fused) {
+int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::vector<FxSeq>& seqs, Pass pass) {
     return each_group(
         c, seqs.data(), seqs.size(), [&](const FxSeq& s) { return (s.count * a.group + FEW - 1) / FEW; },
         [&](const Seqs& q, uint32_t total) {
             const dim3 grid(total * static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(f.splits));
-            const dim3 threads(64 * FEW_WAVES);
-            if (fused) {
-                hipLaunchKernelGGL((fx_attention_few_kernel<DC, FUSED>), grid, threads,
+            if (pass == ONE) {
+                hipLaunchKernelGGL((fx_attention_few_kernel<DC, ONE>), grid, dim3(64 * FEW_WAVES<DC, ONE>), 0, c->stream,
+                                   a, f, q);
+            } else if (pass == FUSED) {
+                hipLaunchKernelGGL((fx_attention_few_kernel<DC, FUSED>), grid, dim3(64 * FEW_WAVES<DC, FUSED>),
                                    static_cast<unsigned>(f.max_tiles * f.cols * 256), c->stream, a, f, q);
             } else {
-                hipLaunchKernelGGL((fx_attention_few_kernel<DC, SCORES>), grid, threads, 0, c->stream, a, f, q);
-                hipLaunchKernelGGL((fx_attention_few_kernel<DC, VALUES>), grid, threads, 0, c->stream, a, f, q);
+                hipLaunchKernelGGL((fx_attention_few_kernel<DC, SCORES>), grid, dim3(64 * FEW_WAVES<DC, SCORES>), 0,
+                                   c->stream, a, f, q);
+                hipLaunchKernelGGL((fx_attention_few_kernel<DC, VALUES>), grid, dim3(64 * FEW_WAVES<DC, VALUES>), 0,
+                                   c->stream, a, f, q);
                 hipLaunchKernelGGL(fx_attention_join_kernel<DC>, dim3(grid.x), dim3(256), 0, c->stream, a, f, q);
             }
         });
@@ -869,9 +926,12 @@ int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_
     f.max_tiles = static_cast<int>(std::max<size_t>(tiles, 1));
     f.splits = 1;
     const size_t score_bytes = f.max_tiles * cols * 256;
-    const bool fused = score_bytes <= 65536 && (tiles <= 2 * FEW_WAVES || units >= static_cast<size_t>(c->cu_count));
-    if (!fused) {
-        const size_t want = (2 * c->cu_count + units - 1) / units, most = (tiles + FEW_WAVES - 1) / FEW_WAVES;
+    const size_t waves = a.dim <= 64 ? FEW_WAVES<1, ONE> : FEW_WAVES<2, ONE>;
+    const Pass pass = tiles <= waves                                                                    ? ONE
+                      : score_bytes <= 65536 && (tiles <= 16 || units >= static_cast<size_t>(c->cu_count)) ? FUSED
+                                                                                                        : SCORES;
+    if (pass == SCORES) {
+        const size_t want = (2 * c->cu_count + units - 1) / units, most = (tiles + 7) / 8;
         f.splits = static_cast<int>(std::max<size_t>(1, std::min(want, most)));
         // every group of sequences reuses the space: its launches are in order
         const size_t z = units * score_bytes, tops = units * f.splits * FEW * 4;
@@ -881,7 +941,7 @@ int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_
         f.sums = reinterpret_cast<int64_t*>(ws<unsigned char>(c, WS_FIXED) + z);
         f.tops = reinterpret_cast<int*>(ws<unsigned char>(c, WS_FIXED) + z + sums);
     }
-    return a.dim <= 64 ? launch_few<1>(c, a, f, seqs, fused) : launch_few<2>(c, a, f, seqs, fused);
+    return a.dim <= 64 ? launch_few<1>(c, a, f, seqs, pass) : launch_few<2>(c, a, f, seqs, pass);
 }
 
 }  // namespace
