@@ -24,6 +24,7 @@ import numpy as np
 ABI_VERSION = 37
 P = 0xFFFF_FFFF_0000_0001
 FP2 = np.dtype([("c0", "<u8"), ("c1", "<u8")])
+_I16, _I32, _I64 = np.dtype(np.int16), np.dtype(np.int32), np.dtype(np.int64)
 
 _PKG = pathlib.Path(__file__).resolve().parent.parent
 DEFAULT_LIBRARY = _PKG / "libvolta_mi355x_backend.so"
@@ -287,8 +288,11 @@ class FixedKvCache:
     dim: int
     capacity: int
 
+    def __post_init__(self):
+        self._c = _FixedCache(self.storage.id, 0, self.slots, self.kv_heads, self.dim, self.capacity)
+
     def _args(self) -> _FixedCache:
-        return _FixedCache(self.storage.id, 0, self.slots, self.kv_heads, self.dim, self.capacity)
+        return self._c
 
 
 def _as_fp2(a) -> np.ndarray:
@@ -805,19 +809,41 @@ class Backend:
         self._check(self.lib.volta_cuda_fp2_mobius_inverse_inplace_device(self.raw, values.id, offset, n))
 
     # ---- fixed-point model operators (MI355X extensions; no reference counterpart) ---------
-    def _typed(self, buf: DeviceBuffer, dtype, what: str) -> DeviceBuffer:
-        self._own(buf)
-        if buf.dtype != np.dtype(dtype):
-            raise InvalidInput(f"{what} must hold {np.dtype(dtype).name}, not {buf.dtype}")
-        return buf
-
-    def _matrix(self, buf: DeviceBuffer, offset: int, stride: int, rows: int, cols: int, dtype, what: str) -> int:
+    # A generated token is a chain of small calls, so the host side of each stays
+    # short: arguments are checked once, without temporary arrays.
+    def _matrix(self, buf: DeviceBuffer, offset: int, stride: int, rows: int, cols: int, dtype: np.dtype,
+                what: str) -> int:
         """Checks a strided matrix inside a buffer and gives the buffer's id."""
-        self._typed(buf, dtype, what)
+        if buf.owner != id(self) or buf.id not in self._live:
+            raise InvalidInput("device buffer belongs to another backend or was freed")
+        if buf.dtype is not dtype and buf.dtype != dtype:
+            raise InvalidInput(f"{what} must hold {dtype.name}, not {buf.dtype}")
         if stride < cols:
             raise InvalidInput(f"{what}: row stride {stride} is shorter than a row of {cols}")
-        self._region(buf, offset, (rows - 1) * stride + cols)
+        if offset < 0 or offset + (rows - 1) * stride + cols > buf.len:
+            raise InvalidInput(f"{what}: device region is out of bounds")
         return buf.id
+
+    def _result(self, out: DeviceBuffer | None, offset: int, stride: int, rows: int, cols: int,
+                dtype: np.dtype) -> DeviceBuffer:
+        """The output buffer of rows x cols: `out`, checked, or a new one."""
+        if out is not None:
+            self._matrix(out, offset, stride, rows, cols, dtype, "output")
+            return out
+        if offset:
+            raise InvalidInput("an output offset needs an output buffer")
+        if stride < cols:
+            raise InvalidInput(f"output: row stride {stride} is shorter than a row of {cols}")
+        return self.alloc_device((rows - 1) * stride + cols, dtype)
+
+    def _done(self, rc: int, result: DeviceBuffer, out: DeviceBuffer | None) -> DeviceBuffer:
+        """`result`, or the call's error with a new result freed."""
+        if rc != 0:
+            msg = self.last_error()
+            if out is None:
+                self.free_device(result)
+            raise GpuError(msg or f"status {rc}")
+        return result
 
     def fixed_weights_device(self, weights: DeviceBuffer, k: int, n: int, *, offset: int = 0, stride: int | None = None,
                              transposed: bool = False) -> FixedWeights:
@@ -827,7 +853,7 @@ class Backend:
             raise InvalidInput("invalid fixed-point weight geometry")
         rows, cols = (n, k) if transposed else (k, n)
         stride = cols if stride is None else stride
-        wid = self._matrix(weights, offset, stride, rows, cols, np.int16, "weights")
+        wid = self._matrix(weights, offset, stride, rows, cols, _I16, "weights")
         out = self.alloc_device(size, np.uint8)
         self._call_or_free(out, self.lib.volta_mi355x_fixed_weights_device, wid, offset, k, n, stride,
                            1 if transposed else 0, out.id, 0)
@@ -850,41 +876,23 @@ class Backend:
             raise InvalidInput("invalid fixed-point linear geometry")
         if raw and (table is not None or residual is not None):
             raise InvalidInput("raw fixed-point sums take neither a table nor a residual")
-        a = _FixedLinear(x_off=x_offset, x_stride=k if x_stride is None else x_stride, bias_off=bias_offset,
-                         table_off=table_offset, residual_off=residual_offset,
-                         residual_stride=n if residual_stride is None else residual_stride, out_off=out_offset,
-                         out_stride=n if out_stride is None else out_stride, rows=rows, k=k, n=n,
-                         bias_shift=bias_shift, shift=0 if raw else shift, raw=1 if raw else 0)
-        a.x_id = self._matrix(x, x_offset, a.x_stride, rows, k, np.int16, "x")
+        x_stride = k if x_stride is None else x_stride
+        residual_stride = n if residual_stride is None else residual_stride
+        out_stride = n if out_stride is None else out_stride
         self._own(weights.storage)
-        a.weights_id = weights.storage.id
+        xid = self._matrix(x, x_offset, x_stride, rows, k, _I16, "x")
+        bid = tid = rid = 0
         if bias is not None:
-            a.bias_id = self._matrix(bias, bias_offset, n, 1, n, np.int16, "bias")
+            bid = self._matrix(bias, bias_offset, n, 1, n, _I16, "bias")
         if table is not None:
-            a.table_id = self._matrix(table, table_offset, 65536, 1, 65536, np.int16, "table")
+            tid = self._matrix(table, table_offset, 65536, 1, 65536, _I16, "table")
         if residual is not None:
-            a.residual_id = self._matrix(residual, residual_offset, a.residual_stride, rows, n, np.int16, "residual")
-        return self._into(out, a, rows, n, np.int64 if raw else np.int16,
-                          lambda: self.lib.volta_mi355x_fixed_linear_device(self.raw, ctypes.byref(a)))
-
-    def _into(self, out: DeviceBuffer | None, a, rows: int, cols: int, dtype, call) -> DeviceBuffer:
-        """Runs `call` with a's output set to `out`, or to a new buffer that a failure frees."""
-        made = out is None
-        if made:
-            if a.out_off:
-                raise InvalidInput("an output offset needs an output buffer")
-            if a.out_stride < cols:
-                raise InvalidInput(f"output: row stride {a.out_stride} is shorter than a row of {cols}")
-            out = self.alloc_device((rows - 1) * a.out_stride + cols, dtype)
-            a.out_id = out.id
-        else:
-            a.out_id = self._matrix(out, a.out_off, a.out_stride, rows, cols, dtype, "output")
-        if call() != 0:
-            msg = self.last_error()
-            if made:
-                self.free_device(out)
-            raise GpuError(msg or "fixed-point operator failed")
-        return out
+            rid = self._matrix(residual, residual_offset, residual_stride, rows, n, _I16, "residual")
+        result = self._result(out, out_offset, out_stride, rows, n, _I64 if raw else _I16)
+        a = _FixedLinear(xid, x_offset, x_stride, weights.storage.id, 0, bid, bias_offset, tid, table_offset, rid,
+                         residual_offset, residual_stride, result.id, out_offset, out_stride, rows, k, n, bias_shift,
+                         0 if raw else shift, 1 if raw else 0, 0)
+        return self._done(self.lib.volta_mi355x_fixed_linear_device(self.raw, a), result, out)
 
     def fixed_kv_cache(self, slots: int, kv_heads: int, dim: int, capacity: int) -> FixedKvCache:
         """An empty cache for `slots` sequences: its tokens are those that appends have written."""
@@ -900,11 +908,16 @@ class Backend:
 
     @staticmethod
     def _sequences(sequences) -> tuple[np.ndarray, int]:
-        """(n x 4 array, rows): slot, first row, rows, tokens in all, of each sequence."""
-        s = np.ascontiguousarray(sequences, dtype=np.int64).reshape(-1, 4)
-        if s.size and s.min() < 0:
-            raise InvalidInput("sequences hold whole numbers from 0 on")
-        return s, int((s[:, 1] + s[:, 2])[s[:, 2] > 0].max(initial=0))
+        """(n x 4 array, rows): slot, first row, rows, tokens in all, of each sequence; the entry point
+        checks the values themselves."""
+        s = sequences
+        if not (type(s) is np.ndarray and s.dtype == _I64 and s.ndim == 2 and s.shape[1] == 4 and s.flags.c_contiguous):
+            s = np.ascontiguousarray(s, dtype=np.int64).reshape(-1, 4)
+        if len(s) <= 4:
+            rows = max((first + count for _, first, count, _ in s.tolist() if count > 0), default=0)
+        else:
+            rows = int((s[:, 1] + s[:, 2])[s[:, 2] > 0].max(initial=0))
+        return s, rows
 
     def fixed_kv_append_device(self, cache: FixedKvCache, k: DeviceBuffer, v: DeviceBuffer, sequences, *,
                                k_offset: int = 0, k_stride: int | None = None, v_offset: int = 0,
@@ -913,14 +926,14 @@ class Backend:
         (slot, first row, new tokens, tokens in all); the new ones are the last."""
         s, rows = self._sequences(sequences)
         cols = cache.kv_heads * cache.dim
-        k_stride, v_stride = (cols if x is None else x for x in (k_stride, v_stride))
+        k_stride = cols if k_stride is None else k_stride
+        v_stride = cols if v_stride is None else v_stride
         self._own(cache.storage)
-        if rows:
-            self._matrix(k, k_offset, k_stride, rows, cols, np.int16, "keys")
-            self._matrix(v, v_offset, v_stride, rows, cols, np.int16, "values")
-        c = cache._args()
-        self._check(self.lib.volta_mi355x_fixed_kv_append_device(self.raw, ctypes.byref(c), k.id, k_offset, k_stride,
-                                                                 v.id, v_offset, v_stride, s.ctypes.data, len(s)))
+        if rows > 0:
+            self._matrix(k, k_offset, k_stride, rows, cols, _I16, "keys")
+            self._matrix(v, v_offset, v_stride, rows, cols, _I16, "values")
+        self._check(self.lib.volta_mi355x_fixed_kv_append_device(self.raw, cache._args(), k.id, k_offset, k_stride, v.id,
+                                                                 v_offset, v_stride, s.ctypes.data, len(s)))
 
     def fixed_attention_device(self, q: DeviceBuffer, cache: FixedKvCache, sequences, heads: int, table: DeviceBuffer,
                                shift: int, *, causal: bool = True, q_offset: int = 0, q_stride: int | None = None,
@@ -936,24 +949,22 @@ class Backend:
             raise InvalidInput("attention heads are not a multiple of the cache's")
         if not 8 <= shift <= 24 or not 0 < entries <= 8192:
             raise InvalidInput("invalid fixed-point attention shift or table")
-        if rows == 0 and out is None:
+        if rows <= 0 and out is None:
             raise InvalidInput("attention without rows needs an output buffer")
-        a = _FixedAttention(q_off=q_offset, q_stride=cols if q_stride is None else q_stride, table_off=table_offset,
-                            entries=entries, out_off=out_offset, out_stride=cols if out_stride is None else out_stride,
-                            heads=heads, shift=shift, causal=1 if causal else 0)
-        self._own(cache.storage)
-        a.table_id = self._matrix(table, table_offset, entries, 1, entries, table.dtype, "table")
         if table.dtype.itemsize != 2 or table.dtype.kind not in "iu":
             raise InvalidInput("the exponential table must hold 16-bit integers")
-        if rows:
-            a.q_id = self._matrix(q, q_offset, a.q_stride, rows, cols, np.int16, "queries")
-        c = cache._args()
-        call = lambda: self.lib.volta_mi355x_fixed_attention_device(  # noqa: E731
-            self.raw, ctypes.byref(c), ctypes.byref(a), s.ctypes.data, len(s))
-        if rows == 0:
-            self._check(call())
-            return out
-        return self._into(out, a, rows, cols, np.int16, call)
+        q_stride = cols if q_stride is None else q_stride
+        out_stride = cols if out_stride is None else out_stride
+        self._own(cache.storage)
+        tid = self._matrix(table, table_offset, entries, 1, entries, table.dtype, "table")
+        result = out
+        if rows > 0:
+            self._matrix(q, q_offset, q_stride, rows, cols, _I16, "queries")
+            result = self._result(out, out_offset, out_stride, rows, cols, _I16)
+        a = _FixedAttention(q.id, q_offset, q_stride, tid, table_offset, entries, result.id, out_offset, out_stride,
+                            heads, shift, 1 if causal else 0)
+        return self._done(self.lib.volta_mi355x_fixed_attention_device(self.raw, cache._args(), a, s.ctypes.data, len(s)),
+                          result, out)
 
     def fixed_norm_device(self, x: DeviceBuffer, rows: int, cols: int, gain: DeviceBuffer, shift: int, eps: int, *,
                           bias: DeviceBuffer | None = None, rms: bool = False, x_offset: int = 0,
@@ -966,21 +977,24 @@ class Backend:
         R = floor(sqrt(cols sum h^2 - S^2 + eps)): sat((cols h - S) gain / (R 2^shift) to the nearest integer + bias)."""
         if rows <= 0 or not 0 < cols <= 65536 or not 0 <= shift <= 15 or not 0 < eps <= 1 << 40:
             raise InvalidInput("invalid fixed-point norm geometry")
-        strides = [cols if st is None else st for st in (x_stride, residual_stride, sum_stride, out_stride)]
-        a = _FixedNorm(x_off=x_offset, x_stride=strides[0], residual_off=residual_offset, residual_stride=strides[1],
-                       sum_off=sum_offset, sum_stride=strides[2], gain_off=gain_offset, bias_off=bias_offset,
-                       out_off=out_offset, out_stride=strides[3], rows=rows, cols=cols, eps=eps, shift=shift,
-                       rms=1 if rms else 0)
-        a.x_id = self._matrix(x, x_offset, a.x_stride, rows, cols, np.int16, "x")
-        a.gain_id = self._matrix(gain, gain_offset, cols, 1, cols, np.int16, "gain")
+        x_stride = cols if x_stride is None else x_stride
+        residual_stride = cols if residual_stride is None else residual_stride
+        sum_stride = cols if sum_stride is None else sum_stride
+        out_stride = cols if out_stride is None else out_stride
+        xid = self._matrix(x, x_offset, x_stride, rows, cols, _I16, "x")
+        gid = self._matrix(gain, gain_offset, cols, 1, cols, _I16, "gain")
+        bid = rid = sid = 0
         if bias is not None:
-            a.bias_id = self._matrix(bias, bias_offset, cols, 1, cols, np.int16, "bias")
+            bid = self._matrix(bias, bias_offset, cols, 1, cols, _I16, "bias")
         if residual is not None:
-            a.residual_id = self._matrix(residual, residual_offset, a.residual_stride, rows, cols, np.int16, "residual")
+            rid = self._matrix(residual, residual_offset, residual_stride, rows, cols, _I16, "residual")
         if sum_out is not None:
-            a.sum_id = self._matrix(sum_out, sum_offset, a.sum_stride, rows, cols, np.int16, "sum")
-        return self._into(out, a, rows, cols, np.int16,
-                          lambda: self.lib.volta_mi355x_fixed_norm_device(self.raw, ctypes.byref(a)))
+            sid = self._matrix(sum_out, sum_offset, sum_stride, rows, cols, _I16, "sum")
+        result = self._result(out, out_offset, out_stride, rows, cols, _I16)
+        a = _FixedNorm(xid, x_offset, x_stride, rid, residual_offset, residual_stride, sid, sum_offset, sum_stride, gid,
+                       gain_offset, bid, bias_offset, result.id, out_offset, out_stride, rows, cols, eps, shift,
+                       1 if rms else 0)
+        return self._done(self.lib.volta_mi355x_fixed_norm_device(self.raw, a), result, out)
 
     def fixed_embed_device(self, tokens: DeviceBuffer, rows: int, table: DeviceBuffer, vocab: int, cols: int, *,
                            scale: int = 1, shift: int = 0, tokens_offset: int = 0, table_offset: int = 0,
@@ -995,19 +1009,21 @@ class Backend:
             raise InvalidInput("invalid fixed-point embedding geometry")
         if (positions is None) != (position_table is None) or (positions is not None and position_rows <= 0):
             raise InvalidInput("positions and their table come together")
-        strides = [cols if st is None else st for st in (table_stride, position_stride, out_stride)]
-        a = _FixedEmbed(tokens_off=tokens_offset, table_off=table_offset, table_stride=strides[0], vocab=vocab,
-                        positions_off=positions_offset, position_table_off=position_offset, position_stride=strides[1],
-                        position_rows=position_rows, out_off=out_offset, out_stride=strides[2], rows=rows, cols=cols,
-                        scale=scale, shift=shift)
-        a.tokens_id = self._matrix(tokens, tokens_offset, rows, 1, rows, np.int32, "tokens")
-        a.table_id = self._matrix(table, table_offset, a.table_stride, vocab, cols, np.int16, "table")
+        table_stride = cols if table_stride is None else table_stride
+        position_stride = cols if position_stride is None else position_stride
+        out_stride = cols if out_stride is None else out_stride
+        nid = self._matrix(tokens, tokens_offset, rows, 1, rows, _I32, "tokens")
+        tid = self._matrix(table, table_offset, table_stride, vocab, cols, _I16, "table")
+        pid = wid = 0
         if positions is not None:
-            a.positions_id = self._matrix(positions, positions_offset, rows, 1, rows, np.int32, "positions")
-            a.position_table_id = self._matrix(position_table, position_offset, a.position_stride, position_rows, cols,
-                                               np.int16, "position table")
-        return self._into(out, a, rows, cols, np.int16,
-                          lambda: self.lib.volta_mi355x_fixed_embed_device(self.raw, ctypes.byref(a)))
+            pid = self._matrix(positions, positions_offset, rows, 1, rows, _I32, "positions")
+            wid = self._matrix(position_table, position_offset, position_stride, position_rows, cols, _I16,
+                               "position table")
+        result = self._result(out, out_offset, out_stride, rows, cols, _I16)
+        a = _FixedEmbed(nid, tokens_offset, tid, table_offset, table_stride, vocab, pid, positions_offset, wid,
+                        position_offset, position_stride, position_rows, result.id, out_offset, out_stride, rows, cols,
+                        scale, shift)
+        return self._done(self.lib.volta_mi355x_fixed_embed_device(self.raw, a), result, out)
 
     def _call_or_free(self, out: DeviceBuffer, fn, *args) -> None:
         rc = fn(self.raw, *args)
