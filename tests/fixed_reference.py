@@ -26,23 +26,30 @@ def linear(x, w, *, bias=None, bias_shift=0, shift=0, table=None, residual=None,
     return h.astype(np.int16)
 
 
+def _sums(a, b):
+    """a @ b of integers below 2^15 and 2^16 in size, over fewer than 2^21 terms: exact in doubles."""
+    return (a.astype(np.float64) @ b.astype(np.float64)).astype(np.int64)
+
+
 def attention(q, keys, values, table, shift, causal):
     """q: rows x heads x dim; keys, values: tokens x kv heads x dim; the rows are the last tokens."""
     rows, heads, _ = q.shape
     tokens, kv_heads, _ = keys.shape
     out = np.zeros(q.shape, np.int16)
+    if tokens == 0:
+        return out
     e_of = np.minimum(table.astype(np.int64), 1 << 14)
+    hidden = np.zeros((rows, tokens), bool)
+    if causal:
+        hidden = np.arange(tokens)[None, :] > (tokens - rows + np.arange(rows))[:, None]
     for h in range(heads):
-        k, v = (t[:, h * kv_heads // heads].astype(np.int64) for t in (keys, values))
-        for i in range(rows):
-            seen = max(0, tokens - rows + i + 1) if causal else tokens
-            if seen == 0:
-                continue
-            z = (k[:seen] @ q[i, h].astype(np.int64)) >> shift
-            e = e_of[np.minimum(z.max() - z, len(e_of) - 1)]
-            total = int(e.sum())
-            if total:
-                out[i, h] = np.floor_divide(2 * (e @ v[:seen]) + total, 2 * total)
+        k, v = (t[:, h * kv_heads // heads] for t in (keys, values))
+        z = _sums(q[:, h], k.T) >> shift
+        z[hidden] = -(1 << 60)
+        e = e_of[np.minimum(z.max(1, keepdims=True) - z, len(e_of) - 1)]
+        e[hidden] = 0
+        total = e.sum(1, keepdims=True)
+        out[:, h] = np.where(total > 0, np.floor_divide(2 * _sums(e, v) + total, np.maximum(2 * total, 1)), 0)
     return out
 
 

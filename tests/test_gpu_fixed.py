@@ -372,6 +372,52 @@ def test_attention_many_sequences(backend):
     check_attention(backend, 13, counts, [c + 7 for c in counts], 6, 2, 64)
 
 
+def prompts(g, batch, longest, past=0):
+    """Sequences enough to fill the GPU with 128-row pieces: one of the longest, the rest of any length."""
+    counts = [longest] + [int(x) for x in g.integers(1, longest + 1, batch - 1)]
+    return counts, [c + (int(g.integers(0, past + 1)) if past else 0) for c in counts]
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads", [(5, 12, 12), (20, 12, 12), (9, 32, 8)])
+@pytest.mark.parametrize("dim", [33, 64, 100, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_many_prompts(backend, batch, heads, kv_heads, dim, causal):
+    g = gen(batch * 1000 + dim + causal)
+    counts, lengths = prompts(g, batch, 300)
+    check_attention(backend, dim, counts, lengths, heads, kv_heads, dim, causal=causal)
+
+
+@pytest.mark.parametrize("batch", [6, 20])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_many_prompts_over_a_past(backend, batch, dim):
+    counts, lengths = prompts(gen(batch + dim), batch, 260, past=150)
+    check_attention(backend, dim, counts, lengths, 12, 12, dim, gap=9, q_offset=3)
+
+
+@pytest.mark.parametrize("batch", [6, 20])
+@pytest.mark.parametrize("dim", [64, 127])
+@pytest.mark.parametrize("shift", [8, 16, 17, 24])
+def test_attention_many_prompts_with_values_at_the_ends(backend, batch, dim, shift):
+    counts, lengths = prompts(gen(batch + dim), batch, 150, past=40)
+    check_attention(backend, shift, counts, lengths, 24, 24, dim, shift=shift, std=None, values=None,
+                    table=exponentials(ENTRIES - 3, 40.0 * 2 ** (24 - shift) / 16))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("key", [32639, 32640])
+def test_attention_few_large_keys_and_queries(backend, dim, key):
+    """Tokens that need the offset of their low byte beside tokens that do not, in both kernels."""
+    for counts, lengths in (([1, 3], [200, 70]), prompts(gen(dim), 20, 200)):
+        g = gen(key)
+        q, k, v, past = attention_case(3, counts, lengths, 12, 12, dim)
+        for t in [q, k] + [p for p, _ in past if len(p)]:
+            flat = t.reshape(-1)
+            flat[g.integers(0, flat.size, max(1, flat.size // 4000))] = key
+        shift = max(8, round(np.log2(np.sqrt(dim) * 1e6 / 1280))) + 3
+        got = run_attention(backend, q, k, v, lengths, counts, past, exponentials(), shift)
+        assert np.array_equal(got, want_attention(q, k, v, lengths, counts, past, exponentials(), shift))
+
+
 def test_attention_appends_in_pieces(backend):
     """Tokens written one to three at a time, at every place of a tile, leave the same cache as one append."""
     g = gen(21)

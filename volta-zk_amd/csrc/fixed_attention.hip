@@ -329,11 +329,17 @@ __device__ inline void load_table(const uint16_t* from, int entries, uint16_t* t
     }
 }
 
-// Many rows: a workgroup takes 128 rows of a sequence and key head, 32 for each
-// group of DC waves, and goes over the tiles of 64 tokens twice: for the
-// maximum, then for the sums.  Keys and values come to LDS by direct copies,
-// three tiles ahead in the first pass, two (DC = 1) or two phases (DC = 2) in the
-// second.
+// Many rows: a workgroup takes 128 rows of a sequence and key head and goes over
+// the tiles of 64 tokens twice: for the maximum, then for the sums.  Keys and
+// values come to LDS by direct copies, three tiles ahead in the first pass, two
+// tiles (DC = 1) or two phases (DC = 2) in the second.
+//
+// With heads up to 64 (DC = 1) a workgroup is one or two teams of four waves, 32
+// rows a wave.  Two teams take the tiles in turn, each with buffers of its own,
+// and join their maxima and sums through LDS: where workgroups are few the
+// longest one decides, and it is done sooner (one 1,024-token prompt, 12 heads:
+// 47 us with one team, 35 us with two; sixteen of them: 131 and 151 us, as two
+// workgroups a CU hide each other's waits better).
 //
 // With heads over 64 (DC = 2) the two waves of a group take 32 tokens of a tile
 // each, exchange the exponentials through LDS, and keep half of the result's
@@ -341,15 +347,17 @@ __device__ inline void load_table(const uint16_t* from, int entries, uint16_t* t
 // phases a tile, scores with exponentials and the sums; the two halves of the
 // workgroup run one phase apart, so that a SIMD's two waves are never both at
 // the vector work.
-template <int DC>
-__global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs a, Seqs q) {
-    constexpr int WAVES = 4 * DC, PART = Record<DC>::VALUES;  // bytes of a tile's keys, and of its values
+template <int DC, int TEAMS>
+__global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(AttentionArgs a, Seqs q) {
+    constexpr int WAVES = 4 * DC;             // of a team
+    constexpr bool SHARED = DC * TEAMS == 2;  // two waves have the same rows
+    constexpr int PART = Record<DC>::VALUES;       // bytes of a tile's keys, and of its values
     constexpr int PARTS = DC == 1 ? 6 : 4, RING = 4;
-    __shared__ __attribute__((aligned(1024))) unsigned char parts[PARTS][PART];
-    __shared__ __attribute__((aligned(16))) int extras[RING][64];
+    __shared__ __attribute__((aligned(1024))) unsigned char all_parts[TEAMS][PARTS][PART];
+    __shared__ __attribute__((aligned(16))) int all_extras[TEAMS][RING][64];
     __shared__ __attribute__((aligned(16))) uint16_t table[FX_TABLE_MAX];
     __shared__ __attribute__((aligned(16))) v4i swap[DC == 2 ? WAVES * 128 : 1];
-    __shared__ int share[WAVES][32];
+    __shared__ int share[WAVES * TEAMS][32];
     // heads vary fastest: an XCD gets few of them, and their keys stay in its L2
     uint32_t item = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
     const int lane = threadIdx.x & 63, head = static_cast<int>(blockIdx.x - item * static_cast<uint32_t>(a.kv_heads));
@@ -364,7 +372,10 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
     }
     place = q.first[reach] - 1 - item / (reach + 1);
     const FxSeq s = q.s[item % (reach + 1)];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave / DC, part = wave % DC;
+    const int id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int team = id / WAVES, wave = id % WAVES, group = wave / DC, part = wave % DC;
+    auto& parts = all_parts[team];
+    auto& extras = all_extras[team];
     const int rows = static_cast<int>(s.count) * a.group;
     const int row0 = static_cast<int>(place) * 128;
     const int row = row0 + group * 32 + (lane & 31);
@@ -389,28 +400,34 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
         copy_to_lds(rec + wave * 1024, lane * 16, to + wave * 1024);
         copy_to_lds(rec + (WAVES + wave) * 1024, lane * 16, to + (WAVES + wave) * 1024);
     };
+    // a team's tiles: mine_of(0), mine_of(1), ...; `turns` of them and of the longer team's
+    auto mine_of = [&](int i) { return i * TEAMS + team; };
+    const int turns = (tiles + TEAMS - 1) / TEAMS;
 #pragma unroll
-    for (int t = 0; t < RING - 1; ++t)
-        if (t < tiles) stage_keys(t, parts[t], extras[t]);
+    for (int i = 0; i < RING - 1; ++i)
+        if (mine_of(i) < tiles) stage_keys(mine_of(i), parts[i], extras[i]);
     Query<DC> mine;
     load_query<DC>(a, s, head, row, lane, &mine);
     const bool no_offset = !__any(mine.o);
-    load_table(a.table, static_cast<int>(a.entries), table, threadIdx.x, 64 * WAVES);
+    load_table(a.table, static_cast<int>(a.entries), table, threadIdx.x, 64 * WAVES * TEAMS);
     const uint32_t last = a.entries - 1;
     auto is_plain = [&](int t, const int* extra) {
         return no_offset && !__any(lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128));
     };
 
     int top = INT_MIN;
-    for (int t = 0; t < tiles; ++t) {
-        if (t + RING - 2 < tiles)
+    for (int i = 0; i < turns; ++i) {
+        const int t = mine_of(i);
+        if (mine_of(i + RING - 2) < tiles)
             lds_copies_done<(RING - 2) * KEYS_COPIES>();
         else
             lds_copies_done<0>();
         __syncthreads();  // this tile has landed for all waves, and all have left the one before
-        if (t + RING - 1 < tiles) stage_keys(t + RING - 1, parts[(t + RING - 1) % RING], extras[(t + RING - 1) % RING]);
-        const unsigned char* keys = parts[t % RING];
-        const int* extra = extras[t % RING];
+        if (mine_of(i + RING - 1) < tiles)
+            stage_keys(mine_of(i + RING - 1), parts[(i + RING - 1) % RING], extras[(i + RING - 1) % RING]);
+        if (TEAMS == 2 && t >= tiles) break;  // the other team's last turn
+        const unsigned char* keys = parts[i % RING];
+        const int* extra = extras[i % RING];
         const bool plain = is_plain(t, extra);
 #pragma unroll
         for (int b = 0; b < 2 / DC; ++b) {
@@ -428,12 +445,11 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
         }
     }
     top = max(top, __shfl_xor(top, 32));
-    if constexpr (DC == 2) {
-        if (lane < 32) share[wave][lane] = top;
-        __syncthreads();
-        top = max(top, share[wave ^ 1][lane & 31]);
-    }
-    __syncthreads();  // the first pass's buffers are free
+    // the other half of the tokens: the other team, or the other wave of the group
+    const int other = DC == 1 ? id ^ 4 : id ^ 1;
+    if (SHARED && lane < 32) share[id][lane] = top;
+    __syncthreads();  // and the first pass's buffers are free
+    if (SHARED) top = max(top, share[other][lane & 31]);
 
     v16i hh[2] = {}, mid[2] = {}, ll[2] = {};  // 32 places each, of this wave's 64
     int sum_h = 0, sum_l = 0;
@@ -484,20 +500,22 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
     if constexpr (DC == 1) {
         constexpr int AHEAD = 2;  // tiles, of three in LDS
 #pragma unroll
-        for (int t = 0; t < AHEAD; ++t)
-            if (t < tiles) stage_keys(t, parts[2 * t], extras[t]), stage_values(t, parts[2 * t + 1]);
+        for (int i = 0; i < AHEAD; ++i)
+            if (mine_of(i) < tiles) stage_keys(mine_of(i), parts[2 * i], extras[i]), stage_values(mine_of(i), parts[2 * i + 1]);
         int now = 0;
-        for (int t = 0; t < tiles; ++t) {
-            if (t + 1 < tiles)
+        for (int i = 0; i < turns; ++i) {
+            const int t = mine_of(i);
+            if (mine_of(i + 1) < tiles)
                 lds_copies_done<KEYS_COPIES + VALUES_COPIES>();
             else
                 lds_copies_done<0>();
             __syncthreads();
-            if (t + AHEAD < tiles) {
+            if (mine_of(i + AHEAD) < tiles) {
                 const int next = now == 0 ? 2 : now - 1;
-                stage_keys(t + AHEAD, parts[2 * next], extras[next]);
-                stage_values(t + AHEAD, parts[2 * next + 1]);
+                stage_keys(mine_of(i + AHEAD), parts[2 * next], extras[next]);
+                stage_values(mine_of(i + AHEAD), parts[2 * next + 1]);
             }
+            if (TEAMS == 2 && t >= tiles) break;
             const bool plain = is_plain(t, extras[now]);
 #pragma unroll
             for (int block = 0; block < 2; ++block) {
@@ -557,22 +575,47 @@ __global__ __launch_bounds__(256 * DC, 2) void fx_attention_kernel(AttentionArgs
     }
     int total = 256 * sum_h + sum_l;
     total += __shfl_xor(total, 32);
-    if constexpr (DC == 2) {
+    __syncthreads();
+    if (SHARED && lane < 32) share[id][lane] = total;
+    if constexpr (TEAMS == 2) {
+        // The teams' sums: each gives the other those of 32 places and finishes the rest.
+        static_assert(sizeof(all_parts) >= 8 * 48 * 64 * sizeof(int), "room for the exchange");
+        int* mail = reinterpret_cast<int*>(all_parts) + lane;
+        auto send = [&](const v16i& x, const v16i& y, const v16i& z) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                mail[(id * 48 + r) * 64] = x[r];
+                mail[(id * 48 + 16 + r) * 64] = y[r];
+                mail[(id * 48 + 32 + r) * 64] = z[r];
+            }
+        };
+        if (team == 0) {
+            send(hh[1], mid[1], ll[1]);
+        } else {
+            send(hh[0], mid[0], ll[0]);
+            hh[0] = hh[1], mid[0] = mid[1], ll[0] = ll[1];
+        }
         __syncthreads();
-        if (lane < 32) share[wave][lane] = total;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            hh[0][r] += mail[(other * 48 + r) * 64];
+            mid[0][r] += mail[(other * 48 + 16 + r) * 64];
+            ll[0][r] += mail[(other * 48 + 32 + r) * 64];
+        }
+    } else {
         __syncthreads();
-        total += share[wave ^ 1][lane & 31];
     }
+    if (SHARED) total += share[other][lane & 31];
     if (row >= rows) return;
     const int token = row / a.group, member = row - token * a.group;
     int16_t* out = a.out + (static_cast<size_t>(s.row) + token) * a.out_stride +
                    (static_cast<size_t>(head) * a.group + member) * a.dim;
     const Divide divide(total);
 #pragma unroll
-    for (int d = 0; d < 2; ++d)
+    for (int d = 0; d < 2 / TEAMS; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int place = part * 64 + d * 32 + 8 * g + 4 * (lane >> 5);
+            const int place = team * 32 + part * 64 + d * 32 + 8 * g + 4 * (lane >> 5);
             if (place >= a.dim) continue;
             int v[4];
 #pragma unroll
@@ -979,23 +1022,49 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
                           s1,
                           t.shift - s1,
                           t.causal};
-    std::vector<FxSeq> many, few;
-    size_t tiles = 0, cols = 0, units = 0;
+    // Where many rows leave CUs idle, the kernel for few rows, which splits the
+    // tiles, is faster.  Estimates in ns from measurements (rows x tokens, heads
+    // of 128 on 4 key heads): 32 x 8,192 268 us by rows and 40 by tiles, 512 x
+    // 8,192 368 and 92, eight of 128 x 4,096 191 and 96, 16 of 64 x 2,048 on 8
+    // key heads 78 and 96, one prompt of 4,096 190 and more than that.
+    auto rows_of = [&](const FxSeq& s) { return size_t{s.count} * group; };
+    auto tiles_of = [&](const FxSeq& s) {  // of a middle row
+        return static_cast<double>(s.length - (t.causal ? s.count / 2 : 0)) / FX_TILE + 1;
+    };
+    double by_rows = 0, by_tiles = 0, longest = 0;
+    size_t tiles = 0, units = 0, workgroups = 0;
     for (size_t i = 0; i < count; ++i) {
         const FxSeq& s = seqs[i];
-        if (s.count * group > FEW) {
+        tiles = std::max<size_t>(tiles, (s.length + FX_TILE - 1) / FX_TILE);
+        units += (rows_of(s) + FEW - 1) / FEW * cache.kv_heads;
+        if (rows_of(s) <= FEW) continue;
+        by_rows += static_cast<double>((rows_of(s) + 127) / 128 * cache.kv_heads) * tiles_of(s) * 11;
+        by_tiles += static_cast<double>((rows_of(s) + FEW - 1) / FEW * cache.kv_heads) * tiles_of(s) * 5;
+        longest = std::max(longest, (s.length + FX_TILE - 1) / FX_TILE * (cache.dim <= 64 ? 1500.0 : 2200.0));
+    }
+    const bool split = by_tiles + 5000 < std::max(by_rows, longest) && units * tiles * FEW * 256 <= size_t{1} << 29;
+    std::vector<FxSeq> many, few;
+    size_t cols = 0;
+    tiles = units = 0;
+    for (size_t i = 0; i < count; ++i) {
+        const FxSeq& s = seqs[i];
+        if (rows_of(s) > FEW && !split) {
             many.push_back(s);
+            workgroups += (rows_of(s) + 127) / 128 * cache.kv_heads;
             continue;
         }
         few.push_back(s);
         tiles = std::max<size_t>(tiles, (s.length + FX_TILE - 1) / FX_TILE);
-        cols = std::max<size_t>(cols, std::min<size_t>(s.count * group, FEW));
-        units += (s.count * group + FEW - 1) / FEW * cache.kv_heads;
+        cols = std::max<size_t>(cols, std::min<size_t>(rows_of(s), FEW));
+        units += (rows_of(s) + FEW - 1) / FEW * cache.kv_heads;
     }
     if (!few.empty()) {
         const int rc = few_rows(c, a, few, tiles, cols, units);
         if (rc < 0) return -1;
-        if (rc) many.assign(seqs, seqs + count);
+        if (rc) {
+            many.assign(seqs, seqs + count);
+            workgroups = SIZE_MAX;
+        }
     }
     auto items = [&](const FxSeq& s) { return (s.count * group + 127) / 128; };
     std::sort(many.begin(), many.end(), [&](const FxSeq& x, const FxSeq& y) { return items(x) > items(y); });
@@ -1004,10 +1073,12 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
             for (uint32_t i = 0; i < q.count; ++i) q.first[i] = items(q.s[i]);
             q.first[q.count] = 0;
             const dim3 grid(total * static_cast<unsigned>(cache.kv_heads));
-            if (cache.dim <= 64)
-                hipLaunchKernelGGL(fx_attention_kernel<1>, grid, dim3(256), 0, c->stream, a, q);
+            if (cache.dim > 64)
+                hipLaunchKernelGGL((fx_attention_kernel<2, 1>), grid, dim3(512), 0, c->stream, a, q);
+            else if (workgroups <= 2 * static_cast<size_t>(c->cu_count))
+                hipLaunchKernelGGL((fx_attention_kernel<1, 2>), grid, dim3(512), 0, c->stream, a, q);
             else
-                hipLaunchKernelGGL(fx_attention_kernel<2>, grid, dim3(512), 0, c->stream, a, q);
+                hipLaunchKernelGGL((fx_attention_kernel<1, 1>), grid, dim3(256), 0, c->stream, a, q);
         });
 }
 
