@@ -1,6 +1,8 @@
 // fixed_rows.hip -- row operators of the fixed-point model: the norm with its
 // residual addition, and the embedding of tokens and positions.  Both are bound
 // by memory: eight elements a thread at a time, whatever the rows' alignment.
+#include <algorithm>
+
 #include "fixed.hpp"
 
 namespace vmx {
@@ -49,9 +51,22 @@ __device__ inline v4i add_sat(v4i a, v4i b) {
     return c;
 }
 
-__device__ inline int64_t wave_sum(int64_t v) {
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-    return v;
+// The sum of a wave's values, in all lanes: four steps within rows of 16 lanes,
+// two across them, no LDS.
+__device__ inline int wave_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The same for values below 2^44.
+__device__ inline uint64_t wave_sum(uint64_t v) {
+    const uint32_t low = static_cast<uint32_t>(wave_sum(static_cast<int>(v & 0xfffff)));
+    return (static_cast<uint64_t>(static_cast<uint32_t>(wave_sum(static_cast<int>(v >> 20)))) << 20) + low;
 }
 
 // floor(sqrt(v)) for 0 < v < 2^63: the rounded square root of the rounded v is
@@ -68,86 +83,112 @@ __device__ inline uint64_t floor_sqrt(uint64_t v) {
 // R = floor(sqrt(V + eps)); y = sat(floor((2 (n h - S) gain + B) / 2B) + bias), B = R 2^shift.
 //
 // THREADS threads a row, KEPT pieces of eight elements each in registers (0: any
-// length, read twice).  |n h - S| <= 2^32 and B < 2^47, so every value of the
-// division is a whole number below 2^53: doubles hold it exactly.
+// length, read twice).  A wave that has rows to itself takes several in turn and
+// keeps the gains.
 //
-// 16,384 rows of 768 with a residual, its sum kept (100 MB): a row a wave 28 us
-// (3.6 TB/s), a row a workgroup and elements one by one 57 us.
+// |n h - S| <= 2^32 and B < 2^47, so every value of the division is a whole number
+// below 2^53: doubles hold it exactly.  The quotient is estimated a little high:
+// where it is below 2^17 the estimate is off by less than 2^-34, so its floor is
+// right or one too high, which the exact remainder's sign shows; where it is not,
+// the result is clamped whatever it is.
+//
+// 16,384 rows of 768 with a residual, its sum kept (100 MB): 25 us, 4.0 TB/s
+// (a copy reaches 5.0); a row a workgroup, elements one by one, took 57.
 template <int THREADS, int KEPT>
 __global__ __launch_bounds__(256) void fx_norm_kernel(FxNorm a) {
-    constexpr int WAVES = THREADS / 64;
+    constexpr int WAVES = THREADS / 64, ROWS = 256 / THREADS;
     __shared__ int64_t part[2][4];
-    const size_t row = static_cast<size_t>(blockIdx.x) * (256 / THREADS) + threadIdx.x / THREADS;
     const int thread = threadIdx.x % THREADS;
-    if (WAVES == 1 && row >= a.rows) return;
-    const int16_t* x = a.x + row * a.x_stride;
-    const int16_t* res = a.residual ? a.residual + row * a.residual_stride : nullptr;
-    auto piece = [&](int at) {
-        const v4i v = load8(x, at, a.cols);
-        return res ? add_sat(v, load8(res, at, a.cols)) : v;
-    };
-    int64_t s = 0;
-    uint64_t q = 0;
-    auto count = [&](v4i v) {
-        int some = 0;
+    double gain[KEPT ? KEPT * 8 : 8];
+    Eight bias[KEPT ? KEPT : 1];
+    auto load_gain = [&](int at, double* g, Eight* b) {
+        Eight u;
+        u.v = load8(a.gain, at, a.cols);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int pair = v[i];
-            const v2s two = __builtin_bit_cast(v2s, pair);
-            some = __builtin_amdgcn_sdot2(two, v2s{1, 1}, some, false);
-            q += static_cast<uint32_t>(__builtin_amdgcn_sdot2(two, two, 0, false));  // at most 2^31
-        }
-        s += some;
-    };
-    v4i kept[KEPT ? KEPT : 1];
-    if constexpr (KEPT > 0) {
-#pragma unroll
-        for (int i = 0; i < KEPT; ++i) {
-            const int at = (i * THREADS + thread) * 8;
-            kept[i] = at < a.cols ? piece(at) : v4i{0, 0, 0, 0};
-            count(kept[i]);
-        }
-    } else {
-        for (int at = thread * 8; at < a.cols; at += THREADS * 8) count(piece(at));
-    }
-    s = wave_sum(s);
-    q = static_cast<uint64_t>(wave_sum(static_cast<int64_t>(q)));
-    if constexpr (WAVES > 1) {
-        if ((threadIdx.x & 63) == 0) {
-            part[0][threadIdx.x >> 6] = s;
-            part[1][threadIdx.x >> 6] = static_cast<int64_t>(q);
-        }
-        __syncthreads();
-        s = part[0][0] + part[0][1] + part[0][2] + part[0][3];
-        q = static_cast<uint64_t>(part[1][0] + part[1][1] + part[1][2] + part[1][3]);
-    }
-    if (a.rms) s = 0;
-    const uint64_t v = static_cast<uint64_t>(a.cols) * q - static_cast<uint64_t>(s * s) + a.eps;
-    const double below = 2.0 * static_cast<double>(floor_sqrt(v) << a.shift), inv = 1.0 / below;
-    const double n = a.cols, sum = static_cast<double>(s);
-    auto finish = [&](int at, v4i h) {
-        Eight hu, gu, bu, out;
-        hu.v = h;
-        gu.v = load8(a.gain, at, a.cols);
-        bu.v = a.bias ? load8(a.bias, at, a.cols) : v4i{0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const double c = __builtin_fma(n, static_cast<double>(hu.e[e]), -sum);
-            const double y = floor_div(__builtin_fma(c, 2.0 * gu.e[e], 0.5 * below), below, inv) + bu.e[e];
-            out.e[e] = static_cast<int16_t>(__builtin_fmin(__builtin_fmax(y, -32768.0), 32767.0));
-        }
-        store8(a.out + row * a.out_stride, at, a.cols, out.v);
-        if (a.sum) store8(a.sum + row * a.sum_stride, at, a.cols, h);
+        for (int e = 0; e < 8; ++e) g[e] = 2.0 * u.e[e];
+        b->v = a.bias ? load8(a.bias, at, a.cols) : v4i{0, 0, 0, 0};
     };
     if constexpr (KEPT > 0) {
 #pragma unroll
         for (int i = 0; i < KEPT; ++i) {
             const int at = (i * THREADS + thread) * 8;
-            if (at < a.cols) finish(at, kept[i]);
+            if (at < a.cols) load_gain(at, gain + 8 * i, &bias[i]);
         }
-    } else {
-        // a sum over x or the residual is written by the thread that has read it
-        for (int at = thread * 8; at < a.cols; at += THREADS * 8) finish(at, piece(at));
+    }
+    for (size_t row = static_cast<size_t>(blockIdx.x) * ROWS + threadIdx.x / THREADS; row < a.rows;
+         row += static_cast<size_t>(gridDim.x) * ROWS) {
+        const int16_t* x = a.x + row * a.x_stride;
+        const int16_t* res = a.residual ? a.residual + row * a.residual_stride : nullptr;
+        auto piece = [&](int at) {
+            const v4i v = load8(x, at, a.cols);
+            return res ? add_sat(v, load8(res, at, a.cols)) : v;
+        };
+        int s = 0;  // at most 2^31 - 2^15, or -2^31, over a row
+        uint64_t q = 0;
+        auto count = [&](v4i v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int pair = v[i];
+                const v2s two = __builtin_bit_cast(v2s, pair);
+                s = __builtin_amdgcn_sdot2(two, v2s{1, 1}, s, false);
+                q += static_cast<uint32_t>(__builtin_amdgcn_sdot2(two, two, 0, false));  // at most 2^31
+            }
+        };
+        v4i kept[KEPT ? KEPT : 1];
+        if constexpr (KEPT > 0) {
+#pragma unroll
+            for (int i = 0; i < KEPT; ++i) {
+                const int at = (i * THREADS + thread) * 8;
+                kept[i] = at < a.cols ? piece(at) : v4i{0, 0, 0, 0};
+                count(kept[i]);
+            }
+        } else {
+            for (int at = thread * 8; at < a.cols; at += THREADS * 8) count(piece(at));
+        }
+        int64_t sum = wave_sum(s);
+        q = wave_sum(q);
+        if constexpr (WAVES > 1) {
+            if (threadIdx.x / 64 * 64 == threadIdx.x) {
+                part[0][threadIdx.x / 64] = sum;
+                part[1][threadIdx.x / 64] = static_cast<int64_t>(q);
+            }
+            __syncthreads();
+            sum = part[0][0] + part[0][1] + part[0][2] + part[0][3];
+            q = static_cast<uint64_t>(part[1][0] + part[1][1] + part[1][2] + part[1][3]);
+            __syncthreads();  // before the next row's
+        }
+        if (a.rms) sum = 0;
+        const uint64_t v = static_cast<uint64_t>(a.cols) * q - static_cast<uint64_t>(sum * sum) + a.eps;
+        const double below = 2.0 * static_cast<double>(floor_sqrt(v) << a.shift), inv = 1.0 / below, half = 0.5 * below;
+        const double n = a.cols, away = -static_cast<double>(sum);
+        auto finish = [&](int at, v4i h, const double* g, const Eight& b) {
+            Eight hu, out;
+            hu.v = h;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double top = __builtin_fma(__builtin_fma(n, static_cast<double>(hu.e[e]), away), g[e], half);
+                const double est = __builtin_floor(__builtin_fma(top, inv, 0x1p-34));
+                const double rest = __builtin_fma(-est, below, top);
+                const double est_in = __builtin_fmin(__builtin_fmax(est, -1048576.0), 1048576.0);
+                int y = static_cast<int>(est_in) + (__builtin_bit_cast(int64_t, rest) < 0 ? -1 : 0) + b.e[e];
+                out.e[e] = static_cast<int16_t>(min(max(y, -32768), 32767));
+            }
+            store8(a.out + row * a.out_stride, at, a.cols, out.v);
+            if (a.sum) store8(a.sum + row * a.sum_stride, at, a.cols, h);
+        };
+        if constexpr (KEPT > 0) {
+#pragma unroll
+            for (int i = 0; i < KEPT; ++i) {
+                const int at = (i * THREADS + thread) * 8;
+                if (at < a.cols) finish(at, kept[i], gain + 8 * i, bias[i]);
+            }
+        } else {
+            // a sum over x or the residual is written by the thread that has read it
+            for (int at = thread * 8; at < a.cols; at += THREADS * 8) {
+                load_gain(at, gain, bias);
+                finish(at, piece(at), gain, bias[0]);
+            }
+        }
     }
 }
 
@@ -186,9 +227,10 @@ __global__ __launch_bounds__(256) void fx_embed_kernel(FxEmbed a, uint32_t piece
 
 template <int THREADS, int KEPT>
 void launch_norm(Context* c, const FxNorm& a) {
-    const size_t rows = 256 / THREADS;
-    hipLaunchKernelGGL((fx_norm_kernel<THREADS, KEPT>), dim3(static_cast<unsigned>((a.rows + rows - 1) / rows)), dim3(256), 0,
-                       c->stream, a);
+    constexpr size_t rows = 256 / THREADS;
+    // several rows a workgroup once there are eight workgroups a CU
+    const size_t groups = std::min<size_t>((a.rows + rows - 1) / rows, 8 * static_cast<size_t>(c->cu_count));
+    hipLaunchKernelGGL((fx_norm_kernel<THREADS, KEPT>), dim3(static_cast<unsigned>(groups)), dim3(256), 0, c->stream, a);
 }
 
 }  // namespace
