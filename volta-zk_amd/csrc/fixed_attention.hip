@@ -319,15 +319,30 @@ __device__ inline v4i encoded8(v4i v) {
     return v;
 }
 
-// The table to LDS, encoded; the rest of the space is not read.
-__device__ inline void load_table(const uint16_t* from, int entries, uint16_t* to, int thread, int threads) {
-    for (int i = thread * 8; i < entries; i += threads * 8) {
-        if (i + 8 <= entries)
-            *reinterpret_cast<v4i*>(to + i) = encoded8(load8(reinterpret_cast<const int16_t*>(from) + i));
-        else
-            for (int k = i; k < entries; ++k) to[k] = static_cast<uint16_t>(encoded(from[k]));
+// The exponential table on its way to LDS, encoded there: loads are under way
+// from load() on, so that they cost no wait of their own.
+template <int THREADS>
+struct Table {
+    static constexpr int PIECES = FX_TABLE_MAX / 8 / THREADS;
+    v4i piece[PIECES];
+    __device__ void load(const uint16_t* from, int entries) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int i = (k * THREADS + static_cast<int>(threadIdx.x)) * 8;
+            if (i + 8 <= entries) piece[k] = load8(reinterpret_cast<const int16_t*>(from) + i);
+        }
     }
-}
+    __device__ void store(const uint16_t* from, int entries, uint16_t* to) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int i = (k * THREADS + static_cast<int>(threadIdx.x)) * 8;
+            if (i + 8 <= entries)
+                *reinterpret_cast<v4i*>(to + i) = encoded8(piece[k]);
+            else
+                for (int e = i; e < entries; ++e) to[e] = static_cast<uint16_t>(encoded(from[e]));
+        }
+    }
+};
 
 // Many rows: a workgroup takes 128 rows of a sequence and key head and goes over
 // the tiles of 64 tokens twice: for the maximum, then for the sums.  Keys and
@@ -403,13 +418,15 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
     // a team's tiles: mine_of(0), mine_of(1), ...; `turns` of them and of the longer team's
     auto mine_of = [&](int i) { return i * TEAMS + team; };
     const int turns = (tiles + TEAMS - 1) / TEAMS;
+    Table<64 * WAVES * TEAMS> to_table;
+    to_table.load(a.table, static_cast<int>(a.entries));
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
         if (mine_of(i) < tiles) stage_keys(mine_of(i), parts[i], extras[i]);
     Query<DC> mine;
     load_query<DC>(a, s, head, row, lane, &mine);
     const bool no_offset = !__any(mine.o);
-    load_table(a.table, static_cast<int>(a.entries), table, threadIdx.x, 64 * WAVES * TEAMS);
+    to_table.store(a.table, static_cast<int>(a.entries), table);
     const uint32_t last = a.entries - 1;
     auto is_plain = [&](int t, const int* extra) {
         return no_offset && !__any(lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128));
@@ -710,12 +727,10 @@ __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_k
     int top = INT_MIN;
     v4i z[4] = {};
     Values ahead;
-    v4i entries = {};
+    Table<THREADS> to_table;
     if constexpr (PASS == ONE) {
         if (wave < to) read_values(wave, &ahead);
-        const int i = threadIdx.x * 8;
-        if (THREADS * 8 >= static_cast<int>(FX_TABLE_MAX) && i + 8 <= static_cast<int>(a.entries))
-            entries = load8(reinterpret_cast<const int16_t*>(a.table) + i);
+        to_table.load(a.table, static_cast<int>(a.entries));
     }
     if constexpr (PASS != VALUES) {
         FewQuery<DC> mq;
@@ -786,17 +801,7 @@ __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_k
         top = max(top, __shfl_xor(top, 16));
         top = max(top, __shfl_xor(top, 32));
         if (lane < FEW) tops[wave][lane] = top;
-        if constexpr (PASS == ONE) {
-            if constexpr (THREADS * 8 >= static_cast<int>(FX_TABLE_MAX)) {
-                const int i = threadIdx.x * 8;
-                if (i + 8 <= static_cast<int>(a.entries))
-                    *reinterpret_cast<v4i*>(table + i) = encoded8(entries);
-                else
-                    for (int k = i; k < static_cast<int>(a.entries); ++k) table[k] = static_cast<uint16_t>(encoded(a.table[k]));
-            } else {
-                load_table(a.table, static_cast<int>(a.entries), table, threadIdx.x, THREADS);
-            }
-        }
+        if constexpr (PASS == ONE) to_table.store(a.table, static_cast<int>(a.entries), table);
         if constexpr (PASS == SCORES) {
             __syncthreads();
             if (threadIdx.x < FEW) {
