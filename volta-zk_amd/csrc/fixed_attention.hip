@@ -239,13 +239,15 @@ __device__ inline void load_query(const AttentionArgs& a, const FxSeq& s, int he
     for (int u = 0; u < 2 * DC; ++u) split16(lo[u], hi[u], q->o, &q->h[u], &q->l[u]);
 }
 
-// Scores z of 32 tokens (block `block` of the record's keys and extras), this
-// lane's query: token 8 (r >> 2) + 4 (lane >> 5) + (r & 3) in place r.  `plain`:
-// neither a key of the tile nor a query of the wave has an offset.
-template <int DC>
-__device__ inline v16i scores(const unsigned char* keys, const int* extra, const Query<DC>& q, int block, int lane,
-                              uint32_t s1, uint32_t s2, bool plain) {
+// The three sums of 32 tokens' scores (block `block` of a record's keys) with this
+// lane's query: token 8 (r >> 2) + 4 (lane >> 5) + (r & 3) in place r.
+struct Raw {
     v16i hh = {}, mid = {}, ll = {};
+};
+
+template <int DC>
+__device__ inline Raw products(const unsigned char* keys, const Query<DC>& q, int block, int lane) {
+    Raw s;
     const v4i* p = reinterpret_cast<const v4i*>(keys) + block * 2 * DC * 128 + lane;
     v4i kh[2 * DC], kl[2 * DC];
 #pragma unroll
@@ -253,23 +255,35 @@ __device__ inline v16i scores(const unsigned char* keys, const int* extra, const
     __builtin_amdgcn_sched_barrier(0);  // all reads first: one wait for LDS, not one a step
 #pragma unroll
     for (int u = 0; u < 2 * DC; ++u) {
-        hh = mfma32(kh[u], q.h[u], hh);
-        mid = mfma32(kh[u], q.l[u], mid);
-        ll = mfma32(kl[u], q.l[u], ll);
-        mid = mfma32(kl[u], q.h[u], mid);
+        s.hh = mfma32(kh[u], q.h[u], s.hh);
+        s.mid = mfma32(kh[u], q.l[u], s.mid);
+        s.ll = mfma32(kl[u], q.l[u], s.ll);
+        s.mid = mfma32(kl[u], q.h[u], s.mid);
     }
+    return s;
+}
+
+// Scores z, up to a shift of 16.
+__device__ inline int score(const Raw& s, int r, uint32_t s1) {
+    return (s.hh[r] << (16 - s1)) + (static_cast<int>((static_cast<uint32_t>(s.mid[r]) << 8) + s.ll[r]) >> s1);
+}
+
+// Scores z.  `plain`: neither a key of the tile nor a query of the wave has an offset.
+template <int DC>
+__device__ inline v16i scores(const unsigned char* keys, const int* extra, const Query<DC>& q, int block, int lane,
+                              uint32_t s1, uint32_t s2, bool plain) {
+    Raw s = products<DC>(keys, q, block, lane);
     if (!plain) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int x = extra[block * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)];
-            ll[r] = static_cast<int>(static_cast<uint32_t>(ll[r]) + static_cast<uint32_t>((x & 128) * q.sum) +
-                                     static_cast<uint32_t>((x >> 8) * q.o));
+            s.ll[r] = static_cast<int>(static_cast<uint32_t>(s.ll[r]) + static_cast<uint32_t>((x & 128) * q.sum) +
+                                       static_cast<uint32_t>((x >> 8) * q.o));
         }
     }
     v16i z;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-        z[r] = (hh[r] << (16 - s1)) + (static_cast<int>((static_cast<uint32_t>(mid[r]) << 8) + ll[r]) >> s1);
+    for (int r = 0; r < 16; ++r) z[r] = score(s, r, s1);
     if (s2) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] >>= s2;
@@ -446,6 +460,15 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
         const unsigned char* keys = parts[i % RING];
         const int* extra = extras[i % RING];
         const bool plain = is_plain(t, extra);
+        if (DC == 1 && plain && a.s2 == 0 && (t + 1) * FX_TILE <= all) {
+            // Most tiles, without a branch: one block's vector work beside the other's products.
+            const Raw s0 = products<DC>(keys, mine, 0, lane), s1 = products<DC>(keys, mine, 1, lane);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = max(top, score(s0, r, a.s1));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = max(top, score(s1, r, a.s1));
+            continue;
+        }
 #pragma unroll
         for (int b = 0; b < 2 / DC; ++b) {
             const int block = DC == 2 ? part : b, token = t * FX_TILE + block * 32;
@@ -470,14 +493,12 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
 
     v16i hh[2] = {}, mid[2] = {}, ll[2] = {};  // 32 places each, of this wave's 64
     int sum_h = 0, sum_l = 0;
-    // exponentials of 32 tokens
-    auto exponentials = [&](const unsigned char* keys, const int* extra, int block, int token, bool plain, v4i* eh,
-                            v4i* el) {
-        const v16i z = scores<DC>(keys, extra, mine, block, lane, a.s1, a.s2, plain);
+    // exponentials of 32 tokens with scores z(r), all of which are seen or those below the lane's limit
+    auto exponentials = [&](auto&& z, int token, bool whole, v4i* eh, v4i* el) {
         uint32_t e[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[r]), last)];
-        if (token + 32 > all) {
+        for (int r = 0; r < 16; ++r) e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z(r)), last)];
+        if (!whole) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 if (token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= limit) e[r] = 0;
@@ -490,6 +511,11 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
             sum_h = __builtin_amdgcn_sdot4((*eh)[g], 0x01010101, sum_h, false);
             sum_l = __builtin_amdgcn_sdot4((*el)[g], 0x01010101, sum_l, false);
         }
+    };
+    auto block_exponentials = [&](const unsigned char* keys, const int* extra, int block, int token, bool plain, v4i* eh,
+                                  v4i* el) {
+        const v16i z = scores<DC>(keys, extra, mine, block, lane, a.s1, a.s2, plain);
+        exponentials([&](int r) { return z[r]; }, token, token + 32 <= all, eh, el);
     };
     // the 64 places' values of a block of 32 tokens
     struct Values {
@@ -520,8 +546,7 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
         for (int i = 0; i < AHEAD; ++i)
             if (mine_of(i) < tiles) stage_keys(mine_of(i), parts[2 * i], extras[i]), stage_values(mine_of(i), parts[2 * i + 1]);
         int now = 0;
-        for (int i = 0; i < turns; ++i) {
-            const int t = mine_of(i);
+        auto begin = [&](int i) {
             if (mine_of(i + 1) < tiles)
                 lds_copies_done<KEYS_COPIES + VALUES_COPIES>();
             else
@@ -532,6 +557,33 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
                 stage_keys(mine_of(i + AHEAD), parts[2 * next], extras[next]);
                 stage_values(mine_of(i + AHEAD), parts[2 * next + 1]);
             }
+        };
+        // Tiles that all rows see, as long as they need no offset: without branches,
+        // the second block's products under way before the first's sums, and its
+        // vector work beside them.
+        bool begun = false;
+        int i = 0;
+        for (; i < turns; ++i) {
+            begin(i);
+            const int t = mine_of(i);
+            begun = true;
+            if (a.s2 || (t + 1) * FX_TILE > all || !is_plain(t, extras[now])) break;
+            v4i eh, el;
+            const Raw s0 = products<DC>(parts[2 * now], mine, 0, lane);
+            const Values v0 = read(parts[2 * now + 1], 0);
+            exponentials([&](int r) { return score(s0, r, a.s1); }, 0, true, &eh, &el);
+            const Raw s1 = products<DC>(parts[2 * now], mine, 1, lane);
+            add(v0, eh, el);
+            const Values v1 = read(parts[2 * now + 1], 1);
+            exponentials([&](int r) { return score(s1, r, a.s1); }, 0, true, &eh, &el);
+            add(v1, eh, el);
+            now = now == 2 ? 0 : now + 1;
+            begun = false;
+        }
+        for (; i < turns; ++i) {
+            if (!begun) begin(i);
+            begun = false;
+            const int t = mine_of(i);
             if (TEAMS == 2 && t >= tiles) break;
             const bool plain = is_plain(t, extras[now]);
 #pragma unroll
@@ -539,7 +591,7 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
                 const int token = t * FX_TILE + block * 32;
                 if (token >= some) continue;
                 v4i eh, el;
-                exponentials(parts[2 * now], extras[now], block, token, plain, &eh, &el);
+                block_exponentials(parts[2 * now], extras[now], block, token, plain, &eh, &el);
                 add(read(parts[2 * now + 1], block), eh, el);
             }
             now = now == 2 ? 0 : now + 1;
@@ -577,7 +629,7 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
             const int token = t * FX_TILE + part * 32;
             v4i eh = {}, el = {};
             if (token < some)
-                exponentials(parts[t & 1], extras[t & 1], part, token, is_plain(t, extras[t & 1]), &eh, &el);
+                block_exponentials(parts[t & 1], extras[t & 1], part, token, is_plain(t, extras[t & 1]), &eh, &el);
             swap[wave * 128 + lane] = eh;
             swap[wave * 128 + 64 + lane] = el;
             begin(phase++);
