@@ -137,6 +137,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
     __shared__ __attribute__((aligned(1024)))
     unsigned char lds[STAGES * STAGE > BM * OUT_STRIDE * 2 ? STAGES * STAGE : BM * OUT_STRIDE * 2];
     __shared__ int x_sum[BM];
+    __shared__ int64_t column[BN];
+    static_assert(BN <= 64 * WAVES, "a column a thread");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
     const int steps = (a.k + 63) / 64, blocks = (a.n + 15) / 16;
@@ -191,19 +193,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
     };
 
     const int64_t* offs = reinterpret_cast<const int64_t*>(a.weights + static_cast<size_t>(blocks) * steps * 2048);
-    // Row sums of x are needed where a weight of the tile needed its offset.
     const int* o = reinterpret_cast<const int*>(offs + static_cast<size_t>(blocks) * 16);
-    bool offset = false;
-    for (int b = block0; b < min(block0 + BN / 16, blocks); ++b) offset |= o[b] != 0;
+    // On their way before the first copies, awaited after them: whether a weight of
+    // the tile needed its offset, and the columns' constants.
+    const int lane_o = lane < BN / 16 && block0 + lane < blocks ? o[block0 + lane] : 0;
+    const int my_col = block0 * 16 + static_cast<int>(threadIdx.x);
+    int64_t mine = 0;
+    int bias = 0;
+    if (threadIdx.x < BN && my_col < a.n) {
+        mine = offs[my_col];
+        if (a.bias) bias = a.bias[my_col];
+    }
 
-    v16i hh[I][J] = {}, mid[I][J] = {}, ll[I][J] = {};
-    int sums[I] = {};
     // A lane's fragment of 32 rows (or columns) and half u of the step: its row is
     // lane & 31, its 16 places start at 32 u + 16 (lane >> 5).
     const int in_block = ((lane >> 4) & 1) * 128 + (lane >> 5) * 16 + (lane & 15);
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s)
         if (s < steps) stage(s, lds + s * STAGE);
+    const bool offset = __any(lane_o);  // then row sums of x are needed
+    if (threadIdx.x < BN) {
+        mine += static_cast<int64_t>(bias) << a.bias_shift;
+        column[threadIdx.x] = !a.raw && a.shift ? mine + (int64_t{1} << (a.shift - 1)) : mine;
+    }
+    v16i hh[I][J] = {}, mid[I][J] = {}, ll[I][J] = {};
+    int sums[I] = {};
     int now_at = 0, next_at = (STAGES - 1) * STAGE;
     for (int s = 0; s < steps; ++s) {
         // This step's copies have landed for all waves, and all have left the
@@ -251,22 +265,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
     __syncthreads();  // and the last step's buffer is free
 
     int16_t* done = reinterpret_cast<int16_t*>(lds);
-    // Every place with its three sums, its column's constant and its row's sum of x.
+    if (offset) {
+        // 128 sum x, as 2^16 (sum >> 9) + 2^7 (sum & 511), joins the outer sums
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int col = block0 * 16 + (wn * J + j) * 32 + (lane & 31), mask = col < a.n && o[col >> 4] ? -1 : 0;
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int sum = x_sum[(wm * I + i) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] & mask;
+                    hh[i][j][r] += sum >> 9;
+                    ll[i][j][r] += (sum & 511) << 7;
+                }
+        }
+    }
+    // Every place with its three sums and its column's constant.
     auto each = [&](auto&& use) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int place = (wn * J + j) * 32 + (lane & 31), col = block0 * 16 + place;
-            int64_t off = col < a.n ? offs[col] : 0;
-            if (a.bias && col < a.n) off += static_cast<int64_t>(a.bias[col]) << a.bias_shift;
-            if (!a.raw && a.shift) off += int64_t{1} << (a.shift - 1);
-            const int64_t more = offset && col < a.n ? o[col >> 4] : 0;
+            const int place = (wn * J + j) * 32 + (lane & 31);
+            if (block0 * 16 + place >= a.n) continue;
+            const int64_t off = column[place];
 #pragma unroll
             for (int i = 0; i < I; ++i) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int row = (wm * I + i) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                    use(row, place, hh[i][j][r], mid[i][j][r], ll[i][j][r],
-                        offset ? off + more * x_sum[row] : off);
+                    use(row, place, hh[i][j][r], mid[i][j][r], ll[i][j][r], off);
                 }
             }
         }
@@ -284,14 +310,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
         // 0 <= low < 2^16 and high in 32 bits, and its shift needs no 64-bit
         // arithmetic (under a shift below 16, high is clamped first: past 15 bits
         // the result is clamped whatever they are).
-        const int up = a.shift < 16 ? 16 - a.shift : 0, down = a.shift < 16 ? a.shift : 16,
-                  more = a.shift < 16 ? 0 : a.shift - 16;
-        each([&](int row, int col, int h, int m, int l, int64_t off) {
-            const int t = ((m & 255) << 8) + l + static_cast<int>(off & 0xffff);
-            int high = h + (m >> 8) + static_cast<int>(off >> 16) + (t >> 16);
-            high = up ? (min(max(high, -32768), 32767) << up) + ((t & 0xffff) >> down) : high >> more;
-            done[row * OUT_STRIDE + col] = static_cast<int16_t>(min(max(high, -32768), 32767));
-        });
+        auto put = [&](int row, int col, int v) {
+            done[row * OUT_STRIDE + col] = static_cast<int16_t>(min(max(v, -32768), 32767));
+        };
+        auto low = [](int m, int l, int64_t off) { return ((m & 255) << 8) + l + static_cast<int>(off & 0xffff); };
+        auto high = [](int h, int m, int t, int64_t off) {
+            return h + (m >> 8) + static_cast<int>(off >> 16) + (t >> 16);
+        };
+        if (a.shift >= 16) {
+            const uint32_t more = a.shift - 16;
+            each([&](int row, int col, int h, int m, int l, int64_t off) {
+                put(row, col, high(h, m, low(m, l, off), off) >> more);
+            });
+        } else {
+            const uint32_t up = 16 - a.shift;
+            each([&](int row, int col, int h, int m, int l, int64_t off) {
+                const int t = low(m, l, off);
+                put(row, col, (min(max(high(h, m, t, off), -32768), 32767) << up) + ((t & 0xffff) >> a.shift));
+            });
+        }
     } else {
         each([&](int row, int col, int h, int m, int l, int64_t off) {
             done[row * OUT_STRIDE + col] = static_cast<int16_t>(sat16((join(h, m, l) + off) >> a.shift));
