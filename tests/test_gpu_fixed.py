@@ -305,6 +305,15 @@ def test_attention_tokens_over_a_cache(backend, n, dim, new):
     check_attention(backend, n + new, [new, 1, new], [n, max(1, n // 3), max(new, n - 1)], 4, 2, dim)
 
 
+@pytest.mark.parametrize("batch,longest,heads,kv_heads,dim", [
+    (40, 300, 16, 8, 64), (9, 1300, 12, 12, 64), (2, 1300, 2, 2, 64), (9, 1300, 12, 12, 128), (70, 3300, 2, 1, 64),
+    (130, 700, 3, 1, 80)])
+def test_attention_tokens_of_many_sequences(backend, batch, longest, heads, kv_heads, dim):
+    """Few and many sequences a launch, and several launches, with lengths from one token to the longest."""
+    lengths = [max(1, longest * ((7 * i) % 11) // 11) if i else longest for i in range(batch)]
+    check_attention(backend, batch, [1] * batch, lengths, heads, kv_heads, dim)
+
+
 @pytest.mark.parametrize("new", [17, 40, 100, 200])
 def test_attention_prompts_in_pieces(backend, new):
     check_attention(backend, new, [new, 1, new + 3], [new + 700, 333, new + 64], 4, 1, 64)
@@ -496,6 +505,16 @@ def test_norm(backend, rows, cols, residual, rms):
             want, want_h = ref.norm(x, gain, shift, eps, bias=bias, residual=res, rms=rms)
             assert np.array_equal(y[:, :cols], want) and (y[:, cols:] == 6).all()
             assert np.array_equal(h[:, :cols], want_h) and (h[:, cols:] == 5).all()
+
+
+@pytest.mark.parametrize("cols", [512, 513, 1024, 1500, 2049, 4096, 4097])
+def test_norm_widths(backend, cols):
+    g = gen(cols)
+    x, gain, bias = normal(g, (5, cols), 3000), full(g, cols), full(g, cols)
+    with Held(backend) as held:
+        out = held.keep(backend.fixed_norm_device(held.put(x), 5, cols, held.put(gain), 3, cols, bias=held.put(bias)))
+        got = backend.download_device(out).reshape(5, cols)
+    assert np.array_equal(got, ref.norm(x, gain, 3, cols, bias=bias)[0])
 
 
 @pytest.mark.parametrize("cols", [2, 768, 65536])

@@ -366,9 +366,10 @@ struct Table {
 // With heads up to 64 (DC = 1) a workgroup is one or two teams of four waves, 32
 // rows a wave.  Two teams take the tiles in turn, each with buffers of its own,
 // and join their maxima and sums through LDS: where workgroups are few the
-// longest one decides, and it is done sooner (one 1,024-token prompt, 12 heads:
-// 47 us with one team, 35 us with two; sixteen of them: 131 and 151 us, as two
-// workgroups a CU hide each other's waits better).
+// longest one decides, and it is done sooner; elsewhere two workgroups a CU hide
+// each other's waits better.  Prompts of 1,024 tokens, 12 heads, us with one team
+// and with two: one 42.7 and 32.9, four (384 workgroups) 48.1 and 40.1, six (576)
+// 52.9 and 61.3, sixteen 118 and 134.
 //
 // With heads over 64 (DC = 2) the two waves of a group take 32 tokens of a tile
 // each, exchange the exponentials through LDS, and keep half of the result's
@@ -1019,21 +1020,44 @@ int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::
 }
 
 // 1 where its space may not grow: the other kernel needs none.
-int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_t tiles, size_t cols, size_t units) {
+int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_t tiles, size_t cols) {
     std::sort(seqs.begin(), seqs.end(), [](const FxSeq& x, const FxSeq& y) { return x.length > y.length; });
+    size_t units = 0;  // of the largest launch: each reuses the space, as they run in order
+    for (size_t at = 0; at < seqs.size(); at += FX_SEQS) {
+        size_t rows = 0;
+        for (size_t i = at; i < seqs.size() && i < at + FX_SEQS; ++i)
+            rows += (size_t{seqs[i].count} * a.group + FEW - 1) / FEW;
+        units = std::max(units, rows * a.kv_heads);
+    }
     FewArgs f{};
     f.cols = static_cast<int>(cols);
     f.max_tiles = static_cast<int>(std::max<size_t>(tiles, 1));
     f.splits = 1;
     const size_t score_bytes = f.max_tiles * cols * 256;
-    const size_t waves = a.dim <= 64 ? FEW_WAVES<1, ONE> : FEW_WAVES<2, ONE>;
-    const Pass pass = tiles <= waves                                                                    ? ONE
-                      : score_bytes <= 65536 && (tiles <= 16 || units >= static_cast<size_t>(c->cu_count)) ? FUSED
-                                                                                                        : SCORES;
+    // us, one token a sequence, for units x tiles with heads of 64 (of 128):
+    //   units x tiles       ONE        FUSED        split
+    //   12 x 4              8.8        8.4 (10.9)   15.1
+    //   12 x 16             9.9        12.5         15.7
+    //   192 x 16            13.9       17.8         23.9
+    //   512 x 16            30.7       27.4         39.1
+    //   12 x 32                        19.9 (25.0)  16.8 (18.3)
+    //   192 x 32                       28.1 (40.2)  43.1 (66.0)
+    //   12 x 128                       73.0 (96.7)  21.8 (26.5)
+    //   192 x 128                      112 (184)    133 (246)
+    // ONE, with heads over 64, is 0.3 to 2 us ahead of FUSED up to its 8 tiles.
+    // Two launches more cost 10 us; what they save is a tile's time alone on a CU,
+    // 0.55 us (0.75), less its share of the whole card's, 5 ns (9) a unit.
+    const bool wide = a.dim > 64;
+    const int64_t alone = wide ? 750 : 550, shared = wide ? 9 : 5;
+    Pass pass = SCORES;
+    if (wide ? tiles <= FEW_WAVES<2, ONE> : tiles > 4 && tiles <= FEW_WAVES<1, ONE> && units <= static_cast<size_t>(c->cu_count))
+        pass = ONE;
+    else if (score_bytes <= 65536 &&
+             static_cast<int64_t>(tiles) * (alone - shared * static_cast<int64_t>(units)) <= 10000)
+        pass = FUSED;
     if (pass == SCORES) {
         const size_t want = (2 * c->cu_count + units - 1) / units, most = (tiles + 7) / 8;
         f.splits = static_cast<int>(std::max<size_t>(1, std::min(want, most)));
-        // every group of sequences reuses the space: its launches are in order
         const size_t z = units * score_bytes, tops = units * f.splits * FEW * 4;
         const size_t sums = units * f.splits * cols * (a.dim <= 64 ? 65 : 129) * 8;
         if (!try_ws(c, WS_FIXED, z + sums + tops)) return 1;
@@ -1102,7 +1126,7 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
     const bool split = by_tiles + 5000 < std::max(by_rows, longest) && units * tiles * FEW * 256 <= size_t{1} << 29;
     std::vector<FxSeq> many, few;
     size_t cols = 0;
-    tiles = units = 0;
+    tiles = 0;
     for (size_t i = 0; i < count; ++i) {
         const FxSeq& s = seqs[i];
         if (rows_of(s) > FEW && !split) {
@@ -1113,10 +1137,9 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
         few.push_back(s);
         tiles = std::max<size_t>(tiles, (s.length + FX_TILE - 1) / FX_TILE);
         cols = std::max<size_t>(cols, std::min<size_t>(rows_of(s), FEW));
-        units += (rows_of(s) + FEW - 1) / FEW * cache.kv_heads;
     }
     if (!few.empty()) {
-        const int rc = few_rows(c, a, few, tiles, cols, units);
+        const int rc = few_rows(c, a, few, tiles, cols);
         if (rc < 0) return -1;
         if (rc) {
             many.assign(seqs, seqs + count);
