@@ -235,13 +235,20 @@ void launch_norm(Context* c, const FxNorm& a) {
 
 }  // namespace
 
+// A row a wave while the wave can keep it: no barrier.  16,384 rows, us by a wave
+// and by 256 threads a row: 512 columns 11.7 and 20.2, 768 18.2 and 26.9, 2,048 32.7
+// and 38.5.  With 256 threads, kept and read twice: 4,096 columns 61.5 and 67.5,
+// 8,192 131 and 151.  Pieces no row has cost too (768 columns in four pieces a
+// thread 54.6), so there are widths in between.
 int fx_norm(Context* c, const FxNorm& a) {
     if (a.cols <= 512)
         launch_norm<64, 1>(c, a);
     else if (a.cols <= 1024)
         launch_norm<64, 2>(c, a);
     else if (a.cols <= 2048)
-        launch_norm<256, 1>(c, a);
+        launch_norm<64, 4>(c, a);
+    else if (a.cols <= 4096)
+        launch_norm<256, 2>(c, a);
     else if (a.cols <= 8192)
         launch_norm<256, 4>(c, a);
     else
@@ -252,9 +259,18 @@ int fx_norm(Context* c, const FxNorm& a) {
 
 int fx_embed(Context* c, const FxEmbed& a) {
     const uint32_t pieces = static_cast<uint32_t>((a.cols + 7) / 8);
-    hipLaunchKernelGGL(fx_embed_kernel, dim3(static_cast<unsigned>((a.rows * pieces + 255) / 256)), dim3(256), 0, c->stream, a,
-                       pieces);
-    VMX_HIP(c, hipGetLastError());
+    // a launch holds less than 2^32 threads
+    const size_t most = std::max<size_t>(1, (size_t{1} << 31) / pieces);
+    FxEmbed part = a;
+    for (size_t row = 0; row < a.rows; row += most) {
+        part.tokens = a.tokens + row;
+        part.positions = a.positions ? a.positions + row : nullptr;
+        part.out = a.out + row * a.out_stride;
+        part.rows = std::min(most, a.rows - row);
+        hipLaunchKernelGGL(fx_embed_kernel, dim3(static_cast<unsigned>((part.rows * pieces + 255) / 256)), dim3(256), 0,
+                           c->stream, part, pieces);
+        VMX_HIP(c, hipGetLastError());
+    }
     return 0;
 }
 
