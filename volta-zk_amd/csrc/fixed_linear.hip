@@ -392,32 +392,36 @@ int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t str
     return 0;
 }
 
-// Which kernel.  us for k x n on the rows given, in a loop (6 us of them the call):
+// Which kernel.  us for k x n on the rows given, in a loop (5 us of them the call):
 //                          16-row    64 x 64,  64 x 64,  128 x 128,  128 x 128,
 //                                    4 stages  2 stages  8 waves, 4  4 waves, 2
-//   3072 x 768, 200 rows   13.7      20.9      24.5      42.3        56.4
-//   768 x 4096, 200        16.1      9.7       10.3      16.8        20.8
-//   768 x 50257, 48        37.4      23.3      20.4      33.0        30.3
-//   768 x 4096, 800        49.6      23.6      21.5      19.4        22.9
-//   768 x 768, 6,000       66.0      27.7      25.6      32.9        28.9
-//   3072 x 768, 1,600      67.4      34.1      34.3      42.8        57.2
-//   768 x 4096, 6,000      325       118       106       111         89.9
-//   768 x 50257, 1,600               372       348       357         292
+//   768 x 4096, 48 rows    6.2       8.4       8.4       14.0        16.1
+//   3072 x 768, 200        13.8      20.2      23.2      41.4        52.3
+//   768 x 4096, 200        16.0      9.1       9.5       15.4        17.6
+//   3072 x 768, 800        39.0      21.5      32.5      41.7        53.1
+//   768 x 50257, 48        37.8      21.4      19.3      30.4        26.3
+//   768 x 4096, 800        51.3      22.3      21.3      20.1        22.0
+//   3072 x 768, 3,200      133       49.9      47.0      43.4        53.5
+//   768 x 768, 6,000       72.0      27.7      26.1      31.7        26.4
+//   3072 x 768, 6,000      238       80.5      84.2      88.0        76.1
+//   768 x 3072, 6,000      253       88.4      80.7      81.2        65.4
+//   768 x 4096, 16,384               329       278       259         211
 // The 16-row kernel reads the packed weights once for 16 rows and splits k over
-// its waves: it wins while its workgroups are few, and always for 16 rows.  Few
-// tiles want depth of prefetch, a tile a CU wants eight waves on it, and past
-// that two workgroups a CU hide each other's waits.  The costs are those of a
-// step (in 1/120 us), by tiles on 256 CUs, that the measurements above show.
+// its waves: it wins up to about 1,400 workgroups, and always for 16 rows.  A
+// small tile a CU wants depth of prefetch, a large one eight waves on it, and past
+// that two workgroups a CU hide each other's waits.  The estimates, in ns from the
+// calls above, are a start and an end plus so much a step, by tiles on each CU.
 int fx_linear(Context* c, const FxLinear& a) {
-    const size_t blocks = fx_blocks(a.n), steps = fx_steps(a.k), row_blocks = (a.rows + 15) / 16;
+    const size_t blocks = fx_blocks(a.n), steps = fx_steps(a.k), row_blocks = (a.rows + 15) / 16, cus = c->cu_count;
     const size_t small = ((blocks + 3) / 4) * ((row_blocks + 3) / 4), large = ((blocks + 7) / 8) * ((row_blocks + 7) / 8);
-    const size_t cus = c->cu_count;
-    const size_t deep = small <= cus ? 33 : small <= 2 * cus ? 80 : SIZE_MAX;
-    const size_t pairs = std::max<size_t>(43, 46 * small / cus);
-    const size_t waves8 = large <= cus ? 133 : 170 * ((large + cus - 1) / cus);
-    const size_t two = large <= cus ? 140 : 270 * ((large + 2 * cus - 1) / (2 * cus));
+    const size_t turns = (large + cus - 1) / cus;
+    const size_t deep = small <= cus ? 5000 + 325 * steps : SIZE_MAX;
+    const size_t pairs = 6000 + std::max<size_t>(600, 350 * small / cus) * steps;
+    const size_t waves8 = turns == 1 ? 7500 + 710 * steps : turns * (6500 + 780 * steps);
+    const size_t two = turns == 1 ? 5700 + 960 * steps : turns * (4700 + 690 * steps) + turns % 2 * 350 * steps;
     const size_t least = std::min(std::min(deep, pairs), std::min(waves8, two));
-    if (row_blocks == 1 || (row_blocks <= 1024 && blocks * row_blocks <= 1400 * std::max<size_t>(1, small / (2 * cus)))) {
+    if (row_blocks == 1 || blocks * row_blocks <= 1400) {
+        // 1 x 3,072 x 768: 6.3 us with 4 waves, 5.7 with 16; 1 x 768 x 50,257: 13.6 and 14.9
         const unsigned waves = static_cast<unsigned>(std::min<size_t>(steps, blocks * row_blocks < cus ? 16 : 4));
         hipLaunchKernelGGL(fx_linear_rows_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(row_blocks)),
                            dim3(64 * waves), 0, c->stream, a);
