@@ -21,7 +21,8 @@
  * Symbols marked "out of scope here" belong to the reference's GEMM,
  * fixed-point inference, LogUp and X4c arena/session subsystems; they are
  * exported with their exact signatures so the loader resolves them, and fail
- * explicitly when called.
+ * explicitly when called.  The fixed-point model operators at the end of this
+ * header are entry points of their own, with no counterpart in the reference.
  */
 #ifndef VOLTA_CUDA_ABI_H
 #define VOLTA_CUDA_ABI_H

@@ -12,7 +12,9 @@ using namespace fx;
 
 // ---- packing -------------------------------------------------------------------------
 // One workgroup per 16 columns: once for their largest value, then its waves
-// take the steps of 64 rows in turn.  3072 x 768: 20 us on 48 workgroups.
+// take the steps of 64 rows in turn.  Done once for a model's weights; bound by
+// latency where columns are few: 3,072 x 768 (4.7 MB) 27 us on 48 workgroups,
+// 768 x 50,257 (77 MB) 110 us, 1.4 TB/s read plus written.
 __global__ __launch_bounds__(1024) void fx_pack_weights_kernel(const int16_t* w, int k, int n, size_t stride,
                                                                bool transposed, unsigned char* out, size_t blocks) {
     __shared__ int most;
@@ -75,7 +77,9 @@ __device__ inline void finish(const FxLinear& a, size_t row, int col, int64_t su
 // ---- few rows ------------------------------------------------------------------------
 // A workgroup computes 16 rows of 16 columns; its waves take the steps of 64
 // along k in turn, each streaming its part of the packed weights once, and add
-// their i64 sums in LDS.
+// their i64 sums in LDS.  Bound by the weights: 7 rows of 768 x 50,257 (77 MB, and
+// 2.8 MB of sums) 13.8 us, 5.8 TB/s, as the weights stay in the last-level cache;
+// one row of 3,072 x 768 4.6 us, a launch and one trip to memory a step.
 __global__ __launch_bounds__(1024) void fx_linear_rows_kernel(FxLinear a) {
     __shared__ unsigned long long total[256];
     __shared__ int x_sum[16];
@@ -122,6 +126,11 @@ __global__ __launch_bounds__(1024) void fx_linear_rows_kernel(FxLinear a) {
 // fragments into planes as it reads them.  Fragments lie in LDS in the order the
 // lanes read them.
 //
+// Large products are bound by the matrix cores, whose clock falls with the data:
+// 16,384 x 768 x 4,096 takes 208 us, 1.98 POP/s of i8 work (a library i8 product of
+// 16,384^3 reaches 2.33), and took 186 of then 235 us on weights of zero.  At one tile
+// a CU the steps' waits bound it: 1,023 x 768 x 3,072 20.4 us, matrix cores busy 0.14.
+//
 // x is copied in pieces of 8 elements when every piece is 16-byte aligned
 // (`Aligned`), else through registers.  Places past k of a row's last piece may
 // then hold anything: their weights are 0, and the identity of fixed.hpp holds
@@ -142,12 +151,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
     const int steps = (a.k + 63) / 64, blocks = (a.n + 15) / 16;
-    // Workgroups go to the XCDs in turn: each XCD takes a run of neighbouring
-    // tiles, so that their rows and columns meet in its L2.
+    // Workgroups go to the XCDs in turn: each XCD takes a run of tiles, which go
+    // down panels of 1,024 columns, so that what its CUs work on at one time shares
+    // rows and columns in its L2 (16,384 x 768 x 4,096 by whole rows of tiles, whose
+    // 6.3 MB of weights an L2 does not hold: 224 us, by panels 208).
+    constexpr unsigned PANEL = 1024 / BN;
     const unsigned tiles = row_tiles * col_tiles, per = (tiles + 7) / 8;
     const unsigned tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (tile >= tiles) return;
-    const unsigned rt = tile / col_tiles, ct = tile % col_tiles;
+    const unsigned panel = tile / (PANEL * row_tiles), place = tile - panel * PANEL * row_tiles;
+    const unsigned across = min(PANEL, col_tiles - panel * PANEL);
+    const unsigned rt = place / across, ct = panel * PANEL + place % across;
     const size_t row0 = static_cast<size_t>(rt) * BM;
     const int rows = static_cast<int>(a.rows - row0 < BM ? a.rows - row0 : BM);
     const int block0 = static_cast<int>(ct) * (BN / 16);
@@ -396,16 +410,16 @@ int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t str
 //                          16-row    64 x 64,  64 x 64,  128 x 128,  128 x 128,
 //                                    4 stages  2 stages  8 waves, 4  4 waves, 2
 //   768 x 4096, 48 rows    6.2       8.4       8.4       14.0        16.1
-//   3072 x 768, 200        13.8      20.2      23.2      41.4        52.3
+//   3072 x 768, 200        13.8      21.4      23.4      40.6        52.9
 //   768 x 4096, 200        16.0      9.1       9.5       15.4        17.6
-//   3072 x 768, 800        39.0      21.5      32.5      41.7        53.1
-//   768 x 50257, 48        37.8      21.4      19.3      30.4        26.3
-//   768 x 4096, 800        51.3      22.3      21.3      20.1        22.0
-//   3072 x 768, 3,200      133       49.9      47.0      43.4        53.5
-//   768 x 768, 6,000       72.0      27.7      26.1      31.7        26.4
-//   3072 x 768, 6,000      238       80.5      84.2      88.0        76.1
-//   768 x 3072, 6,000      253       88.4      80.7      81.2        65.4
-//   768 x 4096, 16,384               329       278       259         211
+//   3072 x 768, 800        39.2      23.0      32.8      40.5        53.2
+//   768 x 50257, 48        38.8      21.8      19.6      30.3        25.9
+//   768 x 4096, 800        51.2      22.3      20.8      17.8        19.8
+//   3072 x 768, 3,200      133       51.9      48.1      43.8        54.3
+//   768 x 768, 6,000       70.6      28.7      26.2      32.1        27.0
+//   3072 x 768, 6,000      238       81.5      84.8      86.9        76.5
+//   768 x 3072, 6,000      255       86.7      75.8      77.6        64.8
+//   768 x 4096, 16,384               310       261       231         201
 // The 16-row kernel reads the packed weights once for 16 rows and splits k over
 // its waves: it wins up to about 1,400 workgroups, and always for 16 rows.  A
 // small tile a CU wants depth of prefetch, a large one eight waves on it, and past
