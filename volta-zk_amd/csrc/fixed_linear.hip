@@ -127,9 +127,11 @@ __global__ __launch_bounds__(1024) void fx_linear_rows_kernel(FxLinear a) {
 // lanes read them.
 //
 // Large products are bound by the matrix cores, whose clock falls with the data:
-// 16,384 x 768 x 4,096 takes 208 us, 1.98 POP/s of i8 work (a library i8 product of
-// 16,384^3 reaches 2.33), and took 186 of then 235 us on weights of zero.  At one tile
-// a CU the steps' waits bound it: 1,023 x 768 x 3,072 20.4 us, matrix cores busy 0.14.
+// 16,384 x 768 x 4,096 takes 202 to 220 us, 1.9 to 2.0 POP/s of i8 work (a library i8
+// product of 16,384^3 reaches 2.33), and took 186 of then 235 us on weights of zero.
+// At one tile a CU the steps' waits bound it: 1,023 x 768 x 3,072 17.7 us, 20.8 with a
+// table, whose lookups are bound by their rate (four times as many under way together
+// took as long); matrix cores busy 0.14.
 //
 // x is copied in pieces of 8 elements when every piece is 16-byte aligned
 // (`Aligned`), else through registers.  Places past k of a row's last piece may
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
     // Workgroups go to the XCDs in turn: each XCD takes a run of tiles, which go
     // down panels of 1,024 columns, so that what its CUs work on at one time shares
     // rows and columns in its L2 (16,384 x 768 x 4,096 by whole rows of tiles, whose
-    // 6.3 MB of weights an L2 does not hold: 224 us, by panels 208).
+    // 6.3 MB of weights an L2 does not hold: 212 us, by panels 202).
     constexpr unsigned PANEL = 1024 / BN;
     const unsigned tiles = row_tiles * col_tiles, per = (tiles + 7) / 8;
     const unsigned tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
