@@ -105,6 +105,61 @@ def test_linear_epilogue(backend, rows, k, n):
     assert np.array_equal(run_linear(backend, x, w, **kw), ref.linear(x, w, **kw))
 
 
+def check_linear_tiles(b, rows, k, n, large, seed=0):
+    """Sums and an epilogue of every part, with weights (and x) over all of i16 or of ordinary size; the reference's sums
+    are exact in doubles."""
+    g = gen(rows + k + n + seed)
+    x, w = (full(g, (rows, k)), full(g, (k, n))) if large else (normal(g, (rows, k), 1000), normal(g, (k, n), 2000))
+    acc = ref._sums(x, w)
+    shift = 31 if large else int(np.log2(2e6 * np.sqrt(k) / 9000))
+    for s in (shift, min(shift, 11)):
+        kw = dict(bias=full(g, n), bias_shift=9, shift=s, table=full(g, 65536), residual=full(g, (rows, n)))
+        h = ref.sat(ref.rs(acc + kw["bias"].astype(np.int64) * 512, s))
+        h = ref.sat(kw["table"].astype(np.int64)[h + 32768] + kw["residual"].astype(np.int64))
+        assert np.array_equal(run_linear(b, x, w, **kw), h)
+    assert np.array_equal(run_linear(b, x, w, raw=True, out_gap=3), acc)
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("rows,k,n", [
+    (800, 136, 500), (801, 131, 497), (1500, 104, 1200), (1499, 99, 1201), (1600, 520, 2000), (1543, 509, 1990),
+    (4090, 200, 2040), (4081, 199, 2033), (17, 64, 12000)])
+def test_linear_of_many_rows_and_columns(backend, rows, k, n, large):
+    """Tiles of every size, whole ones and those at the edges, with rows aligned and not."""
+    check_linear_tiles(backend, rows, k, n, large)
+
+
+def test_without_workspaces_in_a_coarse_scope():
+    """Rows that are not aligned, and few rows of a long sequence, where no workspace may be allocated."""
+    from volta_mi355x import Backend
+    g = gen(77)
+    x, w = normal(g, (801, 131), 1000), normal(g, (131, 497), 2000)
+    q, k, v = normal(g, (1, 2, 64), 1000), normal(g, (3000, 2, 64), 1000), normal(g, (3000, 2, 64), 3000)
+    with Backend(timing_policy=1) as b, Held(b) as held:
+        dx, dq, table = held.put(x), held.put(q), held.put(exponentials())
+        packed = b.fixed_weights_device(held.put(w), 131, 497)
+        held.keep(packed.storage)
+        cache = b.fixed_kv_cache(1, 2, 64, 3000)
+        held.keep(cache.storage)
+        b.fixed_kv_append_device(cache, held.put(k), held.put(v), [[0, 0, 3000, 3000]])
+        y, o = held.new(801 * 497, np.int16), held.new(128, np.int16)
+        live = b.get_stats()["live_device_bytes"]
+        for run in (lambda: b.fixed_linear_device(dx, 801, packed, 12, out=y),
+                    lambda: b.fixed_attention_device(dq, cache, [[0, 0, 1, 3000]], 2, table, 13, out=o)):
+            assert b.lib.volta_cuda_begin_coarse_timing(b.raw, 0) == 0
+            run()
+            assert b.lib.volta_cuda_end_coarse_timing(b.raw) == 0
+        assert b.get_stats()["live_device_bytes"] == live
+        first = b.download_device(y).reshape(801, 497), b.download_device(o)
+        b.fixed_linear_device(dx, 801, packed, 12, out=y)
+        b.fixed_attention_device(dq, cache, [[0, 0, 1, 3000]], 2, table, 13, out=o)
+        assert b.get_stats()["live_device_bytes"] > live
+        second = b.download_device(y).reshape(801, 497), b.download_device(o)
+    want = ref.sat(ref.rs(ref._sums(x, w), 12)), ref.attention(q, k, v, exponentials(), 13, True).reshape(-1)
+    for got in (first, second):
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("use", ["", "bias", "table", "residual", "bias table", "bias residual", "table residual"])
 @pytest.mark.parametrize("rows,k,n", [(5, 100, 40), (200, 100, 150)])
 def test_linear_optional_parts(backend, rows, k, n, use):

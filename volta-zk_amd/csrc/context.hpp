@@ -179,7 +179,7 @@ enum WorkspaceSlot : int {
     WS_AUX2 = 5,      // combination coefficient sums
     WS_HASH = 6,      // Merkle column-group chaining values
     WS_FLAGS = 7,     // rejected-draw flags of ChaCha8 rows (zero between calls)
-    WS_FIXED = 8,     // scores and sums of attention over a split cache
+    WS_FIXED = 8,     // scores and sums of attention over a split cache; aligned rows of a product
     WS_COUNT = 9,
 };
 

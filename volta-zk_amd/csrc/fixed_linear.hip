@@ -118,6 +118,30 @@ __global__ __launch_bounds__(1024) void fx_linear_rows_kernel(FxLinear a) {
     }
 }
 
+// ---- rows that are not aligned ---------------------------------------------------------
+// x with rows of whole 16-byte pieces, a piece a thread.  What a row's last piece
+// holds past k is 0.
+__global__ __launch_bounds__(256) void fx_align_rows_kernel(const int16_t* x, size_t stride, size_t rows, int k,
+                                                            uint32_t pieces, v4i* out) {
+    const size_t id = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, row = id / pieces;
+    if (row >= rows) return;
+    const int at = static_cast<int>(id - row * pieces) * 8;
+    const int16_t* from = x + row * stride + at;
+    union {
+        v4i v;
+        int16_t e[8];
+    } u;
+    u.v = v4i{0, 0, 0, 0};
+    if (at + 8 <= k) {
+        u.v = load8(from);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (at + e < k) u.e[e] = from[e];
+    }
+    out[id] = u.v;
+}
+
 // ---- many rows -----------------------------------------------------------------------
 // A workgroup of WM x WN waves computes a tile of 32 WM I rows x 32 WN J
 // columns, each wave I x J blocks of 32 x 32.  Along k it takes steps of 64: the
@@ -383,11 +407,35 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
     }
 }
 
+// Whether the tile kernel may copy x in pieces; a tile's offsets have to fit 32 bits.
+bool aligned_rows(const FxLinear& a) {
+    return reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0 && a.x_stride < (size_t{1} << 22);
+}
+
+// a with its rows aligned in a workspace, or as it is where that may not grow: copies
+// through registers wait for memory in each step, and rows of other alignment take
+// twice the accesses (us without and with, the aligning included: 1,337 x 961 x 5,203
+// 68 and 43, 16,384 x 767 x 4,096 412 and 232, 1,023 x 767 x 3,072 34 and 22).
+FxLinear with_aligned_rows(Context* c, FxLinear a) {
+    const size_t pieces = (a.k + 7) / 8;
+    if (aligned_rows(a) || !try_ws(c, WS_FIXED, a.rows * pieces * 16)) return a;
+    v4i* to = ws<v4i>(c, WS_FIXED);
+    // a launch holds less than 2^32 threads
+    const size_t most = (size_t{1} << 31) / pieces;
+    for (size_t row = 0; row < a.rows; row += most) {
+        const size_t rows = std::min(most, a.rows - row);
+        hipLaunchKernelGGL(fx_align_rows_kernel, dim3(static_cast<unsigned>((rows * pieces + 255) / 256)), dim3(256), 0,
+                           c->stream, a.x + row * a.x_stride, a.x_stride, rows, a.k, static_cast<uint32_t>(pieces),
+                           to + row * pieces);
+    }
+    a.x = reinterpret_cast<const int16_t*>(to);
+    a.x_stride = pieces * 8;
+    return a;
+}
+
 template <int WM, int WN, int I, int J, int STAGES>
 void launch_tile(Context* c, const FxLinear& a) {
-    // Aligned also needs a tile's offsets to fit 32 bits.
-    const bool aligned =
-        reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0 && a.x_stride < (size_t{1} << 22);
+    const bool aligned = aligned_rows(a);
     constexpr int BM = 32 * WM * I, BN = 32 * WN * J;
     const unsigned rt = static_cast<unsigned>((a.rows + BM - 1) / BM), ct = static_cast<unsigned>((a.n + BN - 1) / BN);
     const dim3 grid((rt * ct + 7) / 8 * 8), threads(64 * WM * WN);
@@ -427,8 +475,14 @@ int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t str
 // small tile a CU wants depth of prefetch, a large one eight waves on it, and past
 // that two workgroups a CU hide each other's waits.  The estimates, in ns from the
 // calls above, are a start and an end plus so much a step, by tiles on each CU.
-int fx_linear(Context* c, const FxLinear& a) {
-    const size_t blocks = fx_blocks(a.n), steps = fx_steps(a.k), row_blocks = (a.rows + 15) / 16, cus = c->cu_count;
+int fx_linear(Context* c, const FxLinear& given) {
+    const size_t blocks = fx_blocks(given.n), steps = fx_steps(given.k), row_blocks = (given.rows + 15) / 16;
+    const size_t cus = c->cu_count;
+    // A launch to align rows costs about 3 us: 100 x 767 x 768 (4,032 steps of 16 x 16)
+    // 9.3 us without and 10.7 with, 20 x 3,001 x 768 (4,512) 11.9 and 9.9, 100 x 767 x
+    // 3,072 (16,128) 18.1 and 12.4.
+    const bool align = row_blocks > 1 && blocks * row_blocks * steps >= 4400;
+    const FxLinear a = align ? with_aligned_rows(c, given) : given;
     const size_t small = ((blocks + 3) / 4) * ((row_blocks + 3) / 4), large = ((blocks + 7) / 8) * ((row_blocks + 7) / 8);
     const size_t turns = (large + cus - 1) / cus;
     const size_t deep = small <= cus ? 5000 + 325 * steps : SIZE_MAX;
