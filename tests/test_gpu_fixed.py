@@ -536,6 +536,33 @@ def test_attention_cache_records_past_four_gib(backend):
         assert np.array_equal(got[part], ref.attention(q[part], k[part], v[part], exponentials(), 13, True))
 
 
+@pytest.mark.parametrize("policy", [0, 1])
+@pytest.mark.parametrize("kv_heads,length", [(1, 200), (1, 600), (2, 4000)])
+def test_attention_reports_a_failed_launch(policy, kv_heads, length):
+    """The check after a launch reads this thread's last HIP error, so an error left by a call before it takes
+    the way of a launch that fails: the call says so and runs no other kernel in its place."""
+    from volta_mi355x import Backend, GpuError
+    g = gen(length)
+    q, k, v = (normal(g, (n, kv_heads, 64), s) for n, s in ((1, 1000), (length, 1000), (length, 3000)))
+    with Backend(timing_policy=policy) as b, Held(b) as held:
+        cache = b.fixed_kv_cache(1, kv_heads, 64, length)
+        held.keep(cache.storage)
+        b.fixed_kv_append_device(cache, held.put(k), held.put(v), [[0, 0, length, length]])
+        dq, table, out = held.put(q), held.put(exponentials()), held.new(kv_heads * 64, np.int16)
+
+        def attend():
+            return b.fixed_attention_device(dq, cache, [[0, 0, 1, length]], kv_heads, table, 13, out=out)
+
+        attend()
+        b.synchronize()
+        assert b.lib.hipSetDevice(1 << 20) != 0
+        with pytest.raises(GpuError, match="hipGetLastError"):
+            attend()
+        attend()
+        assert np.array_equal(b.download_device(out).reshape(q.shape),
+                              ref.attention(q, k, v, exponentials(), 13, True))
+
+
 # ---- rows -----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rms", [False, True])

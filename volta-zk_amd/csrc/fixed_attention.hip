@@ -1035,8 +1035,9 @@ int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::
         });
 }
 
-// 1 where its space may not grow: the other kernel needs none.
-int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_t tiles, size_t cols) {
+// *no_space, with nothing launched, where its space may not grow: the other kernel
+// needs none.  What is returned is an error, of whatever sign, or 0.
+int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_t tiles, size_t cols, bool* no_space) {
     std::sort(seqs.begin(), seqs.end(), [](const FxSeq& x, const FxSeq& y) { return x.length > y.length; });
     size_t units = 0;  // of the largest launch: each reuses the space, as they run in order
     for (size_t at = 0; at < seqs.size(); at += FX_SEQS) {
@@ -1076,7 +1077,8 @@ int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_
         f.splits = static_cast<int>(std::max<size_t>(1, std::min(want, most)));
         const size_t z = units * score_bytes, tops = units * f.splits * FEW * 4;
         const size_t sums = units * f.splits * cols * (a.dim <= 64 ? 65 : 129) * 8;
-        if (!try_ws(c, WS_FIXED, z + sums + tops)) return 1;
+        *no_space = !try_ws(c, WS_FIXED, z + sums + tops);
+        if (*no_space) return 0;
         f.z = ws<int>(c, WS_FIXED);
         f.sums = reinterpret_cast<int64_t*>(ws<unsigned char>(c, WS_FIXED) + z);
         f.tops = reinterpret_cast<int*>(ws<unsigned char>(c, WS_FIXED) + z + sums);
@@ -1155,9 +1157,9 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
         cols = std::max<size_t>(cols, std::min<size_t>(rows_of(s), FEW));
     }
     if (!few.empty()) {
-        const int rc = few_rows(c, a, few, tiles, cols);
-        if (rc < 0) return -1;
-        if (rc) {
+        bool no_space = false;
+        if (few_rows(c, a, few, tiles, cols, &no_space)) return -1;
+        if (no_space) {
             many.assign(seqs, seqs + count);
             workgroups = SIZE_MAX;
         }
