@@ -503,6 +503,30 @@ def test_attention_appends_in_pieces(backend):
             assert np.array_equal(got, want), pieces
 
 
+@pytest.mark.parametrize("dim", [40, 64, 128])
+def test_append_writes_only_its_own_places(backend, dim):
+    """Tokens written again leave those after them in their tile as they were."""
+    g = gen(dim)
+    n = 200
+    q, k, v = (normal(g, (n, 2, dim), s) for s in (1000, 1000, 3000))
+    table = exponentials()
+    with Held(backend) as held:
+        cache = backend.fixed_kv_cache(2, 2, dim, 230)
+        held.keep(cache.storage)
+        backend.upload_into(cache.storage, 0, g.integers(0, 256, cache.storage.len, dtype=np.uint8))
+        backend.fixed_kv_append_device(cache, held.put(k), held.put(v), [[1, 0, n, n]])
+        dq, dt, out = held.put(q), held.put(table), held.new(n * 2 * dim, np.int16)
+        for first, count in ((0, 10), (0, 1), (64, 3), (128, 63), (60, 10), (0, 100), (5, 5), (192, 5), (64, 64), (0, 29),
+                             (64, 36)):
+            k[first:first + count] = full(g, (count, 2, dim))
+            v[first:first + count] = full(g, (count, 2, dim))
+            backend.fixed_kv_append_device(cache, held.put(k[first:first + count]), held.put(v[first:first + count]),
+                                           [[1, 0, count, first + count]])
+            backend.fixed_attention_device(dq, cache, [[1, 0, n, n]], 2, dt, 16, out=out)
+            assert np.array_equal(backend.download_device(out).reshape(q.shape), ref.attention(q, k, v, table, 16, True)), (
+                first, count)
+
+
 @pytest.mark.parametrize("new", [1, 3])
 @pytest.mark.parametrize("value,e", [(-32768, 16384), (32767, 16384), (-32768, 129), (255, 128)])
 def test_attention_longest_sums_of_equal_values(backend, new, value, e):

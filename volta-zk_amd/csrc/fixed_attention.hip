@@ -85,7 +85,8 @@ __device__ inline bool large8(v4i v) {
 // ---- append ---------------------------------------------------------------------------
 // One workgroup per (key head, 64-token tile that new tokens touch).  A token
 // after others of its tile is written byte by byte, as its tile's pieces hold other
-// tokens' bytes; a tile from its first token on in pieces of 16.  Bound by memory,
+// tokens' bytes; a tile from its first token on in pieces of 16, where no token past the
+// last shares them: what the cache holds of those stays.  Bound by memory,
 // one token by its latency: 16 prompts of 10,575 tokens, 12 heads of 64 (67 MB)
 // 13.7 us, 4.9 TB/s, what a copy reaches; one token of 12 heads 2.2 us.
 struct AppendArgs {
@@ -115,8 +116,7 @@ __global__ __launch_bounds__(256) void fx_append_kernel(AppendArgs a, Seqs q) {
     const int16_t* k0 = a.k + static_cast<size_t>(head) * a.dim;
     const int16_t* v0 = a.v + static_cast<size_t>(head) * a.dim;
     if (from == 0) {
-        // A tile from its first token on: whole pieces of 16 bytes; what they
-        // hold of tokens past the last is never used.
+        // A tile from its first token on.
         if (threadIdx.x < 64) sums[threadIdx.x] = large[threadIdx.x] = 0;
         __syncthreads();
         const int j = threadIdx.x & 63;
@@ -134,13 +134,14 @@ __global__ __launch_bounds__(256) void fx_append_kernel(AppendArgs a, Seqs q) {
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
             const int piece = c * 4 + wave;  // places 16 piece ..
+            if (j >= to) continue;
             v4i h, l;
             split16(lo[c], hi[c], large[j], &h, &l);
             v4i* p = reinterpret_cast<v4i*>(rec) + ((j >> 5) * 2 * DC + (piece >> 1)) * 128 + (j & 31) + 32 * (piece & 1);
             p[0] = h;
             p[64] = l;
         }
-        if (threadIdx.x < 64) extra[j] = sums[j] * 256 + large[j];
+        if (threadIdx.x < 64 && j < to) extra[j] = sums[j] * 256 + large[j];
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
             // piece (32-token block, half of it, place)
@@ -157,8 +158,18 @@ __global__ __launch_bounds__(256) void fx_append_kernel(AppendArgs a, Seqs q) {
                 l.b[e] = static_cast<uint8_t>(x ^ 0x80);
             }
             v4i* p = reinterpret_cast<v4i*>(values) + (block * 2 * DC + (d >> 5)) * 128 + (d & 31) + 32 * half;
-            p[0] = h.v;
-            p[64] = l.v;
+            if (block * 32 + 4 * half + 27 < to) {
+                p[0] = h.v;
+                p[64] = l.v;
+            } else {
+                uint8_t* bytes = reinterpret_cast<uint8_t*>(p);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if (block * 32 + 8 * (e >> 2) + 4 * half + (e & 3) >= to) continue;
+                    bytes[e] = h.b[e];
+                    bytes[1024 + e] = l.b[e];
+                }
+            }
         }
         return;
     }
