@@ -104,6 +104,64 @@ def test_decoder_refusals(backend):
         backend.free_device(b)
 
 
+def scale_configs():
+    from volta_mi355x import forward
+    sizes = dict(layers=1, heads=4, kv_heads=2, dim=16, hidden=32, vocab=50, positions=24)
+    return [forward.FixedConfig(**sizes), forward.FixedConfig(**sizes, act_bits=12, weight_bits=9, gain_bits=13)]
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_decoder_of_quantised_tensors_is_near_the_real_model(backend, which):
+    """Real tensors quantised at the binary points that the config states, in a model whose block adds its two biases
+    only (proj and down are zero), against the real model in 64-bit floating point.
+
+    The bound, with u and w half a step of activations and of weights: an element of the stream is off by w (wte), 2 u
+    (its rounding, and wpe) and 2 (w + u) (each bias and its rounding), D in all.  Centred, by at most 2 D; the deviation
+    by D and the roundings of eps and of the root.  The normalised value's quotient, gain and bias add theirs, and the
+    product with wte its own w.  Values stay inside 16 bits (asserted), so nothing is clamped."""
+    from volta_mi355x import forward
+    c = scale_configs()[which]
+    g = np.random.Generator(np.random.PCG64(which))
+    real = {}
+    for name, shape in c.shapes().items():
+        spread = 0.0 if name in ("h0.proj", "h0.down") else 0.4 if name.endswith("bias") else 0.6
+        real[name] = (1.0 + 0.2 * g.uniform(-1, 1, shape)) if name.endswith("gain") else spread * g.uniform(-1, 1, shape)
+    tokens = g.integers(0, c.vocab, c.positions)
+
+    def logits(t):
+        h = t["wte"][tokens] + t["wpe"] + t["h0.proj.bias"] + t["h0.down.bias"]
+        centred = h - h.mean(1, keepdims=True)
+        spread = np.sqrt((centred ** 2).mean(1, keepdims=True) + c.eps)
+        y = centred / spread * t["norm.gain"] + t["norm.bias"]
+        return y @ t["wte"].T, centred / spread, spread, y
+
+    want, hat, spread, y = logits(real)
+    u, w, n = 2.0 ** -(c.act_bits + 1), 2.0 ** -(c.weight_bits + 1), c.width
+    d = (w + 2 * u) + 2 * (w + u)
+    off = d + 1 / (n << c.act_bits) + 0.25 / (n ** 2 * 4 ** c.act_bits * spread)
+    d_hat = (2 * d + np.abs(hat) * off) / (spread - off)
+    d_y = d_hat * real["norm.gain"] + (np.abs(hat) + d_hat) * 2.0 ** -(c.gain_bits + 1) + 2 * u
+    bound = d_y @ (np.abs(real["wte"]) + w).T + np.abs(y).sum(1, keepdims=True) * w
+    assert np.abs(y).max() + d_y.max() < 2.0 ** (15 - c.act_bits)
+
+    dev = {}
+    for name, t in real.items():
+        q = np.rint(t * 2.0 ** c.bits(name))
+        assert np.abs(q).max() < 32768
+        dev[name] = backend.upload_device(q.astype(np.int16).reshape(-1))
+    model = forward.FixedDecoder(backend, c, dev)
+    try:
+        got = np.concatenate([model.step([[int(t)]], [0]) for t in tokens]) / 2.0 ** (c.act_bits + c.weight_bits)
+    finally:
+        model.close()
+        for b in dev.values():
+            backend.free_device(b)
+    assert (np.abs(got - want) <= bound).all()
+    # the bound tells a tensor at twice its scale
+    for name in ("wte", "wpe", "h0.proj.bias", "h0.down.bias", "norm.gain", "norm.bias"):
+        assert (np.abs(logits({**real, name: 2 * real[name]})[0] - want) > 2 * bound).any(), name
+
+
 def test_the_same_tensors_run_and_are_committed(backend, oracle):
     """One layer's matrices: placed and committed from the resident buffers that the decoder runs."""
     from volta_mi355x import forward, ligero, workloads

@@ -25,8 +25,9 @@ from .accel import Backend, DeviceBuffer, InvalidInput
 
 @dataclass(frozen=True)
 class FixedConfig:
-    """Sizes, and the binary points that the shifts keep: activations at 2^-act_bits, weights at 2^-weight_bits,
-    norm gains at 2^-gain_bits.  Biases are stored as weights are."""
+    """Sizes, and the binary points that the shifts keep.  Activations are at 2^-act_bits, and so is what is added to
+    them: norm biases and wpe.  Weights, wte among them, and the biases of products are at 2^-weight_bits, norm gains at
+    2^-gain_bits; `bits` gives each tensor's."""
     layers: int
     heads: int
     kv_heads: int
@@ -38,6 +39,13 @@ class FixedConfig:
     weight_bits: int = 13
     gain_bits: int = 12
     eps: float = 1e-5
+
+    def __post_init__(self):
+        # 15: past it the exponential table no longer reaches down to 0; the others are the operators' shifts
+        if not 0 <= self.act_bits <= 15 or not 0 <= self.weight_bits <= 46:
+            raise InvalidInput("act_bits goes from 0 to 15, weight_bits from 0 to 46")
+        if not 0 <= self.gain_bits - self.act_bits <= 15:
+            raise InvalidInput("gain_bits is act_bits to act_bits + 15")
 
     @property
     def width(self) -> int:
@@ -57,6 +65,15 @@ class FixedConfig:
         return max(1, round(self.eps * self.width ** 2 * 4 ** self.act_bits))
 
     @property
+    def embed_scale(self) -> int:
+        """With embed_shift, takes wte's rows from 2^-weight_bits to 2^-act_bits."""
+        return 1 << max(0, self.act_bits - self.weight_bits)
+
+    @property
+    def embed_shift(self) -> int:
+        return max(0, self.weight_bits - self.act_bits)
+
+    @property
     def score_shift(self) -> int:
         """Leaves scores in steps of about 1/640 after the division by sqrt(dim)."""
         return min(24, max(8, round(2 * self.act_bits + np.log2(np.sqrt(self.dim) / 640))))
@@ -72,6 +89,15 @@ class FixedConfig:
             for name in ("norm1", "norm2"):
                 out[f"h{i}.{name}.gain"] = out[f"h{i}.{name}.bias"] = (self.width,)
         return out
+
+    def bits(self, name: str) -> int:
+        """The binary point of tensor `name`: a value v is held as round(v 2^bits)."""
+        if name not in self.shapes():
+            raise InvalidInput(f"the model has no tensor {name}")
+        if name.endswith(".gain"):
+            return self.gain_bits
+        norm_bias = name.endswith(".bias") and name.split(".")[-2].startswith("norm")
+        return self.act_bits if norm_bias or name == "wpe" else self.weight_bits
 
 
 def activation_table(act_bits: int) -> np.ndarray:
@@ -175,7 +201,7 @@ class FixedDecoder:
                                                        for a, n in zip(after, counts)]))
         h, n, part = self._h, self._n, self._part
         b.fixed_embed_device(self._tokens, rows, self.tensors["wte"], c.vocab, c.width,
-                             scale=1, shift=max(0, c.weight_bits - c.act_bits), positions=self._places,
+                             scale=c.embed_scale, shift=c.embed_shift, positions=self._places,
                              position_table=self.tensors["wpe"], position_rows=c.positions, out=h)
         for i in range(c.layers):
             self._norm(f"h{i}.norm1", h, rows)
