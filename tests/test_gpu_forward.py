@@ -104,6 +104,26 @@ def test_decoder_refusals(backend):
         backend.free_device(b)
 
 
+@pytest.mark.parametrize("prompt", [np.array([1, (1 << 32) + 5]), np.array([(1 << 64) - 1], np.uint64), [1.5],
+                                    [[1, 2], [3, 4]], [1 << 40], ["7"]])
+def test_decoder_refuses_prompts_that_are_no_row_of_tokens(backend, prompt):
+    """Tokens that an i32 would hold as another one, fractions, and prompts of more than one dimension."""
+    from volta_mi355x import InvalidInput, forward
+    c = configs()[0]
+    dev = {name: backend.upload_device(v.reshape(-1)) for name, v in model_tensors(c, 1).items()}
+    model = forward.FixedDecoder(backend, c, dev, slots=2)
+    try:
+        with pytest.raises(InvalidInput):
+            model.step([prompt, [3]], [0, 1])
+        assert model.lengths == [0, 0]
+        same = [model.step([p], [0]) for p in (np.array([3, 5], np.uint8), [3, 5]) if model.reset(0) is None]
+        assert np.array_equal(*same)
+    finally:
+        model.close()
+        for b in dev.values():
+            backend.free_device(b)
+
+
 def scale_configs():
     from volta_mi355x import forward
     sizes = dict(layers=1, heads=4, kv_heads=2, dim=16, hidden=32, vocab=50, positions=24)

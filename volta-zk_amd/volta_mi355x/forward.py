@@ -179,9 +179,19 @@ class FixedDecoder:
         self.backend.fixed_norm_device(x, rows, c.width, self.tensors[name + ".gain"], c.gain_bits - c.act_bits,
                                        c.norm_eps, bias=self.tensors[name + ".bias"], out=self._n, **kw)
 
+    def _prompt(self, prompt) -> np.ndarray:
+        """A prompt's tokens, checked before they become i32: a larger integer would turn into another token."""
+        t = np.asarray(prompt)
+        if t.ndim != 1 or t.size and t.dtype.kind not in "biu":
+            raise InvalidInput("a prompt is one row of integer tokens")
+        if t.size and (t.min() < 0 or t.max() >= self.config.vocab):
+            raise InvalidInput("token is outside the vocabulary")
+        return t.astype(np.int32)
+
     def step_device(self, prompts, slots) -> DeviceBuffer:
         """Appends each prompt's tokens to its slot; the logits' i64 sums after its last token, a row a prompt."""
         c, b = self.config, self.backend
+        prompts = [self._prompt(p) for p in prompts]
         counts = [len(p) for p in prompts]
         rows = sum(counts)
         if len(slots) != len(counts) or not counts or min(counts) == 0 or rows > self.rows or len(set(slots)) != len(slots):
@@ -193,10 +203,7 @@ class FixedDecoder:
             raise InvalidInput("a sequence is longer than the model's positions")
         first = np.concatenate([[0], np.cumsum(counts)[:-1]])
         seqs = np.stack([slots, first, counts, after], 1).astype(np.int64)
-        tokens = np.concatenate([np.asarray(p, np.int32).reshape(-1) for p in prompts])
-        if tokens.min() < 0 or tokens.max() >= c.vocab:
-            raise InvalidInput("token is outside the vocabulary")
-        b.upload_into(self._tokens, 0, tokens)
+        b.upload_into(self._tokens, 0, np.concatenate(prompts))
         b.upload_into(self._places, 0, np.concatenate([np.arange(a - n, a, dtype=np.int32)
                                                        for a, n in zip(after, counts)]))
         h, n, part = self._h, self._n, self._part
