@@ -764,6 +764,24 @@ def test_refusals(backend):
         assert not b.download_device(out).any()
 
 
+@pytest.mark.parametrize("sequences", [[[0, 0, 1.5, 2]], np.array([[0.0, 0.0, 1.0, 1.0]]), [[0, 0], [1, 1]],
+                                       np.zeros((4, 8), np.int64), [0, 0, 1], [[0, 0, 1, 1], [1, 1]], [["0", "0", "1", "1"]]])
+def test_sequences_are_rows_of_four_integers(backend, sequences):
+    from volta_mi355x import InvalidInput
+    b = backend
+    with Held(b) as held:
+        x, w, exp, out = (held.new(4096, np.int16) for _ in range(4))
+        cache = b.fixed_kv_cache(2, 2, 16, 70)
+        held.keep(cache.storage)
+        with pytest.raises(InvalidInput):
+            b.fixed_kv_append_device(cache, x, w, sequences)
+        with pytest.raises(InvalidInput):
+            b.fixed_attention_device(x, cache, sequences, 2, exp, 12, out=out)
+        for none in ([], np.zeros((0, 4), np.int64)):
+            b.fixed_kv_append_device(cache, x, w, none)
+            b.fixed_attention_device(x, cache, none, 2, exp, 12, out=out)
+
+
 def test_refusals_at_the_c_entry(backend):
     """Arguments that the Python layer would catch first, straight through the ABI."""
     import ctypes

@@ -912,6 +912,12 @@ class Backend:
         checks the values themselves."""
         s = sequences
         if not (type(s) is np.ndarray and s.dtype == _I64 and s.ndim == 2 and s.shape[1] == 4 and s.flags.c_contiguous):
+            try:
+                s = np.asarray(s)
+            except ValueError:  # rows of different lengths
+                raise InvalidInput("sequences are rows of four integers") from None
+            if s.size and (s.dtype.kind not in "iu" or (s.shape[-1] != 4 if s.ndim > 1 else s.size % 4)):
+                raise InvalidInput("sequences are rows of four integers")
             s = np.ascontiguousarray(s, dtype=np.int64).reshape(-1, 4)
         if len(s) <= 4:
             rows = max((first + count for _, first, count, _ in s.tolist() if count > 0), default=0)
