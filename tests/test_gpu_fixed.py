@@ -160,6 +160,31 @@ def test_without_workspaces_in_a_coarse_scope():
         assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("gap", [0, 3])
+def test_linear_workspace_is_bounded(gap):
+    """Rows that are not aligned are aligned some at a time (128 MiB)."""
+    from volta_mi355x import Backend
+    rows, k, n = 40000, 2001, 41
+    g = gen(rows)
+    wide, w = normal(g, (rows, k + gap), 1000), normal(g, (k, n), 2000)
+    bias, table, res = full(g, n), full(g, 65536), full(g, (rows, n))
+    acc = ref._sums(wide[:, :k], w)
+    with Backend(timing_policy=1) as b, Held(b) as held:
+        x, packed = held.put(wide), b.fixed_weights_device(held.put(w), k, n)
+        held.keep(packed.storage)
+        db, dt, dr = held.put(bias), held.put(table), held.put(res)
+        y, sums = held.new(rows * (n + 2), np.int16, 7), held.new(rows * (n + 1), np.int64, 8)
+        before = b.get_stats()["live_device_bytes"]
+        b.fixed_linear_device(x, rows, packed, 14, x_stride=k + gap, bias=db, bias_shift=9, table=dt, residual=dr, out=y,
+                              out_stride=n + 2)
+        b.fixed_linear_device(x, rows, packed, x_stride=k + gap, raw=True, out=sums, out_stride=n + 1)
+        y, sums = b.download_device(y).reshape(rows, -1), b.download_device(sums).reshape(rows, -1)
+        assert 0 < b.get_stats()["live_device_bytes"] - before <= 128 << 20
+    h = table.astype(np.int64)[ref.sat(ref.rs(acc + bias.astype(np.int64) * 512, 14)) + 32768]
+    assert np.array_equal(y[:, :n], ref.sat(h + res)) and (y[:, n:] == 7).all()
+    assert np.array_equal(sums[:, :n], acc) and (sums[:, n:] == 8).all()
+
+
 @pytest.mark.parametrize("use", ["", "bias", "table", "residual", "bias table", "bias residual", "table residual"])
 @pytest.mark.parametrize("rows,k,n", [(5, 100, 40), (200, 100, 150)])
 def test_linear_optional_parts(backend, rows, k, n, use):

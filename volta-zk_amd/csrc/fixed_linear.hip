@@ -412,27 +412,6 @@ bool aligned_rows(const FxLinear& a) {
     return reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0 && a.x_stride < (size_t{1} << 22);
 }
 
-// a with its rows aligned in a workspace, or as it is where that may not grow: copies
-// through registers wait for memory in each step, and rows of other alignment take
-// twice the accesses (us without and with, the aligning included: 1,337 x 961 x 5,203
-// 68 and 43, 16,384 x 767 x 4,096 412 and 232, 1,023 x 767 x 3,072 34 and 22).
-FxLinear with_aligned_rows(Context* c, FxLinear a) {
-    const size_t pieces = (a.k + 7) / 8;
-    if (aligned_rows(a) || !try_ws(c, WS_FIXED, a.rows * pieces * 16)) return a;
-    v4i* to = ws<v4i>(c, WS_FIXED);
-    // a launch holds less than 2^32 threads
-    const size_t most = (size_t{1} << 31) / pieces;
-    for (size_t row = 0; row < a.rows; row += most) {
-        const size_t rows = std::min(most, a.rows - row);
-        hipLaunchKernelGGL(fx_align_rows_kernel, dim3(static_cast<unsigned>((rows * pieces + 255) / 256)), dim3(256), 0,
-                           c->stream, a.x + row * a.x_stride, a.x_stride, rows, a.k, static_cast<uint32_t>(pieces),
-                           to + row * pieces);
-    }
-    a.x = reinterpret_cast<const int16_t*>(to);
-    a.x_stride = pieces * 8;
-    return a;
-}
-
 template <int WM, int WN, int I, int J, int STAGES>
 void launch_tile(Context* c, const FxLinear& a) {
     const bool aligned = aligned_rows(a);
@@ -443,17 +422,6 @@ void launch_tile(Context* c, const FxLinear& a) {
         hipLaunchKernelGGL((fx_linear_tile_kernel<WM, WN, I, J, STAGES, true>), grid, threads, 0, c->stream, a, rt, ct);
     else
         hipLaunchKernelGGL((fx_linear_tile_kernel<WM, WN, I, J, STAGES, false>), grid, threads, 0, c->stream, a, rt, ct);
-}
-
-}  // namespace
-
-int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t stride, bool transposed, void* out) {
-    const size_t blocks = fx_blocks(n);
-    hipLaunchKernelGGL(fx_pack_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, c->stream, w,
-                       static_cast<int>(k), static_cast<int>(n), stride, transposed, static_cast<unsigned char*>(out),
-                       blocks);
-    VMX_HIP(c, hipGetLastError());
-    return 0;
 }
 
 // Which kernel.  us for k x n on the rows given, in a loop (5 us of them the call):
@@ -475,14 +443,9 @@ int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t str
 // small tile a CU wants depth of prefetch, a large one eight waves on it, and past
 // that two workgroups a CU hide each other's waits.  The estimates, in ns from the
 // calls above, are a start and an end plus so much a step, by tiles on each CU.
-int fx_linear(Context* c, const FxLinear& given) {
-    const size_t blocks = fx_blocks(given.n), steps = fx_steps(given.k), row_blocks = (given.rows + 15) / 16;
+int launch_product(Context* c, const FxLinear& a) {
+    const size_t blocks = fx_blocks(a.n), steps = fx_steps(a.k), row_blocks = (a.rows + 15) / 16;
     const size_t cus = c->cu_count;
-    // A launch to align rows costs about 3 us: 100 x 767 x 768 (4,032 steps of 16 x 16)
-    // 9.3 us without and 10.7 with, 20 x 3,001 x 768 (4,512) 11.9 and 9.9, 100 x 767 x
-    // 3,072 (16,128) 18.1 and 12.4.
-    const bool align = row_blocks > 1 && blocks * row_blocks * steps >= 4400;
-    const FxLinear a = align ? with_aligned_rows(c, given) : given;
     const size_t small = ((blocks + 3) / 4) * ((row_blocks + 3) / 4), large = ((blocks + 7) / 8) * ((row_blocks + 7) / 8);
     const size_t turns = (large + cus - 1) / cus;
     const size_t deep = small <= cus ? 5000 + 325 * steps : SIZE_MAX;
@@ -505,6 +468,56 @@ int fx_linear(Context* c, const FxLinear& given) {
         launch_tile<2, 2, 2, 2, 2>(c, a);
     }
     VMX_HIP(c, hipGetLastError());
+    return 0;
+}
+
+// Space for aligned rows.
+constexpr size_t ALIGNED_MAX = size_t{128} << 20;
+
+// Rows from .. from + count of a.
+FxLinear rows_of(FxLinear a, size_t from, size_t count) {
+    a.x += from * a.x_stride;
+    if (a.residual) a.residual += from * a.residual_stride;
+    a.out = static_cast<unsigned char*>(a.out) + from * a.out_stride * (a.raw ? 8 : 2);
+    a.rows = count;
+    return a;
+}
+
+}  // namespace
+
+int fx_pack_weights(Context* c, const int16_t* w, size_t k, size_t n, size_t stride, bool transposed, void* out) {
+    const size_t blocks = fx_blocks(n);
+    hipLaunchKernelGGL(fx_pack_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, c->stream, w,
+                       static_cast<int>(k), static_cast<int>(n), stride, transposed, static_cast<unsigned char*>(out),
+                       blocks);
+    VMX_HIP(c, hipGetLastError());
+    return 0;
+}
+
+// Rows that are not aligned are aligned in a workspace, as many at a time as it may
+// hold, where it may grow: copies through registers wait for memory in each step, and
+// rows of other alignment take twice the accesses (us without and with, the aligning
+// included: 1,337 x 961 x 5,203 68 and 43, 16,384 x 767 x 4,096 412 and 232, 1,023 x
+// 767 x 3,072 34 and 22).  A launch to align rows costs about 3 us: 100 x 767 x 768
+// (4,032 steps of 16 x 16) 9.3 us without and 10.7 with, 20 x 3,001 x 768 (4,512) 11.9
+// and 9.9, 100 x 767 x 3,072 (16,128) 18.1 and 12.4.
+int fx_linear(Context* c, const FxLinear& a) {
+    const size_t pieces = (a.k + 7) / 8, row_bytes = pieces * 16;
+    const size_t row_blocks = (a.rows + 15) / 16;
+    const bool align = row_blocks > 1 && fx_blocks(a.n) * row_blocks * fx_steps(a.k) >= 4400 && !aligned_rows(a);
+    // whole tiles, of 1,024 rows at least (k is below 2^16)
+    const size_t most = ALIGNED_MAX / row_bytes / 128 * 128;
+    if (!align || !try_ws(c, WS_FIXED, workspace_step(std::min(a.rows, most) * row_bytes, ALIGNED_MAX)))
+        return launch_product(c, a);
+    v4i* to = ws<v4i>(c, WS_FIXED);
+    for (size_t row = 0; row < a.rows; row += most) {
+        FxLinear part = rows_of(a, row, std::min(most, a.rows - row));
+        hipLaunchKernelGGL(fx_align_rows_kernel, dim3(static_cast<unsigned>((part.rows * pieces + 255) / 256)), dim3(256), 0,
+                           c->stream, part.x, part.x_stride, part.rows, a.k, static_cast<uint32_t>(pieces), to);
+        part.x = reinterpret_cast<const int16_t*>(to);
+        part.x_stride = pieces * 8;
+        if (launch_product(c, part)) return -1;
+    }
     return 0;
 }
 
