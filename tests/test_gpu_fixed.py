@@ -160,6 +160,50 @@ def test_without_workspaces_in_a_coarse_scope():
         assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
+def test_attention_workspace_grows_in_few_steps():
+    """A sequence that gets longer does not allocate again for every tile of tokens."""
+    from volta_mi355x import Backend
+    n = 6000
+    g = gen(n)
+    k, v, q = (normal(g, (m, 4, 64), s) for m, s in ((n, 1000), (n, 3000), (1, 1000)))
+    with Backend(timing_policy=1) as b, Held(b) as held:
+        cache = b.fixed_kv_cache(1, 4, 64, n)
+        held.keep(cache.storage)
+        b.fixed_kv_append_device(cache, held.put(k), held.put(v), [[0, 0, n, n]])
+        dq, table, out = held.put(q), held.put(exponentials()), held.new(256, np.int16)
+        before = b.get_stats()["allocation_calls"]
+        for length in range(2100, n, 64):
+            b.fixed_attention_device(dq, cache, [[0, 0, 1, length]], 4, table, 13, out=out)
+            want = ref.attention(q, k[:length], v[:length], exponentials(), 13, True)
+            assert np.array_equal(b.download_device(out).reshape(q.shape), want)
+        assert 1 <= b.get_stats()["allocation_calls"] - before <= 3
+
+
+def test_attention_workspace_is_bounded():
+    """Scores of sequences whose space together would pass the bound (512 MiB) are taken some sequences at a time."""
+    from volta_mi355x import Backend
+    slots, kv_heads, heads, dim, n = 20, 8, 128, 16, 65536
+    g = gen(5)
+    k, v, q = (normal(g, (m, h, dim), s) for m, h, s in
+               ((n, kv_heads, 1000), (n, kv_heads, 3000), (slots, heads, 1000)))
+    with Backend(timing_policy=1) as b, Held(b) as held:
+        cache = b.fixed_kv_cache(slots, kv_heads, dim, n)
+        held.keep(cache.storage)
+        dk, dv, dq, table = held.put(k), held.put(v), held.put(q), held.put(exponentials())
+        lengths = [n - 1000 * i for i in range(slots)]
+        b.fixed_kv_append_device(cache, dk, dv, [[i, 0, m, m] for i, m in enumerate(lengths)])
+        out = held.new(q.size, np.int16)
+        before = b.get_stats()["live_device_bytes"]
+        b.fixed_attention_device(dq, cache, [[i, i, 1, m] for i, m in enumerate(lengths)], heads, table, 12, out=out)
+        got = b.download_device(out).reshape(q.shape)
+        assert 0 < b.get_stats()["live_device_bytes"] - before <= 512 << 20
+    for i, m in enumerate(lengths):
+        for kv in (i % 8, (i + 3) % 8):
+            mine = slice(kv * 16, kv * 16 + 16)
+            want = ref.attention(q[i:i + 1, mine], k[:m, kv:kv + 1], v[:m, kv:kv + 1], exponentials(), 12, True)
+            assert np.array_equal(got[i:i + 1, mine], want), (i, kv)
+
+
 @pytest.mark.parametrize("gap", [0, 3])
 def test_linear_workspace_is_bounded(gap):
     """Rows that are not aligned are aligned some at a time (128 MiB)."""

@@ -143,13 +143,13 @@ __device__ inline double floor_div(double a, double b, double inv) {
 
 }  // namespace fx
 
-// Workspace to ask for where `bytes` are needed: sizes double from 1 MiB up to
-// `most`, so that needs that grow a little at a time (a tile of tokens, a row) are
-// met by few allocations.
+// Workspace to ask for where `bytes` are needed: sizes double from 1 MiB up to `most`
+// (a power of two) and are its multiples from there, so that needs that grow a little
+// at a time (a tile of tokens, a row) are met by few allocations.
 inline size_t workspace_step(size_t bytes, size_t most) {
     size_t step = size_t{1} << 20;
     while (step < bytes && step < most) step *= 2;
-    return step < bytes ? bytes : step;
+    return (bytes + step - 1) / step * step;
 }
 
 // ---- matrix product --------------------------------------------------------------

@@ -1025,9 +1025,9 @@ int each_group(Context* c, const FxSeq* seqs, size_t count, Items&& items, Launc
 }
 
 template <int DC>
-int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::vector<FxSeq>& seqs, Pass pass) {
+int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const FxSeq* seqs, size_t count, Pass pass) {
     return each_group(
-        c, seqs.data(), seqs.size(), [&](const FxSeq& s) { return (s.count * a.group + FEW - 1) / FEW; },
+        c, seqs, count, [&](const FxSeq& s) { return (s.count * a.group + FEW - 1) / FEW; },
         [&](const Seqs& q, uint32_t total) {
             const dim3 grid(total * static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(f.splits));
             if (pass == ONE) {
@@ -1046,17 +1046,32 @@ int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const std::
         });
 }
 
+// Space for the scores and sums of the sequences of a launch.  One sequence of up to 16
+// rows may take more, but no more than a quarter of its cache: 4 bytes a row and token,
+// of 260 that a token takes there.
+constexpr size_t SPLIT_MAX = size_t{512} << 20;
+
 // *no_space, with nothing launched, where its space may not grow: the other kernel
 // needs none.  What is returned is an error, of whatever sign, or 0.
 int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_t tiles, size_t cols, bool* no_space) {
     std::sort(seqs.begin(), seqs.end(), [](const FxSeq& x, const FxSeq& y) { return x.length > y.length; });
-    size_t units = 0;  // of the largest launch: each reuses the space, as they run in order
-    for (size_t at = 0; at < seqs.size(); at += FX_SEQS) {
-        size_t rows = 0;
-        for (size_t i = at; i < seqs.size() && i < at + FX_SEQS; ++i)
-            rows += (size_t{seqs[i].count} * a.group + FEW - 1) / FEW;
-        units = std::max(units, rows * a.kv_heads);
-    }
+    auto units_of = [&](const FxSeq& s) { return (size_t{s.count} * a.group + FEW - 1) / FEW * a.kv_heads; };
+    // Ends of the launches, in order of at most `most` units each, or of one sequence:
+    // a launch reuses the space of the one before, as they run in order.
+    std::vector<size_t> ends;
+    size_t units = 0;  // of the largest launch
+    auto divide = [&](size_t most) {
+        ends.clear();
+        units = 0;
+        for (size_t at = 0, end = 0; at < seqs.size(); at = end) {
+            size_t here = 0;
+            do here += units_of(seqs[end++]);
+            while (end < seqs.size() && end - at < FX_SEQS && here + units_of(seqs[end]) <= most);
+            ends.push_back(end);
+            units = std::max(units, here);
+        }
+    };
+    divide(SIZE_MAX);
     FewArgs f{};
     f.cols = static_cast<int>(cols);
     f.max_tiles = static_cast<int>(std::max<size_t>(tiles, 1));
@@ -1084,17 +1099,24 @@ int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_
              static_cast<int64_t>(tiles) * (alone - shared * static_cast<int64_t>(units)) <= 10000)
         pass = FUSED;
     if (pass == SCORES) {
+        // splits of all units: 2 x CUs and one a unit at most
+        const size_t split_bytes = cols * (a.dim <= 64 ? 65 : 129) * 8 + FEW * 4;
+        divide((SPLIT_MAX - 2 * c->cu_count * split_bytes) / (score_bytes + split_bytes));
         const size_t want = (2 * c->cu_count + units - 1) / units, most = (tiles + 7) / 8;
         f.splits = static_cast<int>(std::max<size_t>(1, std::min(want, most)));
-        const size_t z = units * score_bytes, tops = units * f.splits * FEW * 4;
-        const size_t sums = units * f.splits * cols * (a.dim <= 64 ? 65 : 129) * 8;
-        *no_space = !try_ws(c, WS_FIXED, z + sums + tops);
+        const size_t z = units * score_bytes, sums = units * f.splits * (split_bytes - FEW * 4);
+        *no_space = !try_ws(c, WS_FIXED, workspace_step(z + units * f.splits * split_bytes, SPLIT_MAX));
         if (*no_space) return 0;
         f.z = ws<int>(c, WS_FIXED);
         f.sums = reinterpret_cast<int64_t*>(ws<unsigned char>(c, WS_FIXED) + z);
         f.tops = reinterpret_cast<int*>(ws<unsigned char>(c, WS_FIXED) + z + sums);
     }
-    return a.dim <= 64 ? launch_few<1>(c, a, f, seqs, pass) : launch_few<2>(c, a, f, seqs, pass);
+    for (size_t at = 0, i = 0; i < ends.size(); at = ends[i++]) {
+        const FxSeq* first = seqs.data() + at;
+        if (a.dim <= 64 ? launch_few<1>(c, a, f, first, ends[i] - at, pass) : launch_few<2>(c, a, f, first, ends[i] - at, pass))
+            return -1;
+    }
+    return 0;
 }
 
 }  // namespace
