@@ -463,7 +463,8 @@ typedef struct VoltaFixedSequence {
 } VoltaFixedSequence;
 size_t volta_mi355x_fixed_cache_bytes(size_t slots, size_t kv_heads, size_t dim, size_t capacity);
 /* Writes k and v rows (kv_heads x dim each, rows k_stride and v_stride apart)
- * to places length - count .. length of their slots.  A slot may occur once. */
+ * to places length - count .. length of their slots and to no others.  A slot
+ * may occur once. */
 int volta_mi355x_fixed_kv_append_device(void* ctx, const VoltaFixedCache* cache, uint64_t k_id, size_t k_off,
                                         size_t k_stride, uint64_t v_id, size_t v_off, size_t v_stride,
                                         const VoltaFixedSequence* sequences, size_t count);

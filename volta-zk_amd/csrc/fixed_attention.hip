@@ -393,10 +393,13 @@ struct Table {
 // workgroup run one phase apart, so that a SIMD's two waves are never both at
 // the vector work.
 //
-// Bound by instruction issue: a score takes about 20 vector instructions, of both
-// passes, which overlap with matrix instructions only in part (a loop of 1,086
-// cycles of matrix work and one of 1,821 of vector work, on a SIMD's two waves,
-// ran 2,330).  16 prompts of 10,575 tokens, 12 heads of 64: 74 us, 0.97 POP/s with
+// Bound by issue and waits together: a score takes about 20 vector instructions, of
+// both passes (0.34 of the issue), which overlap with matrix instructions (0.22) only
+// in part (a loop of 1,086 cycles of matrix work and one of 1,821 of vector work, on a
+// SIMD's two waves, ran 2,330), and waves wait 0.35 of their time, at a barrier for
+// each tile and for LDS.  Keys or queries over 32,639 in every tile, whose scores take
+// the extras: 16 prompts of 9,450 tokens 69 us where 59 without, 8,192 tokens of 16
+// heads of 128 926 and 786.  16 prompts of 10,575 tokens, 12 heads of 64: 74 us, 0.97 POP/s with
 // scores counted twice, as they are computed; 8,192 tokens, 16 heads of 128 on 4:
 // 800 us, 2.1 POP/s.
 template <int DC, int TEAMS>
@@ -1089,7 +1092,11 @@ int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_
     //   192 x 128                      112 (184)    133 (246)
     // ONE, with heads over 64, is 0.3 to 2 us ahead of FUSED up to its 8 tiles.
     // Two launches more cost 10 us; what they save is a tile's time alone on a CU,
-    // 0.55 us (0.75), less its share of the whole card's, 5 ns (9) a unit.
+    // 0.55 us (0.75), less its share of the whole card's, 5 ns (9) a unit.  Scores of
+    // up to 64 KiB are kept.  That limit is low for many units of heads over 64: one
+    // token each of 64 sequences of 4,097, 32 heads of 128 on 8, takes 278 us split and
+    // 218 kept in 65 KiB (4,096 tokens: 143), of 8,192 563 and 458; of 16 sequences of
+    // 8,192, 163 and 162; with heads of 64, 406 both.
     const bool wide = a.dim > 64;
     const int64_t alone = wide ? 750 : 550, shared = wide ? 9 : 5;
     Pass pass = SCORES;

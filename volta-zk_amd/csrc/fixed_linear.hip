@@ -13,8 +13,9 @@ using namespace fx;
 // ---- packing -------------------------------------------------------------------------
 // One workgroup per 16 columns: once for their largest value, then its waves
 // take the steps of 64 rows in turn.  Done once for a model's weights; bound by
-// latency where columns are few: 3,072 x 768 (4.7 MB) 27 us on 48 workgroups,
-// 768 x 50,257 (77 MB) 110 us, 1.4 TB/s read plus written.
+// latency where columns are few: 3,072 x 768 (4.7 MB) 27 us on 48 workgroups (17 in
+// a loop, from the caches), 768 x 50,257 (77 MB) 110 us, 1.4 TB/s read plus written.
+// Transposed weights are read two bytes a lane, rows apart: 45 us in a loop and 144.
 __global__ __launch_bounds__(1024) void fx_pack_weights_kernel(const int16_t* w, int k, int n, size_t stride,
                                                                bool transposed, unsigned char* out, size_t blocks) {
     __shared__ int most;
@@ -150,9 +151,14 @@ __global__ __launch_bounds__(256) void fx_align_rows_kernel(const int16_t* x, si
 // fragments into planes as it reads them.  Fragments lie in LDS in the order the
 // lanes read them.
 //
-// Large products are bound by the matrix cores, whose clock falls with the data:
-// 16,384 x 768 x 4,096 takes 202 to 220 us, 1.9 to 2.0 POP/s of i8 work (a library i8
-// product of 16,384^3 reaches 2.33), and took 186 of then 235 us on weights of zero.
+// Large products: 16,384 x 768 x 4,096 takes 202 to 220 us, 1.9 to 2.0 POP/s of i8
+// work (a library i8 product of 16,384^3 reaches 2.33).  Matrix cores are busy 0.46 of
+// its cycles; a tile a CU takes 13 us, of which 4.7 are its start and end (the estimate
+// in launch_product; the other workgroup of the CU hides part of both), and within the
+// steps waves wait for one another and for copies.  The clock falls with the data: 2.06 GHz here, and on weights of zero
+// 186 of then 235 us.  Weights over 32,639, whose row sums of x are taken in every step:
+// one in a tile 210 and one in each block 224 us where 203 without, seven rows of 768 x
+// 50,257 14.0 with and without.
 // At one tile a CU the steps' waits bound it: 1,023 x 768 x 3,072 17.7 us, 20.8 with a
 // table, whose lookups are bound by their rate (four times as many under way together
 // took as long); matrix cores busy 0.14.
@@ -346,8 +352,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fx_linear_tile_kernel(FxLinea
         return;
     }
     if (a.shift <= 45 && a.bias_shift <= 29) {
-        // Constants below 2^45: with off = 2^16 A + B the sum is 2^16 high + low,
-        // 0 <= low < 2^16 and high in 32 bits, and its shift needs no 64-bit
+        // Constants below 2^45 + 2^39 (bias, half of the shift's step, 128 sum W): with
+        // off = 2^16 A + B the sum is 2^16 high + low, 0 <= low < 2^16 and high, below
+        // 2^30 + 2^29 + 2^25 in size, in 32 bits, and its shift needs no 64-bit
         // arithmetic (under a shift below 16, high is clamped first: past 15 bits
         // the result is clamped whatever they are).
         auto put = [&](int row, int col, int v) {

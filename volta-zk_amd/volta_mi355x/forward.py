@@ -2,8 +2,10 @@
 
 The tensors that `ligero.commit_resident_from_device` commits are the ones that
 run here: the same resident buffers, in fixed point, with exact sums and defined
-roundings, so the trace of an inference is the same however its tokens are
-batched (a whole prompt at once or token by token) and on whatever GPU.
+roundings, so an inference gives the same values however its tokens are batched
+(a whole prompt at once or token by token) and on whatever GPU.  Logits are what
+it returns; a layer's values are overwritten by the next.  The roundings and
+tables are this library's own: no reference output fixes them (parity unpinned).
 
     model = FixedDecoder(backend, config, tensors, slots=4)
     logits = model.step([prompt_a, prompt_b], [0, 1])     # i64 sums, a row a sequence
