@@ -491,6 +491,20 @@ typedef struct VoltaFixedAttention {
 int volta_mi355x_fixed_attention_device(void* ctx, const VoltaFixedCache* cache, const VoltaFixedAttention* args,
                                         const VoltaFixedSequence* sequences, size_t count);
 
+/* The same where a row at place p sees the keys j <= p with j > p - window or
+ * j < sinks: the last `window` (at least 1) with its own, and the first `sinks`.
+ * Only with `causal`. */
+int volta_mi355x_fixed_window_attention_device(void* ctx, const VoltaFixedCache* cache, const VoltaFixedAttention* args,
+                                               size_t window, size_t sinks, const VoltaFixedSequence* sequences,
+                                               size_t count);
+/* The same where every row sees the first prefix_length tokens of prefix_slot
+ * before what it sees of its own sequence (whose lengths and places count
+ * without them).  No sequence may be in prefix_slot, and prefix and sequence
+ * hold at most 65,536 tokens together.  A prefix_length of 0 is no prefix. */
+int volta_mi355x_fixed_prefix_attention_device(void* ctx, const VoltaFixedCache* cache, const VoltaFixedAttention* args,
+                                               uint64_t prefix_slot, uint64_t prefix_length,
+                                               const VoltaFixedSequence* sequences, size_t count);
+
 /* h = sat(x + residual); n = cols, S = sum h (0 for rms), V = n sum h^2 - S^2,
  * R = floor(sqrt(V + eps)):
  *   out = sat((n h - S) gain / (R 2^shift), rounded to nearest, halves up, + bias),
@@ -535,6 +549,78 @@ typedef struct VoltaFixedEmbed {
     uint32_t shift;
 } VoltaFixedEmbed;
 int volta_mi355x_fixed_embed_device(void* ctx, const VoltaFixedEmbed* args);
+
+/* Heads of queries and keys (heads + kv_heads heads of n = dim <= 128 places a
+ * row), normed and rotated:
+ *   with q_gain (the first `heads`) or k_gain (the others): V = n sum h^2 + eps,
+ *     R = floor(sqrt(V)), h = sat(n h gain / (R 2^gain_shift), rounded to nearest,
+ *     halves up);
+ *   for i < rotated / 2 with (c, s) = angles[positions[row]][i], places a, b =
+ *     (i, i + rotated / 2), or (2 i, 2 i + 1) if `adjacent`:
+ *     a' = sat(rs(a c - b s, angle_shift)), b' = sat(rs(a s + b c, angle_shift)).
+ * Places from `rotated` (even) on stay, and so do all of a row whose position is
+ * outside the table.  angles: angle_rows x rotated / 2 pairs of i16; positions:
+ * i32.  gain_shift, angle_shift <= 15, 1 <= eps <= 2^40.  The output may be x
+ * itself (same place and stride); it may not overlap an input otherwise. */
+typedef struct VoltaFixedRotate {
+    uint64_t x_id;
+    size_t x_off, x_stride;
+    uint64_t q_gain_id;
+    size_t q_gain_off;
+    uint64_t k_gain_id;
+    size_t k_gain_off;
+    uint64_t angles_id;
+    size_t angles_off, angle_rows;
+    uint64_t positions_id;
+    size_t positions_off;
+    uint64_t out_id;
+    size_t out_off, out_stride;
+    size_t rows, heads, kv_heads, dim, rotated;
+    uint64_t eps;
+    uint32_t gain_shift, angle_shift;
+    uint32_t adjacent, reserved;
+} VoltaFixedRotate;
+int volta_mi355x_fixed_rotate_device(void* ctx, const VoltaFixedRotate* args);
+
+/* The next token of each of `count` rows of i64 logits.  A token that occurs n > 0
+ * times in its row's history gets l r / 2^16 (l < 0) or l 2^16 / r (l >= 0), to the
+ * nearest integer, halves up, less frequency n + presence (r = repetition; 65,536
+ * changes nothing).  Then every token l + (sum of its biases << bias_shift), exact
+ * and clamped once to [-2^63 + 1, 2^63 - 1]; -2^63 where the row's mask does not
+ * allow it (bit t & 31 of word t >> 5 is 0).
+ *   adjusted (i64), where asked for: these values;
+ *   out (i32): the lowest index of the largest allowed one, -1 if none is.
+ * history and bias_tokens are i32, entries outside the vocabulary are skipped; biases
+ * are i32, a token may have several.  vocab <= 2^24, at most 2^24 entries a row,
+ * bias_shift <= 46.  The adjusted logits may be the logits themselves (same place
+ * and stride); no output may overlap an input otherwise. */
+typedef struct VoltaFixedChoice {
+    uint64_t history_first, history_count;
+    uint64_t bias_first, bias_count;
+    int64_t mask; /* a row of `allowed`; negative: everything is allowed */
+    int64_t frequency, presence;
+    uint32_t repetition, reserved;
+} VoltaFixedChoice;
+typedef struct VoltaFixedChoose {
+    uint64_t logits_id;
+    size_t logits_off, logits_stride;
+    uint64_t history_id;
+    size_t history_off;
+    uint64_t bias_tokens_id;
+    size_t bias_tokens_off;
+    uint64_t bias_values_id;
+    size_t bias_values_off;
+    uint64_t allowed_id;
+    size_t allowed_off, allowed_stride; /* in words of 32 bits */
+    uint64_t adjusted_id;
+    size_t adjusted_off, adjusted_stride;
+    uint64_t out_id;
+    size_t out_off;
+    size_t vocab;
+    uint32_t bias_shift, reserved;
+} VoltaFixedChoose;
+int volta_mi355x_fixed_choose_device(void* ctx, const VoltaFixedChoose* args, const VoltaFixedChoice* choices,
+                                     size_t count);
 
 /* Measurement probes: a 16-byte streaming copy (achievable HBM bandwidth)
  * and the reference's Fp2-multiply stream (rounds == 0) / chain kernels

@@ -213,9 +213,16 @@ VMX_API int volta_mi355x_fixed_kv_append_device(void* raw, const VoltaFixedCache
     });
 }
 
-VMX_API int volta_mi355x_fixed_attention_device(void* raw, const VoltaFixedCache* cache, const VoltaFixedAttention* a,
-                                                const VoltaFixedSequence* sequences, size_t count) {
-    Context* c = static_cast<Context*>(raw);
+namespace {
+
+// What a row sees of the keys: all up to its own, or a window with sinks, or a prefix before its sequence.
+struct Seen {
+    size_t window = 0, sinks = 0;
+    uint64_t prefix_slot = 0, prefix = 0;
+};
+
+int attention(Context* c, const VoltaFixedCache* cache, const VoltaFixedAttention* a, const Seen& seen,
+              const VoltaFixedSequence* sequences, size_t count) {
     if (!c || !a) return fail_msg(c, "invalid fixed-point attention geometry");
     if (a->shift < 8 || a->shift > 24 || !a->entries || a->entries > FX_TABLE_MAX)
         return fail_msg(c, "invalid fixed-point attention shift or table");
@@ -228,6 +235,12 @@ VMX_API int volta_mi355x_fixed_attention_device(void* raw, const VoltaFixedCache
         if (!a->heads || a->heads % kv.kv_heads || a->heads > 65535)
             return fail_msg(c, "attention heads are not a multiple of the cache's");
         if (resolve_sequences(c, kv, sequences, count, false, a->causal != 0, &seqs, &rows)) return -1;
+        if (seen.prefix && (seen.prefix_slot >= kv.slots || seen.prefix > kv.capacity))
+            return fail_msg(c, "prefix is outside the cache");
+        for (const FxSeq& s : seqs) {
+            if (seen.prefix && s.slot == seen.prefix_slot) return fail_msg(c, "a sequence is in the prefix's slot");
+            if (seen.prefix + s.length > FX_CACHE_MAX) return fail_msg(c, "prefix and sequence are longer than 65,536 tokens");
+        }
         if (!rows) return empty_op(c, OP_GEMM);
         const size_t cols = a->heads * kv.dim;
         size_t places = 0;
@@ -248,9 +261,35 @@ VMX_API int volta_mi355x_fixed_attention_device(void* raw, const VoltaFixedCache
                             static_cast<uint32_t>(a->entries),
                             static_cast<uint32_t>(a->heads),
                             a->shift,
-                            a->causal != 0};
+                            a->causal != 0,
+                            seen.window,
+                            seen.sinks,
+                            static_cast<uint32_t>(seen.prefix_slot),
+                            static_cast<uint32_t>(seen.prefix)};
         return counted(c, [&] { return fx_attention(c, kv, t, seqs.data(), seqs.size()); });
     });
+}
+
+}  // namespace
+
+VMX_API int volta_mi355x_fixed_attention_device(void* raw, const VoltaFixedCache* cache, const VoltaFixedAttention* a,
+                                                const VoltaFixedSequence* sequences, size_t count) {
+    return attention(static_cast<Context*>(raw), cache, a, Seen{}, sequences, count);
+}
+
+VMX_API int volta_mi355x_fixed_window_attention_device(void* raw, const VoltaFixedCache* cache,
+                                                       const VoltaFixedAttention* a, size_t window, size_t sinks,
+                                                       const VoltaFixedSequence* sequences, size_t count) {
+    Context* c = static_cast<Context*>(raw);
+    if (!c || !a || !window || !a->causal) return fail_msg(c, "a window of at least one key needs causal attention");
+    return attention(c, cache, a, Seen{window, sinks, 0, 0}, sequences, count);
+}
+
+VMX_API int volta_mi355x_fixed_prefix_attention_device(void* raw, const VoltaFixedCache* cache,
+                                                       const VoltaFixedAttention* a, uint64_t prefix_slot,
+                                                       uint64_t prefix_length, const VoltaFixedSequence* sequences,
+                                                       size_t count) {
+    return attention(static_cast<Context*>(raw), cache, a, Seen{0, 0, prefix_slot, prefix_length}, sequences, count);
 }
 
 VMX_API int volta_mi355x_fixed_norm_device(void* raw, const VoltaFixedNorm* a) {
@@ -328,5 +367,131 @@ VMX_API int volta_mi355x_fixed_embed_device(void* raw, const VoltaFixedEmbed* a)
         e.scale = a->scale;
         e.shift = a->shift;
         return counted(c, [&] { return fx_embed(c, e); });
+    });
+}
+
+VMX_API int volta_mi355x_fixed_rotate_device(void* raw, const VoltaFixedRotate* a) {
+    Context* c = static_cast<Context*>(raw);
+    if (!c || !a || !a->rows || a->rows > MAX_ROWS || !a->dim || a->dim > FX_HEAD_MAX || a->heads > 65535 ||
+        a->kv_heads > 65535 || !(a->heads + a->kv_heads) || a->rotated > a->dim || a->rotated % 2 || a->gain_shift > 15 ||
+        a->angle_shift > 15 || !a->eps || a->eps > uint64_t{1} << 40)
+        return fail_msg(c, "invalid fixed-point rotation geometry");
+    if (!a->rotated != !a->angles_id || !a->rotated != !a->positions_id || (a->rotated && !a->angle_rows))
+        return fail_msg(c, "rotated places, angles and positions come together");
+    return guarded(c, "fixed-point rotation", [&] {
+        void *x = nullptr, *qg = nullptr, *kg = nullptr, *angles = nullptr, *places = nullptr, *out = nullptr;
+        Span xs, qs, ks, as, ps, os;
+        const size_t cols = (a->heads + a->kv_heads) * a->dim;
+        if (matrix(c, a->x_id, a->x_off, a->x_stride, a->rows, cols, 2, &x, &xs, true) ||
+            (a->q_gain_id && matrix(c, a->q_gain_id, a->q_gain_off, a->dim, 1, a->dim, 2, &qg, &qs, true)) ||
+            (a->k_gain_id && matrix(c, a->k_gain_id, a->k_gain_off, a->dim, 1, a->dim, 2, &kg, &ks, true)) ||
+            (a->rotated && (matrix(c, a->angles_id, a->angles_off, a->rotated, a->angle_rows, a->rotated, 2, &angles,
+                                   &as, true) ||
+                            matrix(c, a->positions_id, a->positions_off, a->rows, 1, a->rows, 4, &places, &ps, true))) ||
+            matrix(c, a->out_id, a->out_off, a->out_stride, a->rows, cols, 2, &out, &os, false))
+            return -1;
+        const bool in_place = out == x && a->out_stride == a->x_stride;
+        if ((!in_place && overlap(os, xs)) || overlap(os, qs) || overlap(os, ks) || overlap(os, as) || overlap(os, ps))
+            return fail_msg(c, "fixed-point rotation output overlaps an input");
+        FxRotate r{};
+        r.x = static_cast<const int16_t*>(x);
+        r.x_stride = a->x_stride;
+        r.q_gain = static_cast<const int16_t*>(qg);
+        r.k_gain = static_cast<const int16_t*>(kg);
+        r.angles = static_cast<const int16_t*>(angles);
+        r.angle_rows = a->angle_rows;
+        r.positions = static_cast<const int32_t*>(places);
+        r.out = static_cast<int16_t*>(out);
+        r.out_stride = a->out_stride;
+        r.rows = a->rows;
+        r.heads = static_cast<uint32_t>(a->heads);
+        r.all_heads = static_cast<uint32_t>(a->heads + a->kv_heads);
+        r.dim = static_cast<int>(a->dim);
+        r.pairs = static_cast<int>(a->rotated / 2);
+        r.eps = a->eps;
+        r.gain_shift = a->gain_shift;
+        r.angle_shift = a->angle_shift;
+        r.adjacent = a->adjacent != 0;
+        return counted(c, [&] { return fx_rotate(c, r); });
+    });
+}
+
+VMX_API int volta_mi355x_fixed_choose_device(void* raw, const VoltaFixedChoose* a, const VoltaFixedChoice* choices,
+                                             size_t count) {
+    Context* c = static_cast<Context*>(raw);
+    if (!c || !a || !count || count > MAX_ROWS || !choices || !a->vocab || a->vocab > MAX_COLS || a->bias_shift > 46)
+        return fail_msg(c, "invalid fixed-point choice geometry");
+    return guarded(c, "fixed-point choice", [&] {
+        const size_t words = (a->vocab + 31) / 32;
+        if (a->allowed_id && a->allowed_stride < words) return fail_msg(c, "row stride is shorter than a row");
+        std::vector<FxChoice> rows;
+        rows.reserve(count);
+        // ends of the lists and of the masks that the rows read
+        size_t history = 0, biases = 0, masks = 0;
+        for (size_t i = 0; i < count; ++i) {
+            const VoltaFixedChoice& s = choices[i];
+            size_t end = 0;
+            if (!s.repetition) return fail_msg(c, "repetition is zero");
+            if (s.history_count > MAX_ROWS || s.bias_count > MAX_ROWS)
+                return fail_msg(c, "a row's history or biases are too long");
+            if ((s.history_count && !a->history_id) || (s.bias_count && (!a->bias_tokens_id || !a->bias_values_id)) ||
+                (s.mask >= 0 && !a->allowed_id))
+                return fail_msg(c, "a row reads a list that is missing");
+            FxChoice r{};
+            r.mask = -1;
+            r.frequency = s.frequency;
+            r.presence = s.presence;
+            r.repetition = s.repetition;
+            if (s.history_count) {
+                if (!add_ok(s.history_first, s.history_count, &end)) return fail_msg(c, "a row's history is out of range");
+                history = std::max(history, end);
+                r.history = s.history_first;
+                r.history_count = static_cast<uint32_t>(s.history_count);
+            }
+            if (s.bias_count) {
+                if (!add_ok(s.bias_first, s.bias_count, &end)) return fail_msg(c, "a row's biases are out of range");
+                biases = std::max(biases, end);
+                r.bias = s.bias_first;
+                r.bias_count = static_cast<uint32_t>(s.bias_count);
+            }
+            if (s.mask >= 0) {
+                size_t at = 0;
+                if (!mul_ok(static_cast<size_t>(s.mask), a->allowed_stride, &at) || at > INT64_MAX)
+                    return fail_msg(c, "a row's mask is out of range");
+                masks = std::max(masks, static_cast<size_t>(s.mask) + 1);
+                r.mask = static_cast<int64_t>(at);
+            }
+            rows.push_back(r);
+        }
+        void *logits = nullptr, *past = nullptr, *tokens = nullptr, *values = nullptr, *allowed = nullptr,
+             *adjusted = nullptr, *out = nullptr;
+        Span ls, hs, bs, vs, ms, as, os;
+        if (matrix(c, a->logits_id, a->logits_off, a->logits_stride, count, a->vocab, 8, &logits, &ls, true) ||
+            (history && matrix(c, a->history_id, a->history_off, history, 1, history, 4, &past, &hs, true)) ||
+            (biases && (matrix(c, a->bias_tokens_id, a->bias_tokens_off, biases, 1, biases, 4, &tokens, &bs, true) ||
+                        matrix(c, a->bias_values_id, a->bias_values_off, biases, 1, biases, 4, &values, &vs, true))) ||
+            (masks && matrix(c, a->allowed_id, a->allowed_off, a->allowed_stride, masks, words, 4, &allowed, &ms, true)) ||
+            (a->adjusted_id && matrix(c, a->adjusted_id, a->adjusted_off, a->adjusted_stride, count, a->vocab, 8, &adjusted,
+                                      &as, false)) ||
+            matrix(c, a->out_id, a->out_off, count, 1, count, 4, &out, &os, false))
+            return -1;
+        const bool in_place = adjusted == logits && a->adjusted_stride == a->logits_stride;
+        for (const Span& in : {hs, bs, vs, ms})
+            if (overlap(os, in) || overlap(as, in)) return fail_msg(c, "fixed-point choice output overlaps an input");
+        if (overlap(os, ls) || overlap(os, as) || (!in_place && overlap(as, ls)))
+            return fail_msg(c, "fixed-point choice output overlaps an input");
+        FxChoose f{};
+        f.logits = static_cast<const int64_t*>(logits);
+        f.logits_stride = a->logits_stride;
+        f.history = static_cast<const int32_t*>(past);
+        f.bias_tokens = static_cast<const int32_t*>(tokens);
+        f.bias_values = static_cast<const int32_t*>(values);
+        f.allowed = static_cast<const uint32_t*>(allowed);
+        f.adjusted = static_cast<int64_t*>(adjusted);
+        f.adjusted_stride = a->adjusted_stride;
+        f.tokens = static_cast<int32_t*>(out);
+        f.vocab = static_cast<uint32_t>(a->vocab);
+        f.bias_shift = a->bias_shift;
+        return counted(c, [&] { return fx_choose(c, f, rows.data(), rows.size()); });
     });
 }

@@ -143,6 +143,9 @@ __device__ inline double floor_div(double a, double b, double inv) {
 
 }  // namespace fx
 
+// Workspace of a launch at most, but for a single sequence or row that needs more.
+constexpr size_t FX_SPACE_MAX = size_t{512} << 20;
+
 // Workspace to ask for where `bytes` are needed: sizes double from 1 MiB up to `most`
 // (a power of two) and are its multiples from there, so that needs that grow a little
 // at a time (a tile of tokens, a row) are met by few allocations.
@@ -219,6 +222,8 @@ struct FxAttention {
     const uint16_t* table;
     uint32_t entries, heads, shift;
     bool causal;
+    size_t window, sinks;          // 0: all keys; otherwise the last `window` and the first `sinks`
+    uint32_t prefix_slot, prefix;  // tokens of another slot before each sequence's own
 };
 
 int fx_kv_append(Context* c, const FxCache& cache, const int16_t* k, size_t k_stride, const int16_t* v, size_t v_stride,
@@ -259,7 +264,52 @@ struct FxEmbed {
     uint32_t shift;
 };
 
+struct FxRotate {
+    const int16_t* x;
+    size_t x_stride;
+    const int16_t *q_gain, *k_gain;  // null: not normed
+    const int16_t* angles;           // null: none
+    size_t angle_rows;
+    const int32_t* positions;
+    int16_t* out;
+    size_t out_stride;
+    size_t rows;
+    uint32_t heads, all_heads;  // all_heads: with the key heads
+    int dim, pairs;
+    uint64_t eps;
+    uint32_t gain_shift, angle_shift;
+    bool adjacent;
+};
+
 int fx_norm(Context* c, const FxNorm& a);
 int fx_embed(Context* c, const FxEmbed& a);
+int fx_rotate(Context* c, const FxRotate& a);
+
+// ---- choice of a token ------------------------------------------------------------------
+// What a row's logits go through: places of its lists, and its settings.
+struct FxChoice {
+    uint64_t history, bias;
+    int64_t mask;  // first word; negative: none
+    int64_t frequency, presence;
+    uint32_t history_count, bias_count;
+    uint32_t repetition;  // at 2^-16
+    uint32_t reserved;
+};
+constexpr int FX_CHOICES = 64;  // rows a launch: their settings are a kernel's arguments
+
+struct FxChoose {
+    const int64_t* logits;
+    size_t logits_stride;
+    const int32_t* history;
+    const int32_t *bias_tokens, *bias_values;
+    const uint32_t* allowed;
+    int64_t* adjusted;  // null: not kept
+    size_t adjusted_stride;
+    int32_t* tokens;
+    uint32_t vocab;
+    uint32_t bias_shift;
+};
+
+int fx_choose(Context* c, const FxChoose& a, const FxChoice* rows, size_t count);
 
 }  // namespace vmx

@@ -216,12 +216,88 @@ struct AttentionArgs {
     uint32_t entries;
     uint32_t s1, s2;  // shift = s1 + s2, s1 = min(shift, 16)
     bool causal;
+    int window, sinks;             // WINDOW
+    uint32_t prefix_slot, prefix;  // PREFIX: its tokens
 };
+
+// Which keys a row sees: those up to its limit (ALL); of them only the last
+// `window` and the first `sinks` (WINDOW); those of a prefix in another slot,
+// then its own up to the limit (PREFIX).
+enum Map { ALL, WINDOW, PREFIX };
 
 // Keys that row `row` of a sequence may see.
 __device__ inline int limit_of(const AttentionArgs& a, const FxSeq& s, int row) {
     return static_cast<int>(s.length) - (a.causal ? static_cast<int>(s.count) - row / a.group - 1 : 0);
 }
+
+// The tiles that a block of rows reads, in the order in which it reads them, and
+// which of their tokens are seen.  Tiles that all rows see whole come first where
+// there are many: the loops take those without branches.
+//   ALL     0, 1, ...
+//   WINDOW  those whose first token all rows' windows hold; those that hold the
+//           first of some row's; those of the sinks before them
+//   PREFIX  the prefix's whole tiles, the sequence's own, the rest of the prefix
+template <Map MAP>
+struct Tiles {
+    const unsigned char *own, *shared;  // records of the slots' first tiles
+    int count, first, second;           // in all; in the first part; in the first two
+    int inner, edge;                    // WINDOW: the first tiles of the first two parts
+    int written, prefix;                // tokens of the slots
+
+    // For rows with limits from `low` to `high`.
+    template <int BYTES>
+    __device__ static Tiles of(const AttentionArgs& a, const FxSeq& s, int head, int low, int high) {
+        Tiles m{};
+        auto slot = [&](uint32_t at) {
+            return a.data + (static_cast<size_t>(at) * a.kv_heads + head) * a.tiles * static_cast<size_t>(BYTES);
+        };
+        m.own = slot(s.slot);
+        m.written = static_cast<int>(s.length);
+        m.count = (high + FX_TILE - 1) / FX_TILE;
+        if constexpr (MAP == WINDOW) {
+            m.edge = max(low - a.window, 0) / FX_TILE;
+            m.inner = min((max(high - a.window, 0) + FX_TILE - 1) / FX_TILE, m.count);
+            m.first = m.count - m.inner;
+            m.second = m.count - m.edge;
+            m.count = m.second + min((a.sinks + FX_TILE - 1) / FX_TILE, m.edge);
+        }
+        if constexpr (MAP == PREFIX) {
+            m.shared = slot(a.prefix_slot);
+            m.prefix = static_cast<int>(a.prefix);
+            m.first = m.prefix / FX_TILE;
+            m.second = m.first + m.count;
+            m.count = m.second + (m.prefix % FX_TILE != 0);
+        }
+        return m;
+    }
+    __device__ bool in_prefix(int i) const { return MAP == PREFIX && (i < first || i >= second); }
+    // The i-th tile's place in its slot.
+    __device__ int at(int i) const {
+        if constexpr (MAP == WINDOW) return i < first ? inner + i : i < second ? edge + (i - first) : i - second;
+        if constexpr (MAP == PREFIX) return i < first ? i : i < second ? i - first : first;
+        return i;
+    }
+    template <int BYTES>
+    __device__ const unsigned char* record(int i) const {
+        return (in_prefix(i) ? shared : own) + static_cast<size_t>(at(i)) * BYTES;
+    }
+    __device__ int tokens(int i) const { return in_prefix(i) ? prefix : written; }
+    // Whether a row with `limit` sees `token` of the i-th tile.
+    __device__ bool sees(const AttentionArgs& a, int i, int token, int limit) const {
+        if constexpr (MAP == WINDOW) return token < limit && (token >= limit - a.window || token < a.sinks);
+        return token < (in_prefix(i) ? prefix : limit);
+    }
+    // Whether all rows with limits from low to high see `n` tokens of the i-th tile from `token` on.
+    __device__ bool all_see(const AttentionArgs& a, int i, int token, int n, int low, int high) const {
+        if constexpr (MAP == WINDOW) return token + n <= low && (token >= high - a.window || token + n <= a.sinks);
+        return token + n <= (in_prefix(i) ? prefix : low);
+    }
+    // Whether none of them does; high < 0: there are no rows.
+    __device__ bool none_see(const AttentionArgs& a, int i, int token, int n, int low, int high) const {
+        if constexpr (MAP == WINDOW) return token >= high || (token + n <= low - a.window && token >= a.sinks);
+        return high < 0 || token >= (in_prefix(i) ? prefix : high);
+    }
+};
 
 // A lane's query: its planes (32 places a step) and sum_d (q - o) and o.
 template <int DC>
@@ -402,7 +478,7 @@ struct Table {
 // heads of 128 926 and 786.  16 prompts of 10,575 tokens, 12 heads of 64: 74 us, 0.97 POP/s with
 // scores counted twice, as they are computed; 8,192 tokens, 16 heads of 128 on 4:
 // 800 us, 2.1 POP/s.
-template <int DC, int TEAMS>
+template <int DC, int TEAMS, Map MAP>
 __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(AttentionArgs a, Seqs q) {
     constexpr int WAVES = 4 * DC;             // of a team
     constexpr bool SHARED = DC * TEAMS == 2;  // two waves have the same rows
@@ -434,24 +510,27 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
     const int rows = static_cast<int>(s.count) * a.group;
     const int row0 = static_cast<int>(place) * 128;
     const int row = row0 + group * 32 + (lane & 31);
-    const unsigned char* base = a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles *
-                                             static_cast<size_t>(Record<DC>::BYTES);
     const int limit = limit_of(a, s, min(row, rows - 1));
     // what all rows of the wave see, what any of them does, and any of the workgroup's
     const int all = limit_of(a, s, min(row0 + group * 32, rows - 1));
-    const int some = row0 + group * 32 < rows ? limit_of(a, s, min(row0 + group * 32 + 31, rows - 1)) : 0;
-    const int tiles = (limit_of(a, s, min(row0 + 127, rows - 1)) + FX_TILE - 1) / FX_TILE;
+    const int some = row0 + group * 32 < rows ? limit_of(a, s, min(row0 + group * 32 + 31, rows - 1)) : -1;
+    const Tiles<MAP> map = Tiles<MAP>::template of<Record<DC>::BYTES>(a, s, head, limit_of(a, s, row0),
+                                                                      limit_of(a, s, min(row0 + 127, rows - 1)));
+    const int tiles = map.count;
+    // of tokens token .. token + n of the t-th tile, in the wave's rows
+    auto all_see = [&](int t, int token, int n) { return map.all_see(a, t, token, n, all, some); };
+    auto none_see = [&](int t, int token, int n) { return map.none_see(a, t, token, n, all, some); };
 
     // A wave's share of a tile's keys with its extras (KEYS instructions), or of its values (VALUES).
     constexpr int VALUES_COPIES = 2, KEYS_COPIES = 3;
     auto stage_keys = [&](int t, unsigned char* to, int* extra) {
-        const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES;
+        const unsigned char* rec = map.template record<Record<DC>::BYTES>(t);
         copy_to_lds(rec + wave * 1024, lane * 16, to + wave * 1024);
         copy_to_lds(rec + (WAVES + wave) * 1024, lane * 16, to + (WAVES + wave) * 1024);
         if (lane < 16) copy_to_lds(rec + Record<DC>::EXTRA, lane * 16, extra);  // every wave the same
     };
     auto stage_values = [&](int t, unsigned char* to) {
-        const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES + Record<DC>::VALUES;
+        const unsigned char* rec = map.template record<Record<DC>::BYTES>(t) + Record<DC>::VALUES;
         copy_to_lds(rec + wave * 1024, lane * 16, to + wave * 1024);
         copy_to_lds(rec + (WAVES + wave) * 1024, lane * 16, to + (WAVES + wave) * 1024);
     };
@@ -469,7 +548,7 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
     to_table.store(a.table, static_cast<int>(a.entries), table);
     const uint32_t last = a.entries - 1;
     auto is_plain = [&](int t, const int* extra) {
-        return no_offset && !__any(lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128));
+        return no_offset && !__any(lane + map.at(t) * FX_TILE < map.tokens(t) && (extra[lane] & 128));
     };
 
     int top = INT_MIN;
@@ -486,7 +565,7 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
         const unsigned char* keys = parts[i % RING];
         const int* extra = extras[i % RING];
         const bool plain = is_plain(t, extra);
-        if (DC == 1 && plain && a.s2 == 0 && (t + 1) * FX_TILE <= all) {
+        if (DC == 1 && plain && a.s2 == 0 && all_see(t, map.at(t) * FX_TILE, FX_TILE)) {
             // Most tiles, without a branch: one block's vector work beside the other's products.
             const Raw s0 = products<DC>(keys, mine, 0, lane), s1 = products<DC>(keys, mine, 1, lane);
 #pragma unroll
@@ -497,16 +576,16 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
         }
 #pragma unroll
         for (int b = 0; b < 2 / DC; ++b) {
-            const int block = DC == 2 ? part : b, token = t * FX_TILE + block * 32;
-            if (token >= some) continue;
+            const int block = DC == 2 ? part : b, token = map.at(t) * FX_TILE + block * 32;
+            if (none_see(t, token, 32)) continue;
             const v16i z = scores<DC>(keys, extra, mine, block, lane, a.s1, a.s2, plain);
-            if (token + 32 <= all) {
+            if (all_see(t, token, 32)) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = max(top, z[r]);
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) < limit) top = max(top, z[r]);
+                    if (map.sees(a, t, token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), limit)) top = max(top, z[r]);
             }
         }
     }
@@ -519,15 +598,15 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
 
     v16i hh[2] = {}, mid[2] = {}, ll[2] = {};  // 32 places each, of this wave's 64
     int sum_h = 0, sum_l = 0;
-    // exponentials of 32 tokens with scores z(r), all of which are seen or those below the lane's limit
-    auto exponentials = [&](auto&& z, int token, bool whole, v4i* eh, v4i* el) {
+    // exponentials of 32 tokens of tile t with scores z(r), all of which are seen or those that the lane's row sees
+    auto exponentials = [&](auto&& z, int t, int token, bool whole, v4i* eh, v4i* el) {
         uint32_t e[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z(r)), last)];
         if (!whole) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= limit) e[r] = 0;
+                if (!map.sees(a, t, token + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), limit)) e[r] = 0;
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -538,10 +617,10 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
             sum_l = __builtin_amdgcn_sdot4((*el)[g], 0x01010101, sum_l, false);
         }
     };
-    auto block_exponentials = [&](const unsigned char* keys, const int* extra, int block, int token, bool plain, v4i* eh,
-                                  v4i* el) {
+    auto block_exponentials = [&](const unsigned char* keys, const int* extra, int block, int t, int token, bool plain,
+                                  v4i* eh, v4i* el) {
         const v16i z = scores<DC>(keys, extra, mine, block, lane, a.s1, a.s2, plain);
-        exponentials([&](int r) { return z[r]; }, token, token + 32 <= all, eh, el);
+        exponentials([&](int r) { return z[r]; }, t, token, all_see(t, token, 32), eh, el);
     };
     // the 64 places' values of a block of 32 tokens
     struct Values {
@@ -593,15 +672,18 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
             begin(i);
             const int t = mine_of(i);
             begun = true;
-            if (a.s2 || (t + 1) * FX_TILE > all || !is_plain(t, extras[now])) break;
+            // (a tile past the last, of the longer team's turn, is not seen whole, but for the place that a window's map gives it)
+            if (a.s2 || (TEAMS == 2 && MAP == WINDOW && t >= tiles) || !all_see(t, map.at(t) * FX_TILE, FX_TILE) ||
+                !is_plain(t, extras[now]))
+                break;
             v4i eh, el;
             const Raw s0 = products<DC>(parts[2 * now], mine, 0, lane);
             const Values v0 = read(parts[2 * now + 1], 0);
-            exponentials([&](int r) { return score(s0, r, a.s1); }, 0, true, &eh, &el);
+            exponentials([&](int r) { return score(s0, r, a.s1); }, t, 0, true, &eh, &el);
             const Raw s1 = products<DC>(parts[2 * now], mine, 1, lane);
             add(v0, eh, el);
             const Values v1 = read(parts[2 * now + 1], 1);
-            exponentials([&](int r) { return score(s1, r, a.s1); }, 0, true, &eh, &el);
+            exponentials([&](int r) { return score(s1, r, a.s1); }, t, 0, true, &eh, &el);
             add(v1, eh, el);
             now = now == 2 ? 0 : now + 1;
             begun = false;
@@ -614,10 +696,10 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
             const bool plain = is_plain(t, extras[now]);
 #pragma unroll
             for (int block = 0; block < 2; ++block) {
-                const int token = t * FX_TILE + block * 32;
-                if (token >= some) continue;
+                const int token = map.at(t) * FX_TILE + block * 32;
+                if (none_see(t, token, 32)) continue;
                 v4i eh, el;
-                block_exponentials(parts[2 * now], extras[now], block, token, plain, &eh, &el);
+                block_exponentials(parts[2 * now], extras[now], block, t, token, plain, &eh, &el);
                 add(read(parts[2 * now + 1], block), eh, el);
             }
             now = now == 2 ? 0 : now + 1;
@@ -630,7 +712,7 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
         // they are waited for two phases later.
         constexpr int COPIES = 3;
         auto stage = [&](int t, int odd) {
-            const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES;
+            const unsigned char* rec = map.template record<Record<DC>::BYTES>(t);
             const unsigned char* from = rec + (odd ? Record<DC>::VALUES : 0) + wave * 1024;
             unsigned char* to = parts[2 * odd + (t & 1)] + wave * 1024;
             copy_to_lds(from, lane * 16, to);
@@ -652,10 +734,10 @@ __global__ __launch_bounds__((256 * DC * TEAMS), 2) void fx_attention_kernel(Att
         if (behind) begin(phase++);
         for (int t = 0; t < tiles; ++t) {
             begin(phase++);
-            const int token = t * FX_TILE + part * 32;
+            const int token = map.at(t) * FX_TILE + part * 32;
             v4i eh = {}, el = {};
-            if (token < some)
-                block_exponentials(parts[t & 1], extras[t & 1], part, token, is_plain(t, extras[t & 1]), &eh, &el);
+            if (!none_see(t, token, 32))
+                block_exponentials(parts[t & 1], extras[t & 1], part, t, token, is_plain(t, extras[t & 1]), &eh, &el);
             swap[wave * 128 + lane] = eh;
             swap[wave * 128 + 64 + lane] = el;
             begin(phase++);
@@ -756,7 +838,7 @@ struct FewQuery {
     int sum, o;
 };
 
-template <int DC, Pass PASS>
+template <int DC, Pass PASS, Map MAP>
 __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_kernel(AttentionArgs a, FewArgs f, Seqs q) {
     constexpr int WAVES = FEW_WAVES<DC, PASS>, THREADS = 64 * WAVES;
     extern __shared__ __attribute__((aligned(16))) int kept[];  // FUSED: scores
@@ -775,10 +857,10 @@ __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_k
     const int cols = min(rows - row0, FEW);  // at most f.cols
     const bool mine = (lane & 15) < cols;
     const size_t unit = blockIdx.x;
-    const unsigned char* base =
-        a.data + (static_cast<size_t>(s.slot) * a.kv_heads + head) * a.tiles * static_cast<size_t>(Record<DC>::BYTES);
     const int limit = limit_of(a, s, min(row, rows - 1));
-    const int tiles = (limit_of(a, s, min(row0 + FEW, rows) - 1) + FX_TILE - 1) / FX_TILE;
+    const Tiles<MAP> map = Tiles<MAP>::template of<Record<DC>::BYTES>(a, s, head, limit_of(a, s, row0),
+                                                                      limit_of(a, s, min(row0 + FEW, rows) - 1));
+    const int tiles = map.count;  // at most f.max_tiles
     const int each = (f.max_tiles + f.splits - 1) / f.splits;
     const int from = split * each, to = min(from + each, tiles);
     const uint32_t last = a.entries - 1;
@@ -796,8 +878,8 @@ __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_k
         v4i h[4 * DC], l[4 * DC];
     };
     auto read_values = [&](int t, Values* v) {
-        const v4i* p = reinterpret_cast<const v4i*>(base + static_cast<size_t>(t) * Record<DC>::BYTES + Record<DC>::VALUES) +
-                       in_values;
+        const v4i* p =
+            reinterpret_cast<const v4i*>(map.template record<Record<DC>::BYTES>(t) + Record<DC>::VALUES) + in_values;
 #pragma unroll
         for (int b = 0; b < 4 * DC; ++b) {
             v->h[b] = p[(b >> 1) * 128 + (b & 1) * 16];
@@ -842,10 +924,11 @@ __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_k
         // token 32 (i >> 3) + 4 ((i >> 2) & 1) + (i & 3)
         const int in_tile = (((lane >> 3) & 1) * 2 * DC + (lane >> 5)) * 128 + (lane & 7) + 32 * ((lane >> 4) & 1);
         for (int t = from + wave; t < to; t += WAVES) {
-            const unsigned char* rec = base + static_cast<size_t>(t) * Record<DC>::BYTES;
+            const unsigned char* rec = map.template record<Record<DC>::BYTES>(t);
+            const int token = map.at(t) * FX_TILE;
             const v4i* keys = reinterpret_cast<const v4i*>(rec) + in_tile;
             const int* extra = reinterpret_cast<const int*>(rec + Record<DC>::EXTRA);
-            const bool offset = lane + t * FX_TILE < static_cast<int>(s.length) && (extra[lane] & 128);
+            const bool offset = lane + token < map.tokens(t) && (extra[lane] & 128);
             v4i hh[4] = {}, mid[4] = {}, ll[4] = {};
 #pragma unroll
             for (int c = 0; c < DC; ++c)
@@ -874,7 +957,7 @@ __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_k
                 for (int r = 0; r < 4; ++r) {
                     const int low = static_cast<int>((static_cast<uint32_t>(mid[k][r]) << 8) + ll[k][r]);
                     z[k][r] = ((hh[k][r] << (16 - a.s1)) + (low >> a.s1)) >> a.s2;
-                    if (t * FX_TILE + first + 8 * k + r < limit) top = max(top, z[k][r]);
+                    if (map.sees(a, t, token + first + 8 * k + r, limit)) top = max(top, z[k][r]);
                 }
                 if (PASS != ONE && mine) *reinterpret_cast<v4i*>(z_at(t) + 16 * k) = z[k];
             }
@@ -913,7 +996,8 @@ __global__ __launch_bounds__((64 * FEW_WAVES<DC, PASS>)) void fx_attention_few_k
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const uint32_t d = min(static_cast<uint32_t>(top) - static_cast<uint32_t>(zk[r]), last);
-                        if (t * FX_TILE + first + 8 * k + r < limit) e[r] = PASS == ONE ? table[d] : encoded(a.table[d]);
+                        if (map.sees(a, t, map.at(t) * FX_TILE + first + 8 * k + r, limit))
+                            e[r] = PASS == ONE ? table[d] : encoded(a.table[d]);
                     }
                 }
                 const uint32_t a01 = e[0] | e[1] << 16, a23 = e[2] | e[3] << 16;
@@ -1027,36 +1111,53 @@ int each_group(Context* c, const FxSeq* seqs, size_t count, Items&& items, Launc
     return 0;
 }
 
+template <Map MAP>
+struct MapIs {
+    static constexpr Map map = MAP;
+};
+template <class F>
+void with_map(Map map, F&& f) {
+    if (map == WINDOW)
+        f(MapIs<WINDOW>{});
+    else if (map == PREFIX)
+        f(MapIs<PREFIX>{});
+    else
+        f(MapIs<ALL>{});
+}
+
 template <int DC>
-int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const FxSeq* seqs, size_t count, Pass pass) {
+int launch_few(Context* c, const AttentionArgs& a, const FewArgs& f, const FxSeq* seqs, size_t count, Pass pass, Map map) {
     return each_group(
         c, seqs, count, [&](const FxSeq& s) { return (s.count * a.group + FEW - 1) / FEW; },
         [&](const Seqs& q, uint32_t total) {
             const dim3 grid(total * static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(f.splits));
-            if (pass == ONE) {
-                hipLaunchKernelGGL((fx_attention_few_kernel<DC, ONE>), grid, dim3(64 * FEW_WAVES<DC, ONE>), 0, c->stream,
-                                   a, f, q);
-            } else if (pass == FUSED) {
-                hipLaunchKernelGGL((fx_attention_few_kernel<DC, FUSED>), grid, dim3(64 * FEW_WAVES<DC, FUSED>),
-                                   static_cast<unsigned>(f.max_tiles * f.cols * 256), c->stream, a, f, q);
-            } else {
-                hipLaunchKernelGGL((fx_attention_few_kernel<DC, SCORES>), grid, dim3(64 * FEW_WAVES<DC, SCORES>), 0,
-                                   c->stream, a, f, q);
-                hipLaunchKernelGGL((fx_attention_few_kernel<DC, VALUES>), grid, dim3(64 * FEW_WAVES<DC, VALUES>), 0,
-                                   c->stream, a, f, q);
-                hipLaunchKernelGGL(fx_attention_join_kernel<DC>, dim3(grid.x), dim3(256), 0, c->stream, a, f, q);
-            }
+            with_map(map, [&](auto m) {
+                constexpr Map MAP = decltype(m)::map;
+                if (pass == ONE) {
+                    hipLaunchKernelGGL((fx_attention_few_kernel<DC, ONE, MAP>), grid, dim3(64 * FEW_WAVES<DC, ONE>), 0,
+                                       c->stream, a, f, q);
+                } else if (pass == FUSED) {
+                    hipLaunchKernelGGL((fx_attention_few_kernel<DC, FUSED, MAP>), grid, dim3(64 * FEW_WAVES<DC, FUSED>),
+                                       static_cast<unsigned>(f.max_tiles * f.cols * 256), c->stream, a, f, q);
+                } else {
+                    hipLaunchKernelGGL((fx_attention_few_kernel<DC, SCORES, MAP>), grid, dim3(64 * FEW_WAVES<DC, SCORES>),
+                                       0, c->stream, a, f, q);
+                    hipLaunchKernelGGL((fx_attention_few_kernel<DC, VALUES, MAP>), grid, dim3(64 * FEW_WAVES<DC, VALUES>),
+                                       0, c->stream, a, f, q);
+                    hipLaunchKernelGGL(fx_attention_join_kernel<DC>, dim3(grid.x), dim3(256), 0, c->stream, a, f, q);
+                }
+            });
         });
 }
 
-// Space for the scores and sums of the sequences of a launch.  One sequence of up to 16
-// rows may take more, but no more than a quarter of its cache: 4 bytes a row and token,
-// of 260 that a token takes there.
-constexpr size_t SPLIT_MAX = size_t{512} << 20;
-
+// The scores and sums of the sequences of a launch take FX_SPACE_MAX.  One sequence of
+// up to 16 rows may take more, but no more than a quarter of its cache: 4 bytes a row
+// and token, of 260 that a token takes there.
+//
 // *no_space, with nothing launched, where its space may not grow: the other kernel
 // needs none.  What is returned is an error, of whatever sign, or 0.
-int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_t tiles, size_t cols, bool* no_space) {
+int few_rows(Context* c, const AttentionArgs& a, Map map, std::vector<FxSeq>& seqs, size_t tiles, size_t cols,
+             bool* no_space) {
     std::sort(seqs.begin(), seqs.end(), [](const FxSeq& x, const FxSeq& y) { return x.length > y.length; });
     auto units_of = [&](const FxSeq& s) { return (size_t{s.count} * a.group + FEW - 1) / FEW * a.kv_heads; };
     // Ends of the launches, in order of at most `most` units each, or of one sequence:
@@ -1108,11 +1209,11 @@ int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_
     if (pass == SCORES) {
         // splits of all units: 2 x CUs and one a unit at most
         const size_t split_bytes = cols * (a.dim <= 64 ? 65 : 129) * 8 + FEW * 4;
-        divide((SPLIT_MAX - 2 * c->cu_count * split_bytes) / (score_bytes + split_bytes));
+        divide((FX_SPACE_MAX - 2 * c->cu_count * split_bytes) / (score_bytes + split_bytes));
         const size_t want = (2 * c->cu_count + units - 1) / units, most = (tiles + 7) / 8;
         f.splits = static_cast<int>(std::max<size_t>(1, std::min(want, most)));
         const size_t z = units * score_bytes, sums = units * f.splits * (split_bytes - FEW * 4);
-        *no_space = !try_ws(c, WS_FIXED, workspace_step(z + units * f.splits * split_bytes, SPLIT_MAX));
+        *no_space = !try_ws(c, WS_FIXED, workspace_step(z + units * f.splits * split_bytes, FX_SPACE_MAX));
         if (*no_space) return 0;
         f.z = ws<int>(c, WS_FIXED);
         f.sums = reinterpret_cast<int64_t*>(ws<unsigned char>(c, WS_FIXED) + z);
@@ -1120,7 +1221,8 @@ int few_rows(Context* c, const AttentionArgs& a, std::vector<FxSeq>& seqs, size_
     }
     for (size_t at = 0, i = 0; i < ends.size(); at = ends[i++]) {
         const FxSeq* first = seqs.data() + at;
-        if (a.dim <= 64 ? launch_few<1>(c, a, f, first, ends[i] - at, pass) : launch_few<2>(c, a, f, first, ends[i] - at, pass))
+        if (a.dim <= 64 ? launch_few<1>(c, a, f, first, ends[i] - at, pass, map)
+                        : launch_few<2>(c, a, f, first, ends[i] - at, pass, map))
             return -1;
     }
     return 0;
@@ -1160,7 +1262,23 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
                           t.entries,
                           s1,
                           t.shift - s1,
-                          t.causal};
+                          t.causal,
+                          static_cast<int>(std::min<size_t>(t.window, FX_CACHE_MAX)),
+                          static_cast<int>(std::min<size_t>(t.sinks, FX_CACHE_MAX)),
+                          t.prefix_slot,
+                          t.prefix};
+    size_t all_tokens = 0;
+    for (size_t i = 0; i < count; ++i) all_tokens = std::max<size_t>(all_tokens, seqs[i].length);
+    // a window that holds every sequence hides nothing
+    const bool hides = t.window && static_cast<size_t>(a.window) + a.sinks < all_tokens;
+    const Map map = t.prefix ? PREFIX : hides ? WINDOW : ALL;
+    // Tiles of any 16 rows of a sequence at most: a window's of 16 tokens start anywhere in a tile.
+    auto most_tiles = [&](const FxSeq& s) {
+        const size_t all = (s.length + FX_TILE - 1) / FX_TILE;
+        if (map == PREFIX) return all + (t.prefix + FX_TILE - 1) / FX_TILE;
+        if (map != WINDOW) return all;
+        return std::min<size_t>(all, (a.window + FEW + 2 * FX_TILE - 2) / FX_TILE + (a.sinks + FX_TILE - 1) / FX_TILE);
+    };
     // Where many rows leave CUs idle, the kernel for few rows, which splits the
     // tiles, is faster.  Estimates in ns from measurements (rows x tokens, heads
     // of 128 on 4 key heads): 32 x 8,192 268 us by rows and 40 by tiles, 512 x
@@ -1168,18 +1286,20 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
     // key heads 78 and 96, one prompt of 4,096 190 and more than that.
     auto rows_of = [&](const FxSeq& s) { return size_t{s.count} * group; };
     auto tiles_of = [&](const FxSeq& s) {  // of a middle row
-        return static_cast<double>(s.length - (t.causal ? s.count / 2 : 0)) / FX_TILE + 1;
+        const double all = static_cast<double>(s.length - (t.causal ? s.count / 2 : 0)) / FX_TILE + 1;
+        if (map == WINDOW) return std::min(all, static_cast<double>(most_tiles(s)));
+        return all + static_cast<double>(t.prefix) / FX_TILE;
     };
     double by_rows = 0, by_tiles = 0, longest = 0;
     size_t tiles = 0, units = 0, workgroups = 0;
     for (size_t i = 0; i < count; ++i) {
         const FxSeq& s = seqs[i];
-        tiles = std::max<size_t>(tiles, (s.length + FX_TILE - 1) / FX_TILE);
+        tiles = std::max(tiles, most_tiles(s));
         units += (rows_of(s) + FEW - 1) / FEW * cache.kv_heads;
         if (rows_of(s) <= FEW) continue;
         by_rows += static_cast<double>((rows_of(s) + 127) / 128 * cache.kv_heads) * tiles_of(s) * 11;
         by_tiles += static_cast<double>((rows_of(s) + FEW - 1) / FEW * cache.kv_heads) * tiles_of(s) * 5;
-        longest = std::max(longest, (s.length + FX_TILE - 1) / FX_TILE * (cache.dim <= 64 ? 1500.0 : 2200.0));
+        longest = std::max(longest, static_cast<double>(most_tiles(s)) * (cache.dim <= 64 ? 1500.0 : 2200.0));
     }
     const bool split = by_tiles + 5000 < std::max(by_rows, longest) && units * tiles * FEW * 256 <= size_t{1} << 29;
     std::vector<FxSeq> many, few;
@@ -1193,12 +1313,12 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
             continue;
         }
         few.push_back(s);
-        tiles = std::max<size_t>(tiles, (s.length + FX_TILE - 1) / FX_TILE);
+        tiles = std::max(tiles, most_tiles(s));
         cols = std::max<size_t>(cols, std::min<size_t>(rows_of(s), FEW));
     }
     if (!few.empty()) {
         bool no_space = false;
-        if (few_rows(c, a, few, tiles, cols, &no_space)) return -1;
+        if (few_rows(c, a, map, few, tiles, cols, &no_space)) return -1;
         if (no_space) {
             many.assign(seqs, seqs + count);
             workgroups = SIZE_MAX;
@@ -1211,12 +1331,15 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
             for (uint32_t i = 0; i < q.count; ++i) q.first[i] = items(q.s[i]);
             q.first[q.count] = 0;
             const dim3 grid(total * static_cast<unsigned>(cache.kv_heads));
-            if (cache.dim > 64)
-                hipLaunchKernelGGL((fx_attention_kernel<2, 1>), grid, dim3(512), 0, c->stream, a, q);
-            else if (workgroups <= 2 * static_cast<size_t>(c->cu_count))
-                hipLaunchKernelGGL((fx_attention_kernel<1, 2>), grid, dim3(512), 0, c->stream, a, q);
-            else
-                hipLaunchKernelGGL((fx_attention_kernel<1, 1>), grid, dim3(256), 0, c->stream, a, q);
+            with_map(map, [&](auto m) {
+                constexpr Map MAP = decltype(m)::map;
+                if (cache.dim > 64)
+                    hipLaunchKernelGGL((fx_attention_kernel<2, 1, MAP>), grid, dim3(512), 0, c->stream, a, q);
+                else if (workgroups <= 2 * static_cast<size_t>(c->cu_count))
+                    hipLaunchKernelGGL((fx_attention_kernel<1, 2, MAP>), grid, dim3(512), 0, c->stream, a, q);
+                else
+                    hipLaunchKernelGGL((fx_attention_kernel<1, 1, MAP>), grid, dim3(256), 0, c->stream, a, q);
+            });
         });
 }
 

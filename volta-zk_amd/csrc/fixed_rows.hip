@@ -1,6 +1,7 @@
 // fixed_rows.hip -- row operators of the fixed-point model: the norm with its
-// residual addition, and the embedding of tokens and positions.  Both are bound
-// by memory: eight elements a thread at a time, whatever the rows' alignment.
+// residual addition, the embedding of tokens and positions, and heads normed and
+// rotated.  All are bound by memory: eight elements a thread at a time, whatever
+// the rows' alignment.
 #include <algorithm>
 
 #include "fixed.hpp"
@@ -225,6 +226,134 @@ __global__ __launch_bounds__(256) void fx_embed_kernel(FxEmbed a, uint32_t piece
     store8(a.out + row * a.out_stride, at, a.cols, u.v);
 }
 
+// ---- heads normed and rotated -------------------------------------------------------------
+// For each head of n places: with a gain, V = n sum h^2 + eps, R = floor(sqrt(V)),
+// B = R 2^gain_shift, h = sat(floor((2 n h gain + B) / 2B)): the norm's rounding to 16
+// bits, so that this is the norm of each head followed by the rotation.  Then the
+// places of pair i < pairs, (i, i + pairs) or (2 i, 2 i + 1), are turned by (c, s) =
+// angles[position][i]; those after them stay, and so do all of a row whose position
+// is outside the table.
+//
+// LANES lanes a head, four pairs of places each (what follows the pairs counts as
+// pairs that stay): a head's sum takes log2 LANES steps between neighbours, and both
+// places of a pair are in one lane.
+template <int LANES>
+__device__ inline int group_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);  // lanes 2 3 0 1
+    if constexpr (LANES > 4) v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);  // 7 - lane of 8
+    if constexpr (LANES > 8) v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);  // 15 - lane of 16
+    return v;
+}
+
+template <int LANES>
+__global__ __launch_bounds__(256) void fx_rotate_kernel(FxRotate a, uint32_t items) {
+    const uint32_t item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (item >= items) return;  // whole groups of lanes
+    const uint32_t row = item / a.all_heads, head = item - row * a.all_heads;
+    const int first = static_cast<int>(threadIdx.x % LANES) * 4;  // pair
+    const int16_t* x = a.x + row * a.x_stride + static_cast<size_t>(head) * a.dim;
+    int16_t* out = a.out + row * a.out_stride + static_cast<size_t>(head) * a.dim;
+    // places of pair u: `one` and `two`
+    auto one = [&](int u) { return a.adjacent || u >= a.pairs ? 2 * u : u; };
+    auto two = [&](int u) { return a.adjacent || u >= a.pairs ? 2 * u + 1 : u + a.pairs; };
+    // The lane's places are eight in a row, or four and four; a lane with pairs of both
+    // kinds, or at the head's end, takes them one by one.
+    const bool joint = a.adjacent || first >= a.pairs;
+    const bool whole = joint ? 2 * first + 8 <= a.dim : first + 4 <= a.pairs;
+    auto load = [&](const int16_t* p, int* h) {
+        if (whole) {
+            Eight u;
+            if (joint) {
+                u.v = fx::load8(p + 2 * first);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[i] = u.e[i];
+            } else {
+                const uint2 lo = reinterpret_cast<const Row8*>(p + first)->v;
+                const uint2 hi = reinterpret_cast<const Row8*>(p + first + a.pairs)->v;
+                u.v = v4i{static_cast<int>(lo.x), static_cast<int>(lo.y), static_cast<int>(hi.x), static_cast<int>(hi.y)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[2 * i] = u.e[i], h[2 * i + 1] = u.e[4 + i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[2 * i] = one(first + i) < a.dim ? p[one(first + i)] : 0;
+                h[2 * i + 1] = two(first + i) < a.dim ? p[two(first + i)] : 0;
+            }
+        }
+    };
+    int h[8];
+    load(x, h);
+    const int16_t* gains = head < a.heads ? a.q_gain : a.k_gain;
+    if (gains) {
+        int g[8];
+        load(gains, g);
+        uint64_t q = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q += static_cast<uint32_t>(h[i] * h[i]);
+        // at most 2^33 a lane: in parts of 20 bits
+        const uint32_t low = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q & 0xfffff)));
+        const uint32_t high = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q >> 20)));
+        const uint64_t v = static_cast<uint64_t>(a.dim) * ((static_cast<uint64_t>(high) << 20) + low) + a.eps;
+        // as in fx_norm_kernel; |n h gain| <= 2^37
+        const double below = 2.0 * static_cast<double>(floor_sqrt(v) << a.gain_shift), inv = 1.0 / below;
+        const double half = 0.5 * below, n2 = 2.0 * a.dim;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double top = __builtin_fma(n2, static_cast<double>(h[i] * g[i]), half);
+            const double est = __builtin_floor(__builtin_fma(top, inv, 0x1p-34));
+            const double rest = __builtin_fma(-est, below, top);
+            const double est_in = __builtin_fmin(__builtin_fmax(est, -1048576.0), 1048576.0);
+            const int y = static_cast<int>(est_in) + (__builtin_bit_cast(int64_t, rest) < 0 ? -1 : 0);
+            h[i] = min(max(y, -32768), 32767);
+        }
+    }
+    if (a.pairs && first < a.pairs) {
+        const int64_t place = a.positions[row];
+        if (place >= 0 && static_cast<size_t>(place) < a.angle_rows) {
+            const int16_t* turn = a.angles + (static_cast<size_t>(place) * a.pairs + first) * 2;
+            Eight u;
+            u.v = load8(turn, 0, 2 * (a.pairs - first));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (first + i >= a.pairs) continue;
+                // 2^31 at most: past 32 bits by one
+                const int64_t c = u.e[2 * i], s = u.e[2 * i + 1], p = h[2 * i], q = h[2 * i + 1];
+                h[2 * i] = sat16(rounded(p * c - q * s, a.angle_shift));
+                h[2 * i + 1] = sat16(rounded(p * s + q * c, a.angle_shift));
+            }
+        }
+    }
+    if (whole) {
+        Eight u;
+        if (joint) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u.e[i] = static_cast<int16_t>(h[i]);
+            reinterpret_cast<Row16*>(out + 2 * first)->v = u.v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u.e[i] = static_cast<int16_t>(h[2 * i]), u.e[4 + i] = static_cast<int16_t>(h[2 * i + 1]);
+            reinterpret_cast<Row8*>(out + first)->v = make_uint2(static_cast<uint32_t>(u.v[0]), static_cast<uint32_t>(u.v[1]));
+            reinterpret_cast<Row8*>(out + first + a.pairs)->v =
+                make_uint2(static_cast<uint32_t>(u.v[2]), static_cast<uint32_t>(u.v[3]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (one(first + i) < a.dim) out[one(first + i)] = static_cast<int16_t>(h[2 * i]);
+            if (two(first + i) < a.dim) out[two(first + i)] = static_cast<int16_t>(h[2 * i + 1]);
+        }
+    }
+}
+
+template <int LANES>
+void launch_rotate(Context* c, const FxRotate& a) {
+    const uint32_t items = static_cast<uint32_t>(a.rows) * a.all_heads;
+    hipLaunchKernelGGL(fx_rotate_kernel<LANES>, dim3((items + 256 / LANES - 1) / (256 / LANES)), dim3(256), 0, c->stream,
+                       a, items);
+}
+
 template <int THREADS, int KEPT>
 void launch_norm(Context* c, const FxNorm& a) {
     constexpr size_t rows = 256 / THREADS;
@@ -269,6 +398,26 @@ int fx_embed(Context* c, const FxEmbed& a) {
         part.rows = std::min(most, a.rows - row);
         hipLaunchKernelGGL(fx_embed_kernel, dim3(static_cast<unsigned>((part.rows * pieces + 255) / 256)), dim3(256), 0,
                            c->stream, part, pieces);
+        VMX_HIP(c, hipGetLastError());
+    }
+    return 0;
+}
+
+int fx_rotate(Context* c, const FxRotate& a) {
+    // a launch holds less than 2^32 threads, of 16 a head at most
+    const size_t most = std::max<size_t>(1, (size_t{1} << 27) / a.all_heads);
+    FxRotate part = a;
+    for (size_t row = 0; row < a.rows; row += most) {
+        part.x = a.x + row * a.x_stride;
+        part.out = a.out + row * a.out_stride;
+        part.positions = a.positions ? a.positions + row : nullptr;
+        part.rows = std::min(most, a.rows - row);
+        if (a.dim <= 32)
+            launch_rotate<4>(c, part);
+        else if (a.dim <= 64)
+            launch_rotate<8>(c, part);
+        else
+            launch_rotate<16>(c, part);
         VMX_HIP(c, hipGetLastError());
     }
     return 0;

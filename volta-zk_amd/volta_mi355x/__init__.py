@@ -6,10 +6,10 @@ volta_cuda_* C ABI (v37).  This package is its host-side mirror: `accel`
 `forward` (a decoder over the committed tensors, from the fixed-point model
 operators) and `workloads` (synthetic benchmark inputs).
 """
-from .accel import (ABI_VERSION, FP2, P, AbiMismatch, AccelError, Backend, DeviceBuffer, DeviceMerkleTree, FixedKvCache,
+from .accel import (ABI_VERSION, FIXED_CHOICE, FP2, P, AbiMismatch, AccelError, Backend, DeviceBuffer, DeviceMerkleTree, FixedKvCache,
                     FixedWeights, GpuError, InvalidInput, LibraryLoad, MissingSymbol, abi_symbols, extension_symbols, fp2_as_u64,
                     load_library)
 
-__all__ = ["ABI_VERSION", "FP2", "P", "AbiMismatch", "AccelError", "Backend", "DeviceBuffer", "DeviceMerkleTree", "FixedKvCache",
+__all__ = ["ABI_VERSION", "FIXED_CHOICE", "FP2", "P", "AbiMismatch", "AccelError", "Backend", "DeviceBuffer", "DeviceMerkleTree", "FixedKvCache",
            "FixedWeights", "GpuError", "InvalidInput", "LibraryLoad", "MissingSymbol", "abi_symbols", "extension_symbols", "fp2_as_u64",
            "load_library"]

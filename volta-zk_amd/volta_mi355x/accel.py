@@ -24,6 +24,10 @@ import numpy as np
 ABI_VERSION = 37
 P = 0xFFFF_FFFF_0000_0001
 FP2 = np.dtype([("c0", "<u8"), ("c1", "<u8")])
+# A row's settings for fixed_choose_device (VoltaFixedChoice).
+FIXED_CHOICE = np.dtype([("history_first", "<u8"), ("history_count", "<u8"), ("bias_first", "<u8"), ("bias_count", "<u8"),
+                         ("mask", "<i8"), ("frequency", "<i8"), ("presence", "<i8"), ("repetition", "<u4"),
+                         ("reserved", "<u4")])
 _I16, _I32, _I64 = np.dtype(np.int16), np.dtype(np.int32), np.dtype(np.int64)
 
 _PKG = pathlib.Path(__file__).resolve().parent.parent
@@ -133,6 +137,31 @@ class _FixedEmbed(ctypes.Structure):
                 ("scale", ctypes.c_int32), ("shift", ctypes.c_uint32)]
 
 
+class _FixedRotate(ctypes.Structure):
+    _fields_ = [("x_id", ctypes.c_uint64), ("x_off", ctypes.c_size_t), ("x_stride", ctypes.c_size_t),
+                ("q_gain_id", ctypes.c_uint64), ("q_gain_off", ctypes.c_size_t),
+                ("k_gain_id", ctypes.c_uint64), ("k_gain_off", ctypes.c_size_t),
+                ("angles_id", ctypes.c_uint64), ("angles_off", ctypes.c_size_t), ("angle_rows", ctypes.c_size_t),
+                ("positions_id", ctypes.c_uint64), ("positions_off", ctypes.c_size_t),
+                ("out_id", ctypes.c_uint64), ("out_off", ctypes.c_size_t), ("out_stride", ctypes.c_size_t),
+                ("rows", ctypes.c_size_t), ("heads", ctypes.c_size_t), ("kv_heads", ctypes.c_size_t),
+                ("dim", ctypes.c_size_t), ("rotated", ctypes.c_size_t), ("eps", ctypes.c_uint64),
+                ("gain_shift", ctypes.c_uint32), ("angle_shift", ctypes.c_uint32),
+                ("adjacent", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
+class _FixedChoose(ctypes.Structure):
+    _fields_ = [("logits_id", ctypes.c_uint64), ("logits_off", ctypes.c_size_t), ("logits_stride", ctypes.c_size_t),
+                ("history_id", ctypes.c_uint64), ("history_off", ctypes.c_size_t),
+                ("bias_tokens_id", ctypes.c_uint64), ("bias_tokens_off", ctypes.c_size_t),
+                ("bias_values_id", ctypes.c_uint64), ("bias_values_off", ctypes.c_size_t),
+                ("allowed_id", ctypes.c_uint64), ("allowed_off", ctypes.c_size_t), ("allowed_stride", ctypes.c_size_t),
+                ("adjusted_id", ctypes.c_uint64), ("adjusted_off", ctypes.c_size_t),
+                ("adjusted_stride", ctypes.c_size_t),
+                ("out_id", ctypes.c_uint64), ("out_off", ctypes.c_size_t), ("vocab", ctypes.c_size_t),
+                ("bias_shift", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
 def abi_symbols(header: pathlib.Path = HEADER) -> list[str]:
     """The reference-ABI symbol names declared in include/volta_cuda_abi.h."""
     text = header.read_text()
@@ -213,6 +242,12 @@ _SIGS = {
                                                    _vp, _sz]),
     "volta_mi355x_fixed_attention_device": (_int, [_vp, ctypes.POINTER(_FixedCache), ctypes.POINTER(_FixedAttention),
                                                    _vp, _sz]),
+    "volta_mi355x_fixed_window_attention_device": (_int, [_vp, ctypes.POINTER(_FixedCache),
+                                                          ctypes.POINTER(_FixedAttention), _sz, _sz, _vp, _sz]),
+    "volta_mi355x_fixed_prefix_attention_device": (_int, [_vp, ctypes.POINTER(_FixedCache),
+                                                          ctypes.POINTER(_FixedAttention), _u64, _u64, _vp, _sz]),
+    "volta_mi355x_fixed_rotate_device": (_int, [_vp, ctypes.POINTER(_FixedRotate)]),
+    "volta_mi355x_fixed_choose_device": (_int, [_vp, ctypes.POINTER(_FixedChoose), _vp, _sz]),
     "volta_mi355x_fixed_norm_device": (_int, [_vp, ctypes.POINTER(_FixedNorm)]),
     "volta_mi355x_fixed_embed_device": (_int, [_vp, ctypes.POINTER(_FixedEmbed)]),
     "volta_mi355x_probe_copy_device": (_int, [_vp, _u64, _u64, _sz]),
@@ -942,12 +977,16 @@ class Backend:
                                                                  v_offset, v_stride, s.ctypes.data, len(s)))
 
     def fixed_attention_device(self, q: DeviceBuffer, cache: FixedKvCache, sequences, heads: int, table: DeviceBuffer,
-                               shift: int, *, causal: bool = True, q_offset: int = 0, q_stride: int | None = None,
+                               shift: int, *, causal: bool = True, window: int = 0, sinks: int = 0,
+                               prefix: tuple[int, int] | None = None, q_offset: int = 0, q_stride: int | None = None,
                                table_offset: int = 0, entries: int | None = None, out: DeviceBuffer | None = None,
                                out_offset: int = 0, out_stride: int | None = None) -> DeviceBuffer:
         """Attention of packed rows (heads x dim) over the cache: z = (q . k) >> shift, e =
         table[min(max z - z, entries - 1)], out = sum e v / sum e to the nearest integer.  sequences as for
-        fixed_kv_append_device; causal rows see the tokens up to their own, others all of their sequence."""
+        fixed_kv_append_device; causal rows see the tokens up to their own, others all of their sequence.
+        window (causal only; 0: none): of these the last `window`, the row's own among them, and the first `sinks`.
+        prefix (slot, tokens): every row sees the first tokens of that slot before its sequence's, whose lengths
+        count without them."""
         s, rows = self._sequences(sequences)
         cols = heads * cache.dim
         entries = table.len - table_offset if entries is None else entries
@@ -957,6 +996,12 @@ class Backend:
             raise InvalidInput("invalid fixed-point attention shift or table")
         if rows <= 0 and out is None:
             raise InvalidInput("attention without rows needs an output buffer")
+        if window < 0 or sinks < 0 or (sinks and not window) or (window and (not causal or prefix is not None)):
+            raise InvalidInput("a window, with its sinks, is for causal attention without a prefix")
+        if prefix is not None:
+            slot, tokens = prefix
+            if not 0 <= slot < cache.slots or not 0 <= tokens <= cache.capacity:
+                raise InvalidInput("prefix is outside the cache")
         if table.dtype.itemsize != 2 or table.dtype.kind not in "iu":
             raise InvalidInput("the exponential table must hold 16-bit integers")
         q_stride = cols if q_stride is None else q_stride
@@ -969,6 +1014,12 @@ class Backend:
             result = self._result(out, out_offset, out_stride, rows, cols, _I16)
         a = _FixedAttention(q.id, q_offset, q_stride, tid, table_offset, entries, result.id, out_offset, out_stride,
                             heads, shift, 1 if causal else 0)
+        if window:
+            return self._done(self.lib.volta_mi355x_fixed_window_attention_device(
+                self.raw, cache._args(), a, min(window, 65536), min(sinks, 65536), s.ctypes.data, len(s)), result, out)
+        if prefix is not None:
+            return self._done(self.lib.volta_mi355x_fixed_prefix_attention_device(
+                self.raw, cache._args(), a, slot, tokens, s.ctypes.data, len(s)), result, out)
         return self._done(self.lib.volta_mi355x_fixed_attention_device(self.raw, cache._args(), a, s.ctypes.data, len(s)),
                           result, out)
 
@@ -1030,6 +1081,110 @@ class Backend:
                         position_offset, position_stride, position_rows, result.id, out_offset, out_stride, rows, cols,
                         scale, shift)
         return self._done(self.lib.volta_mi355x_fixed_embed_device(self.raw, a), result, out)
+
+    def fixed_rotate_device(self, x: DeviceBuffer, rows: int, heads: int, dim: int, *, kv_heads: int = 0,
+                            q_gain: DeviceBuffer | None = None, k_gain: DeviceBuffer | None = None, gain_shift: int = 0,
+                            eps: int = 1, angles: DeviceBuffer | None = None, angle_rows: int = 0,
+                            positions: DeviceBuffer | None = None, rotated: int | None = None, adjacent: bool = False,
+                            angle_shift: int = 14, x_offset: int = 0, x_stride: int | None = None,
+                            q_gain_offset: int = 0, k_gain_offset: int = 0, angles_offset: int = 0,
+                            positions_offset: int = 0, out: DeviceBuffer | None = None, out_offset: int = 0,
+                            out_stride: int | None = None) -> DeviceBuffer:
+        """Rows of heads + kv_heads heads of dim, normed with q_gain (the first `heads`) and k_gain (the others), and
+        rotated by the (cos, sin) of their i32 positions in angles (angle_rows x rotated / 2 pairs of i16 at
+        2^-angle_shift; rotated: the first places of a head, all unless given).  Pairs are places (i, i + rotated / 2), or
+        (2 i, 2 i + 1) if adjacent.  With R = floor(sqrt(dim sum h^2 + eps)) the norm is sat(dim h gain /
+        (R 2^gain_shift)) to the nearest integer; a row whose position is outside the table is not rotated.  out may be x."""
+        if rotated is None:
+            rotated = dim if angles is not None else 0
+        all_heads = heads + kv_heads
+        if rows <= 0 or min(heads, kv_heads) < 0 or max(heads, kv_heads) > 65535 or not all_heads or not 0 < dim <= 128:
+            raise InvalidInput("invalid fixed-point rotation geometry")
+        if not 0 <= gain_shift <= 15 or not 0 <= angle_shift <= 15 or not 0 < eps <= 1 << 40:
+            raise InvalidInput("invalid fixed-point rotation geometry")
+        if not 0 <= rotated <= dim or rotated % 2:
+            raise InvalidInput("rotated places are an even number of a head's")
+        if (rotated > 0) != (angles is not None) or (rotated > 0) != (positions is not None) or (rotated and angle_rows <= 0):
+            raise InvalidInput("rotated places, angles and positions come together")
+        cols = all_heads * dim
+        x_stride = cols if x_stride is None else x_stride
+        out_stride = cols if out_stride is None else out_stride
+        xid = self._matrix(x, x_offset, x_stride, rows, cols, _I16, "x")
+        qid = kid = aid = pid = 0
+        if q_gain is not None:
+            qid = self._matrix(q_gain, q_gain_offset, dim, 1, dim, _I16, "query gain")
+        if k_gain is not None:
+            kid = self._matrix(k_gain, k_gain_offset, dim, 1, dim, _I16, "key gain")
+        if rotated:
+            aid = self._matrix(angles, angles_offset, rotated, angle_rows, rotated, _I16, "angles")
+            pid = self._matrix(positions, positions_offset, rows, 1, rows, _I32, "positions")
+        result = self._result(out, out_offset, out_stride, rows, cols, _I16)
+        a = _FixedRotate(xid, x_offset, x_stride, qid, q_gain_offset, kid, k_gain_offset, aid, angles_offset,
+                         angle_rows if rotated else 0, pid, positions_offset, result.id, out_offset, out_stride, rows, heads,
+                         kv_heads, dim, rotated, eps, gain_shift, angle_shift, 1 if adjacent else 0, 0)
+        return self._done(self.lib.volta_mi355x_fixed_rotate_device(self.raw, a), result, out)
+
+    def fixed_choose_device(self, logits: DeviceBuffer, rows: int, vocab: int, choices: np.ndarray | None = None, *,
+                            history: DeviceBuffer | None = None, bias_tokens: DeviceBuffer | None = None,
+                            bias_values: DeviceBuffer | None = None, bias_shift: int = 0,
+                            allowed: DeviceBuffer | None = None, logits_offset: int = 0, logits_stride: int | None = None,
+                            history_offset: int = 0, bias_offset: int = 0, allowed_offset: int = 0,
+                            allowed_stride: int | None = None, adjusted: DeviceBuffer | None = None,
+                            adjusted_offset: int = 0, adjusted_stride: int | None = None, out: DeviceBuffer | None = None,
+                            out_offset: int = 0) -> DeviceBuffer:
+        """The next token (i32) of each row of i64 logits; `adjusted` keeps the logits that it was chosen by.
+
+        choices, a row each (FIXED_CHOICE; none: the largest logits as they are): a token that occurs n > 0 times in the
+        row's history, history_count i32 from history_first on, gets l r / 2^16 (l < 0) or l 2^16 / r (l >= 0), r =
+        repetition, to the nearest integer, less frequency n + presence.  The row's biases (i32 << bias_shift; bias_tokens
+        and bias_values from bias_first on) are added, and a token whose bit in row `mask` of `allowed` (32 tokens a
+        word; mask < 0: none) is 0 gets -2^63.  The choice is the lowest index of the largest, -1 if nothing is allowed."""
+        if rows <= 0 or not 0 < vocab <= 1 << 24 or not 0 <= bias_shift <= 46:
+            raise InvalidInput("invalid fixed-point choice geometry")
+        if choices is None:
+            choices = np.zeros(rows, FIXED_CHOICE)
+            choices["mask"], choices["repetition"] = -1, 65536
+        if getattr(choices, "dtype", None) != FIXED_CHOICE or choices.shape != (rows,):
+            raise InvalidInput("choices are a FIXED_CHOICE array with an entry a row")
+        if (bias_tokens is None) != (bias_values is None):
+            raise InvalidInput("biases have tokens and values")
+        choices = np.ascontiguousarray(choices)
+        if not choices["repetition"].all():
+            raise InvalidInput("repetition is zero")
+        words = (vocab + 31) // 32
+        logits_stride = vocab if logits_stride is None else logits_stride
+        allowed_stride = words if allowed_stride is None else allowed_stride
+        adjusted_stride = vocab if adjusted_stride is None else adjusted_stride
+        lid = self._matrix(logits, logits_offset, logits_stride, rows, vocab, _I64, "logits")
+        mid = aid = 0
+        lists = [("history", history, history_offset), ("bias", bias_tokens, bias_offset), ("bias", bias_values, bias_offset)]
+        ids = []
+        for name, buf, offset in lists:
+            count = choices[name + "_count"]
+            if buf is None:
+                if count.any():
+                    raise InvalidInput(f"a row reads a {name} that is missing")
+                ids.append(0)
+                continue
+            if (count > 1 << 24).any() or (choices[name + "_first"] >= 1 << 62).any():
+                raise InvalidInput(f"a row's {name} is out of range")
+            end = int((choices[name + "_first"] + count)[count > 0].max(initial=0))
+            ids.append(self._matrix(buf, offset, end, 1, end, _I32, name))
+        hid, tid, vid = ids
+        top = int(choices["mask"].max())
+        if top >= 0:
+            if allowed is None:
+                raise InvalidInput("a row reads a mask that is missing")
+            if allowed.dtype != np.uint32 and allowed.dtype != np.int32:
+                raise InvalidInput("masks must hold 32-bit integers")
+            mid = self._matrix(allowed, allowed_offset, allowed_stride, top + 1, words, allowed.dtype, "masks")
+        if adjusted is not None:
+            aid = self._matrix(adjusted, adjusted_offset, adjusted_stride, rows, vocab, _I64, "adjusted logits")
+        result = self._result(out, out_offset, rows, 1, rows, _I32)
+        a = _FixedChoose(lid, logits_offset, logits_stride, hid, history_offset, tid, bias_offset, vid, bias_offset, mid,
+                         allowed_offset, allowed_stride, aid, adjusted_offset, adjusted_stride, result.id, out_offset, vocab,
+                         bias_shift, 0)
+        return self._done(self.lib.volta_mi355x_fixed_choose_device(self.raw, a, choices.ctypes.data, rows), result, out)
 
     def _call_or_free(self, out: DeviceBuffer, fn, *args) -> None:
         rc = fn(self.raw, *args)
