@@ -161,6 +161,64 @@ def test_prefix_of_tokens_of_many_sequences(backend, dim, heads, kv_heads, batch
     check_prefix(backend, batch + prefix, [new] * batch, lengths, prefix, heads, kv_heads, dim)
 
 
+# Few rows of many sequences behind a long prefix read it together: 33 tiles and 124 units of 16 rows.
+TOGETHER = dict(counts=[1] * 31, prefix=2100, kv_heads=4)
+
+
+@pytest.mark.parametrize("dim", [1, 33, 64, 65, 128])
+@pytest.mark.parametrize("heads", [4, 12, 64])
+@pytest.mark.parametrize("prefix", [2049, 2111, 2112])
+def test_prefix_read_together(backend, dim, heads, prefix):
+    g = gen(dim + heads)
+    check_prefix(backend, prefix, TOGETHER["counts"], [int(n) for n in g.integers(1, 200, 31)], prefix, heads, 4, dim)
+
+
+@pytest.mark.parametrize("dim", [40, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefix_read_together_by_different_counts_rows_apart(backend, dim, causal):
+    g = gen(dim)
+    counts = [int(n) for n in g.integers(0, 4, 50)]
+    lengths = [max(n, int(m)) if causal else int(m) for n, m in zip(counts, g.integers(0, 300, 50))]
+    order = [int(i) for i in g.permutation(50)]
+    check_prefix(backend, dim, counts, lengths, 2100, 12, 4, dim, causal=causal, row_gap=2, gap=3, offset=1, order=order)
+    check_prefix(backend, dim + 1, [2] * 40, [n + 2 for n in lengths[:40]], 2100, 8, 4, dim, causal=causal, row_gap=1)
+
+
+@pytest.mark.parametrize("shift", [8, 13, 17, 24])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prefix_read_together_with_values_at_the_ends(backend, shift, dim):
+    g = gen(shift)
+    check_prefix(backend, shift, TOGETHER["counts"], [int(n) for n in g.integers(1, 100, 31)], 2100, 8, 4, dim, shift=shift,
+                 ends=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch", [63, 64, 65, 130, 192])
+def test_prefix_read_together_by_launches_of_64_sequences(backend, dim, batch):
+    g = gen(batch)
+    check_prefix(backend, batch, [1] * batch, [int(n) for n in g.integers(1, 90, batch)], 2000, 4, 4, dim)
+
+
+def test_prefix_read_together_beside_prompts(backend):
+    """Sequences of few rows and of many in one call."""
+    g = gen(4)
+    counts = [1, 200, 1, 90] + [1] * 40
+    lengths = [50, 200, 1, 130] + [int(n) for n in g.integers(1, 70, 40)]
+    check_prefix(backend, 8, counts, lengths, 2200, 8, 4, 64)
+    check_prefix(backend, 8, counts, lengths, 2200, 4, 4, 96)
+
+
+def test_prefix_read_together_longest_sums_of_equal_values(backend):
+    """65,536 keys of the same score with exponentials of 2^14 and values at the end: sums of a part near 2^31."""
+    for value in (32767, -32768):
+        q = [np.full((1, 2, 3), 100, np.int16) for _ in range(2)]
+        k = [np.full((n, 2, 3), 100, np.int16) for n in (1000, 36)]
+        v = [np.full((n, 2, 3), value, np.int16) for n in (1000, 36)]
+        pk, pv = np.full((64500, 2, 3), 100, np.int16), np.full((64500, 2, 3), value, np.int16)
+        got = run(backend, q, k, v, pk, pv, 13, np.full(4, 1 << 14, np.uint16))
+        assert all((part == value).all() for part in got)
+
+
 @pytest.mark.parametrize("dim,batch", [(64, 3), (64, 20), (128, 4)])
 @pytest.mark.parametrize("prefix", [64, 777])
 def test_prefix_of_many_prompts(backend, dim, batch, prefix):
