@@ -506,6 +506,58 @@ def test_choose_long_histories(backend):
     check_choose(backend, logits, rows, bias_shift=2, gap=5, offset=3)
 
 
+@pytest.mark.parametrize("repetition", [(1 << 15) - 1, 1 << 15, (1 << 15) + 1, 70001, (1 << 17) - 1, 1 << 17, (1 << 17) + 1])
+def test_choose_where_doubles_and_64_bits_end(backend, repetition):
+    """Logits, frequencies, presences and biases at the ends of what the shorter arithmetic holds, in rows of their own."""
+    g = gen(repetition)
+    end, rows, logits = 1 << 35, [], []
+    for top in (end - 1, end, end + 1):
+        for frequency, presence in ((0, 0), ((1 << 31) - 1, (1 << 55) - 1), (-(1 << 31) + 1, -(1 << 55) + 1), (1 << 31, 5),
+                                    (-(1 << 31), 1 << 55)):
+            logits.append(g.choice([top, -top, top - 1, 1 - top, 12345, -54321, 0, -1], 300))
+            rows.append(dict(history=g.integers(0, 300, 500), mask=None, frequency=frequency, presence=presence,
+                             repetition=repetition, biases=[(int(i), int(v)) for i, v in zip(
+                                 g.integers(0, 300, 40), g.choice([1, -1, (1 << 31) - 1, -(1 << 31)], 40))]))
+    logits = np.array(logits, np.int64)
+    for shift in (0, 10, 29, 30, 46):
+        check_choose(backend, logits, rows, bias_shift=shift)
+
+
+@pytest.mark.parametrize("biases", [511, 512, 513, 1500])
+def test_choose_many_biases(backend, biases):
+    """Biases of as many tokens as the table holds, of more, and several of a token."""
+    g = gen(biases)
+    rows = choice_rows(g, 2, 5000)
+    for r in rows:
+        r["biases"] = [(int(i), int(v)) for i, v in zip(g.permutation(5000)[:biases], g.integers(-9999, 9999, biases))]
+    rows[1]["biases"] = [(i % 400, v) for i, v in rows[1]["biases"]]
+    check_choose(backend, np.rint(g.normal(0, 3000, (2, 5000))).astype(np.int64), rows, bias_shift=1)
+
+
+@pytest.mark.parametrize("history", [32767, 32768])
+def test_choose_one_token_that_often(backend, history):
+    g = gen(history)
+    rows = [dict(history=[77] * history, biases=[(77, 5), (78, 6)], mask=None, frequency=3, presence=1, repetition=66000)]
+    check_choose(backend, g.integers(-10 ** 6, 10 ** 6, (1, 200)), rows)
+
+
+@pytest.mark.parametrize("vocab", [57343, 57344, 57345, 130001])
+def test_choose_rows_of_the_largest_chunks(backend, vocab):
+    """A workgroup a chunk of up to 57,344 tokens, of as many rows as there are CUs; three rows have lists."""
+    g = gen(vocab)
+    n = 256
+    logits = g.integers(-(1 << 30), 1 << 30, (n, vocab))
+    plain = dict(history=[], biases=[], mask=None, frequency=0, presence=0, repetition=65536)
+    rows = [plain] * n
+    some = [0, 100, 255]
+    for i, r in zip(some, choice_rows(g, 3, vocab, history=9000, biases=100)):
+        rows[i] = r
+    tokens, adjusted = logits.argmax(1), logits.copy()
+    tokens[some], adjusted[some] = want.choose(logits[some], [rows[i] for i in some], bias_shift=9)
+    got, out = run_choose(backend, logits, rows, bias_shift=9)
+    assert np.array_equal(got, tokens) and np.array_equal(out, adjusted)
+
+
 def test_choose_without_choices_is_the_largest(backend):
     g = gen(1)
     logits = g.integers(-99, 99, (70, 4000))

@@ -1144,37 +1144,50 @@ class Backend:
         if choices is None:
             choices = np.zeros(rows, FIXED_CHOICE)
             choices["mask"], choices["repetition"] = -1, 65536
-        if getattr(choices, "dtype", None) != FIXED_CHOICE or choices.shape != (rows,):
+        if type(choices) is not np.ndarray or choices.dtype != FIXED_CHOICE or choices.shape != (rows,):
             raise InvalidInput("choices are a FIXED_CHOICE array with an entry a row")
         if (bias_tokens is None) != (bias_values is None):
             raise InvalidInput("biases have tokens and values")
-        choices = np.ascontiguousarray(choices)
-        if not choices["repetition"].all():
+        if not choices.flags.c_contiguous:
+            choices = np.ascontiguousarray(choices)
+        # ends of the lists that the rows read, and the last mask
+        if rows <= 8:
+            history_end = bias_end = most = 0
+            top, least = -1, 1
+            for first, count, bias_first, bias_count, mask, _, _, repetition, _ in choices.tolist():
+                if count:
+                    history_end, most = max(history_end, first + count), max(most, count)
+                if bias_count:
+                    bias_end, most = max(bias_end, bias_first + bias_count), max(most, bias_count)
+                top, least = max(top, mask), min(least, repetition)
+        else:
+            ends = []
+            for name in ("history", "bias"):
+                count, first = choices[name + "_count"], choices[name + "_first"]
+                used = count > 0
+                # (sums past 2^64 are out of any buffer's bounds)
+                ends.append(int(np.where(first > (1 << 62), 1 << 62, first + count)[used].max(initial=0)))
+            history_end, bias_end = ends
+            most = int(max(choices["history_count"].max(), choices["bias_count"].max()))
+            top, least = int(choices["mask"].max()), int(choices["repetition"].min())
+        if least == 0:
             raise InvalidInput("repetition is zero")
+        if most > 1 << 24:
+            raise InvalidInput("a row's history or biases are too long")
+        if (history_end and history is None) or (bias_end and bias_tokens is None) or (top >= 0 and allowed is None):
+            raise InvalidInput("a row reads a list that is missing")
         words = (vocab + 31) // 32
         logits_stride = vocab if logits_stride is None else logits_stride
         allowed_stride = words if allowed_stride is None else allowed_stride
         adjusted_stride = vocab if adjusted_stride is None else adjusted_stride
         lid = self._matrix(logits, logits_offset, logits_stride, rows, vocab, _I64, "logits")
-        mid = aid = 0
-        lists = [("history", history, history_offset), ("bias", bias_tokens, bias_offset), ("bias", bias_values, bias_offset)]
-        ids = []
-        for name, buf, offset in lists:
-            count = choices[name + "_count"]
-            if buf is None:
-                if count.any():
-                    raise InvalidInput(f"a row reads a {name} that is missing")
-                ids.append(0)
-                continue
-            if (count > 1 << 24).any() or (choices[name + "_first"] >= 1 << 62).any():
-                raise InvalidInput(f"a row's {name} is out of range")
-            end = int((choices[name + "_first"] + count)[count > 0].max(initial=0))
-            ids.append(self._matrix(buf, offset, end, 1, end, _I32, name))
-        hid, tid, vid = ids
-        top = int(choices["mask"].max())
+        hid = tid = vid = mid = aid = 0
+        if history_end:
+            hid = self._matrix(history, history_offset, history_end, 1, history_end, _I32, "history")
+        if bias_end:
+            tid = self._matrix(bias_tokens, bias_offset, bias_end, 1, bias_end, _I32, "bias tokens")
+            vid = self._matrix(bias_values, bias_offset, bias_end, 1, bias_end, _I32, "bias values")
         if top >= 0:
-            if allowed is None:
-                raise InvalidInput("a row reads a mask that is missing")
             if allowed.dtype != np.uint32 and allowed.dtype != np.int32:
                 raise InvalidInput("masks must hold 32-bit integers")
             mid = self._matrix(allowed, allowed_offset, allowed_stride, top + 1, words, allowed.dtype, "masks")
