@@ -235,7 +235,9 @@ struct Tiles {
 // longest one decides, and it is done sooner; elsewhere two workgroups a CU hide
 // each other's waits better.  Prompts of 1,024 tokens, 12 heads, us with one team
 // and with two: one 42.7 and 32.9, four (384 workgroups) 48.1 and 40.1, six (576)
-// 52.9 and 61.3, sixteen 118 and 134.
+// 52.9 and 61.3, sixteen 118 and 134.  Behind a prefix or a window all workgroups
+// are about as long, and two teams pay up to one a CU only: one of 4,096 tokens with
+// a window of 1,024 (384 workgroups) 73.3 and 82.3, of 2,048 (192) 56.2 and 42.0.
 //
 // With heads over 64 (DC = 2) the two waves of a group take 32 tokens of a tile
 // each, exchange the exponentials through LDS, and keep half of the result's
@@ -1036,12 +1038,50 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
         if (map != WINDOW) return all;
         return std::min<size_t>(all, (a.window + FEW + 2 * FX_TILE - 2) / FX_TILE + (a.sinks + FX_TILE - 1) / FX_TILE);
     };
+    auto rows_of = [&](const FxSeq& s) { return size_t{s.count} * group; };
+    // Few rows of several sequences read a long prefix together.  us, one token a sequence,
+    // for units of 16 rows x tiles of the prefix, together and each sequence by itself:
+    //   heads of 64 (12 key heads)       of 128 (8 key heads)
+    //   24 x 250     31.6 and 42.2       16 x 250     47.6 and 46.8
+    //   48 x 63      21.9 and 20.7       32 x 63      30.8 and 26.3
+    //   96 x 63      23.8 and 35.0       64 x 63      34.1 and 35.0
+    //   768 x 4      25.5 and 17.8       512 x 4      33.7 and 22.4
+    //   768 x 16     26.6 and 29.4       512 x 16     35.1 and 37.5
+    //   768 x 250    49.1 and 266        512 x 250    82.7 and 372
+    // Three launches are 10 us; own tiles are as dear together as 32 rows', so that they
+    // should be the smaller part.  A tile of 32 rows takes the card 5.2 ns (3.9) together, one of
+    // 128 rows 7.7 (12) by itself: sequences of more than 47 (98) rows are better off so.
+    std::vector<FxSeq> rest;
+    if (map == PREFIX) {
+        std::vector<FxSeq> together;
+        size_t units = 0, own_tiles = 0;
+        for (size_t i = 0; i < count; ++i) {
+            const FxSeq& s = seqs[i];
+            if (rows_of(s) > (cache.dim <= 64 ? 47 : 98)) {
+                rest.push_back(s);
+                continue;
+            }
+            together.push_back(s);
+            units += (rows_of(s) + FEW - 1) / FEW * cache.kv_heads;
+            own_tiles += (s.length + FX_TILE - 1) / FX_TILE;
+        }
+        const size_t shared = (t.prefix + FX_TILE - 1) / FX_TILE, reads = units * shared;
+        if (together.size() > 1 && (reads >= 9000 || (reads >= 4000 && shared >= 32)) &&
+            2 * shared * together.size() >= own_tiles) {
+            bool no_space = false;
+            if (fx_prefix_attention(c, cache, t, together.data(), together.size(), &no_space)) return -1;
+            if (!no_space) {
+                if (rest.empty()) return 0;
+                seqs = rest.data();
+                count = rest.size();
+            }
+        }
+    }
     // Where many rows leave CUs idle, the kernel for few rows, which splits the
     // tiles, is faster.  Estimates in ns from measurements (rows x tokens, heads
     // of 128 on 4 key heads): 32 x 8,192 268 us by rows and 40 by tiles, 512 x
     // 8,192 368 and 92, eight of 128 x 4,096 191 and 96, 16 of 64 x 2,048 on 8
     // key heads 78 and 96, one prompt of 4,096 190 and more than that.
-    auto rows_of = [&](const FxSeq& s) { return size_t{s.count} * group; };
     auto tiles_of = [&](const FxSeq& s) {  // of a middle row
         const double all = static_cast<double>(s.length - (t.causal ? s.count / 2 : 0)) / FX_TILE + 1;
         if (map == WINDOW) return std::min(all, static_cast<double>(most_tiles(s)));
@@ -1073,29 +1113,6 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
         tiles = std::max(tiles, most_tiles(s));
         cols = std::max<size_t>(cols, std::min<size_t>(rows_of(s), FEW));
     }
-    // Few rows of several sequences read a long prefix together.  us, one token a sequence,
-    // for units x tiles of the prefix, together and each sequence by itself:
-    //   heads of 64 (12 key heads)       of 128 (8 key heads)
-    //   24 x 250     31.6 and 42.2       16 x 250     47.6 and 46.8
-    //   48 x 63      21.9 and 20.7       32 x 63      30.8 and 26.3
-    //   96 x 63      23.8 and 35.0       64 x 63      34.1 and 35.0
-    //   768 x 4      25.5 and 17.8       512 x 4      33.7 and 22.4
-    //   768 x 16     26.6 and 29.4       512 x 16     35.1 and 37.5
-    //   768 x 250    49.1 and 266        512 x 250    82.7 and 372
-    // Three launches are 10 us; own tiles are as dear together as 32 rows', so that they
-    // should be the smaller part.
-    size_t few_units = 0, own_tiles = 0;
-    for (const FxSeq& s : few) {
-        few_units += (rows_of(s) + FEW - 1) / FEW * cache.kv_heads;
-        own_tiles += (s.length + FX_TILE - 1) / FX_TILE;
-    }
-    const size_t shared_tiles = (t.prefix + FX_TILE - 1) / FX_TILE, reads = few_units * shared_tiles;
-    if (map == PREFIX && few.size() > 1 && (reads >= 9000 || (reads >= 4000 && shared_tiles >= 32)) &&
-        2 * shared_tiles * few.size() >= own_tiles) {
-        bool no_space = false;
-        if (fx_prefix_attention(c, cache, t, few.data(), few.size(), &no_space)) return -1;
-        if (!no_space) few.clear();
-    }
     if (!few.empty()) {
         bool no_space = false;
         if (few_rows(c, a, map, few, tiles, cols, &no_space)) return -1;
@@ -1115,7 +1132,7 @@ int fx_attention(Context* c, const FxCache& cache, const FxAttention& t, const F
                 constexpr Map MAP = decltype(m)::map;
                 if (cache.dim > 64)
                     hipLaunchKernelGGL((fx_attention_kernel<2, 1, MAP>), grid, dim3(512), 0, c->stream, a, q);
-                else if (workgroups <= 2 * static_cast<size_t>(c->cu_count))
+                else if (workgroups <= (MAP == ALL ? 2 : 1) * static_cast<size_t>(c->cu_count))
                     hipLaunchKernelGGL((fx_attention_kernel<1, 2, MAP>), grid, dim3(512), 0, c->stream, a, q);
                 else
                     hipLaunchKernelGGL((fx_attention_kernel<1, 1, MAP>), grid, dim3(256), 0, c->stream, a, q);
