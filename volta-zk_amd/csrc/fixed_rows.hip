@@ -236,7 +236,11 @@ __global__ __launch_bounds__(256) void fx_embed_kernel(FxEmbed a, uint32_t piece
 //
 // LANES lanes a head, four pairs of places each (what follows the pairs counts as
 // pairs that stay): a head's sum takes log2 LANES steps between neighbours, and both
-// places of a pair are in one lane.
+// places of a pair are in one lane, in one register.
+//
+// The norm is fx_norm_kernel's; R is at least half the root of V >= n h^2, so that a
+// quotient is below 2 sqrt(n) 2^15 in size and needs no bounds.  a c - b s = a c + (~b) s + s:
+// a product of two pairs that saturates at 32 bits, which the sum's clamp to 16 does not show.
 template <int LANES>
 __device__ inline int group_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2
@@ -261,88 +265,85 @@ __global__ __launch_bounds__(256) void fx_rotate_kernel(FxRotate a, uint32_t ite
     // kinds, or at the head's end, takes them one by one.
     const bool joint = a.adjacent || first >= a.pairs;
     const bool whole = joint ? 2 * first + 8 <= a.dim : first + 4 <= a.pairs;
-    auto load = [&](const int16_t* p, int* h) {
-        if (whole) {
-            Eight u;
-            if (joint) {
-                u.v = fx::load8(p + 2 * first);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) h[i] = u.e[i];
-            } else {
-                const uint2 lo = reinterpret_cast<const Row8*>(p + first)->v;
-                const uint2 hi = reinterpret_cast<const Row8*>(p + first + a.pairs)->v;
-                u.v = v4i{static_cast<int>(lo.x), static_cast<int>(lo.y), static_cast<int>(hi.x), static_cast<int>(hi.y)};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) h[2 * i] = u.e[i], h[2 * i + 1] = u.e[4 + i];
-            }
+    auto load = [&](const int16_t* p) {
+        v4i h;
+        if (whole && joint) {
+            h = fx::load8(p + 2 * first);
+        } else if (whole) {
+            const uint2 lo = reinterpret_cast<const Row8*>(p + first)->v;
+            const uint2 hi = reinterpret_cast<const Row8*>(p + first + a.pairs)->v;
+            h[0] = static_cast<int>(__builtin_amdgcn_perm(hi.x, lo.x, 0x05040100u));
+            h[1] = static_cast<int>(__builtin_amdgcn_perm(hi.x, lo.x, 0x07060302u));
+            h[2] = static_cast<int>(__builtin_amdgcn_perm(hi.y, lo.y, 0x05040100u));
+            h[3] = static_cast<int>(__builtin_amdgcn_perm(hi.y, lo.y, 0x07060302u));
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                h[2 * i] = one(first + i) < a.dim ? p[one(first + i)] : 0;
-                h[2 * i + 1] = two(first + i) < a.dim ? p[two(first + i)] : 0;
+                const uint16_t x = static_cast<uint16_t>(one(first + i) < a.dim ? p[one(first + i)] : 0);
+                const uint16_t y = static_cast<uint16_t>(two(first + i) < a.dim ? p[two(first + i)] : 0);
+                h[i] = static_cast<int>(x | static_cast<uint32_t>(y) << 16);
             }
         }
+        return h;
     };
-    int h[8];
-    load(x, h);
+    auto pair_of = [](int x, int y) { return static_cast<int>((static_cast<uint32_t>(x) & 0xffff) | static_cast<uint32_t>(y) << 16); };
+    auto clamp = [](int y) { return min(max(y, -32768), 32767); };
+    v4i h = load(x);
     const int16_t* gains = head < a.heads ? a.q_gain : a.k_gain;
     if (gains) {
-        int g[8];
-        load(gains, g);
+        const v4i g = load(gains);
         uint64_t q = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q += static_cast<uint32_t>(h[i] * h[i]);
+        for (int i = 0; i < 4; ++i) {
+            const int pair = h[i];
+            const v2s two = __builtin_bit_cast(v2s, pair);
+            q += static_cast<uint32_t>(__builtin_amdgcn_sdot2(two, two, 0, false));  // at most 2^31
+        }
         // at most 2^33 a lane: in parts of 20 bits
         const uint32_t low = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q & 0xfffff)));
         const uint32_t high = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q >> 20)));
         const uint64_t v = static_cast<uint64_t>(a.dim) * ((static_cast<uint64_t>(high) << 20) + low) + a.eps;
-        // as in fx_norm_kernel; |n h gain| <= 2^37
         const double below = 2.0 * static_cast<double>(floor_sqrt(v) << a.gain_shift), inv = 1.0 / below;
         const double half = 0.5 * below, n2 = 2.0 * a.dim;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const double top = __builtin_fma(n2, static_cast<double>(h[i] * g[i]), half);
+        auto normed = [&](int x, int gain) {
+            const double top = __builtin_fma(n2, static_cast<double>(__mul24(x, gain)), half);
             const double est = __builtin_floor(__builtin_fma(top, inv, 0x1p-34));
             const double rest = __builtin_fma(-est, below, top);
-            const double est_in = __builtin_fmin(__builtin_fmax(est, -1048576.0), 1048576.0);
-            const int y = static_cast<int>(est_in) + (__builtin_bit_cast(int64_t, rest) < 0 ? -1 : 0);
-            h[i] = min(max(y, -32768), 32767);
-        }
+            return clamp(static_cast<int>(est) + (__builtin_bit_cast(int64_t, rest) < 0 ? -1 : 0));
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            h[i] = pair_of(normed(static_cast<int16_t>(h[i]), static_cast<int16_t>(g[i])), normed(h[i] >> 16, g[i] >> 16));
     }
-    if (a.pairs && first < a.pairs) {
+    if (first < a.pairs) {
         const int64_t place = a.positions[row];
         if (place >= 0 && static_cast<size_t>(place) < a.angle_rows) {
-            const int16_t* turn = a.angles + (static_cast<size_t>(place) * a.pairs + first) * 2;
-            Eight u;
-            u.v = load8(turn, 0, 2 * (a.pairs - first));
+            const v4i turns = load8(a.angles + (static_cast<size_t>(place) * a.pairs + first) * 2, 0, 2 * (a.pairs - first));
+            const int half = a.angle_shift ? 1 << (a.angle_shift - 1) : 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (first + i >= a.pairs) continue;
-                // 2^31 at most: past 32 bits by one
-                const int64_t c = u.e[2 * i], s = u.e[2 * i + 1], p = h[2 * i], q = h[2 * i + 1];
-                h[2 * i] = sat16(rounded(p * c - q * s, a.angle_shift));
-                h[2 * i + 1] = sat16(rounded(p * s + q * c, a.angle_shift));
+                const int pair = h[i], less = pair ^ static_cast<int>(0xffff0000), cs = turns[i];
+                const int sc = static_cast<int>(__builtin_amdgcn_perm(cs, cs, 0x01000302u));
+                auto dot = [](int p, int q, int acc) {
+                    return __builtin_amdgcn_sdot2(__builtin_bit_cast(v2s, p), __builtin_bit_cast(v2s, q), acc, true);
+                };
+                h[i] = pair_of(clamp(dot(less, cs, half + (cs >> 16)) >> a.angle_shift), clamp(dot(pair, sc, half) >> a.angle_shift));
             }
         }
     }
-    if (whole) {
-        Eight u;
-        if (joint) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u.e[i] = static_cast<int16_t>(h[i]);
-            reinterpret_cast<Row16*>(out + 2 * first)->v = u.v;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u.e[i] = static_cast<int16_t>(h[2 * i]), u.e[4 + i] = static_cast<int16_t>(h[2 * i + 1]);
-            reinterpret_cast<Row8*>(out + first)->v = make_uint2(static_cast<uint32_t>(u.v[0]), static_cast<uint32_t>(u.v[1]));
-            reinterpret_cast<Row8*>(out + first + a.pairs)->v =
-                make_uint2(static_cast<uint32_t>(u.v[2]), static_cast<uint32_t>(u.v[3]));
-        }
+    if (whole && joint) {
+        reinterpret_cast<Row16*>(out + 2 * first)->v = h;
+    } else if (whole) {
+        reinterpret_cast<Row8*>(out + first)->v =
+            make_uint2(__builtin_amdgcn_perm(h[1], h[0], 0x05040100u), __builtin_amdgcn_perm(h[3], h[2], 0x05040100u));
+        reinterpret_cast<Row8*>(out + first + a.pairs)->v =
+            make_uint2(__builtin_amdgcn_perm(h[1], h[0], 0x07060302u), __builtin_amdgcn_perm(h[3], h[2], 0x07060302u));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (one(first + i) < a.dim) out[one(first + i)] = static_cast<int16_t>(h[2 * i]);
-            if (two(first + i) < a.dim) out[two(first + i)] = static_cast<int16_t>(h[2 * i + 1]);
+            if (one(first + i) < a.dim) out[one(first + i)] = static_cast<int16_t>(h[i]);
+            if (two(first + i) < a.dim) out[two(first + i)] = static_cast<int16_t>(h[i] >> 16);
         }
     }
 }
