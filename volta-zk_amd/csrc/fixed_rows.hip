@@ -238,7 +238,13 @@ __global__ __launch_bounds__(256) void fx_embed_kernel(FxEmbed a, uint32_t piece
 // pairs that stay): a head's sum takes log2 LANES steps between neighbours, and both
 // places of a pair are in one lane, in one register.
 //
-// The norm is fx_norm_kernel's; R is at least half the root of V >= n h^2, so that a
+// KEPT heads a lane, in turn: the root and the reciprocal cost as much as eight places'
+// quotients, and lane k of a head's lanes computes those of the k-th head for all.
+//
+// V is below 2^46, and a root that is no whole number at least 2^-24 below the next, far more
+// than its rounding: its floor is R.  The estimate of a quotient (below 2^20 in size) is
+// off by less than 2^-20, so that its floor with that much added is right or one too high, which
+// the exact remainder's sign shows.  R is at least half the root of V >= n h^2, so that a
 // quotient is below 2 sqrt(n) 2^15 in size and needs no bounds.  a c - b s = a c + (~b) s + s:
 // a product of two pairs that saturates at 32 bits, which the sum's clamp to 16 does not show.
 template <int LANES>
@@ -250,14 +256,11 @@ __device__ inline int group_sum(int v) {
     return v;
 }
 
-template <int LANES>
-__global__ __launch_bounds__(256) void fx_rotate_kernel(FxRotate a, uint32_t items) {
-    const uint32_t item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    if (item >= items) return;  // whole groups of lanes
-    const uint32_t row = item / a.all_heads, head = item - row * a.all_heads;
-    const int first = static_cast<int>(threadIdx.x % LANES) * 4;  // pair
-    const int16_t* x = a.x + row * a.x_stride + static_cast<size_t>(head) * a.dim;
-    int16_t* out = a.out + row * a.out_stride + static_cast<size_t>(head) * a.dim;
+template <int LANES, int KEPT>
+__global__ __launch_bounds__(256, 8) void fx_rotate_kernel(FxRotate a, uint32_t items) {
+    constexpr uint32_t HEADS = 64 / LANES;  // of a wave at a time
+    const int lane = threadIdx.x & 63, part = lane % LANES, first = part * 4;  // pair
+    const uint32_t item0 = (blockIdx.x * 4 + threadIdx.x / 64) * (HEADS * KEPT) + lane / LANES;
     // places of pair u: `one` and `two`
     auto one = [&](int u) { return a.adjacent || u >= a.pairs ? 2 * u : u; };
     auto two = [&](int u) { return a.adjacent || u >= a.pairs ? 2 * u + 1 : u + a.pairs; };
@@ -288,62 +291,94 @@ __global__ __launch_bounds__(256) void fx_rotate_kernel(FxRotate a, uint32_t ite
     };
     auto pair_of = [](int x, int y) { return static_cast<int>((static_cast<uint32_t>(x) & 0xffff) | static_cast<uint32_t>(y) << 16); };
     auto clamp = [](int y) { return min(max(y, -32768), 32767); };
-    v4i h = load(x);
-    const int16_t* gains = head < a.heads ? a.q_gain : a.k_gain;
-    if (gains) {
-        const v4i g = load(gains);
-        uint64_t q = 0;
+    v4i kept[KEPT];
+    uint32_t rows[KEPT], heads[KEPT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int pair = h[i];
-            const v2s two = __builtin_bit_cast(v2s, pair);
-            q += static_cast<uint32_t>(__builtin_amdgcn_sdot2(two, two, 0, false));  // at most 2^31
-        }
-        // at most 2^33 a lane: in parts of 20 bits
-        const uint32_t low = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q & 0xfffff)));
-        const uint32_t high = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q >> 20)));
-        const uint64_t v = static_cast<uint64_t>(a.dim) * ((static_cast<uint64_t>(high) << 20) + low) + a.eps;
-        const double below = 2.0 * static_cast<double>(floor_sqrt(v) << a.gain_shift), inv = 1.0 / below;
-        const double half = 0.5 * below, n2 = 2.0 * a.dim;
-        auto normed = [&](int x, int gain) {
-            const double top = __builtin_fma(n2, static_cast<double>(__mul24(x, gain)), half);
-            const double est = __builtin_floor(__builtin_fma(top, inv, 0x1p-34));
-            const double rest = __builtin_fma(-est, below, top);
-            return clamp(static_cast<int>(est) + (__builtin_bit_cast(int64_t, rest) < 0 ? -1 : 0));
-        };
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            h[i] = pair_of(normed(static_cast<int16_t>(h[i]), static_cast<int16_t>(g[i])), normed(h[i] >> 16, g[i] >> 16));
+    for (int k = 0; k < KEPT; ++k) {
+        const uint32_t item = item0 + k * HEADS;
+        rows[k] = item / a.all_heads;
+        heads[k] = item - rows[k] * a.all_heads;
+        kept[k] = v4i{0, 0, 0, 0};
+        if (item < items) kept[k] = load(a.x + rows[k] * a.x_stride + static_cast<size_t>(heads[k]) * a.dim);
     }
-    if (first < a.pairs) {
-        const int64_t place = a.positions[row];
-        if (place >= 0 && static_cast<size_t>(place) < a.angle_rows) {
-            const v4i turns = load8(a.angles + (static_cast<size_t>(place) * a.pairs + first) * 2, 0, 2 * (a.pairs - first));
-            const int half = a.angle_shift ? 1 << (a.angle_shift - 1) : 0;
+    double below = 1.0, inv = 1.0;
+    if (a.q_gain || a.k_gain) {
+        uint64_t sum = 0;  // of this lane's head
+#pragma unroll
+        for (int k = 0; k < KEPT; ++k) {
+            uint64_t q = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (first + i >= a.pairs) continue;
-                const int pair = h[i], less = pair ^ static_cast<int>(0xffff0000), cs = turns[i];
-                const int sc = static_cast<int>(__builtin_amdgcn_perm(cs, cs, 0x01000302u));
-                auto dot = [](int p, int q, int acc) {
-                    return __builtin_amdgcn_sdot2(__builtin_bit_cast(v2s, p), __builtin_bit_cast(v2s, q), acc, true);
-                };
-                h[i] = pair_of(clamp(dot(less, cs, half + (cs >> 16)) >> a.angle_shift), clamp(dot(pair, sc, half) >> a.angle_shift));
+                const int pair = kept[k][i];
+                const v2s two_places = __builtin_bit_cast(v2s, pair);
+                q += static_cast<uint32_t>(__builtin_amdgcn_sdot2(two_places, two_places, 0, false));  // at most 2^31
+            }
+            // at most 2^33 a lane: in parts of 20 bits
+            const uint32_t low = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q & 0xfffff)));
+            const uint32_t high = static_cast<uint32_t>(group_sum<LANES>(static_cast<int>(q >> 20)));
+            if (KEPT == 1 || part == k) sum = (static_cast<uint64_t>(high) << 20) + low;
+        }
+        const uint64_t v = static_cast<uint64_t>(a.dim) * sum + a.eps;
+        const double value = __builtin_fma(static_cast<double>(static_cast<uint32_t>(v >> 32)), 4294967296.0,
+                                           static_cast<double>(static_cast<uint32_t>(v)));
+        below = __builtin_floor(__builtin_sqrt(value)) * static_cast<double>(2u << a.gain_shift);
+        inv = __builtin_amdgcn_rcp(below);
+        inv = __builtin_fma(inv, __builtin_fma(-below, inv, 1.0), inv);
+        inv = __builtin_fma(inv, __builtin_fma(-below, inv, 1.0), inv);
+    }
+    const double n2 = 2.0 * a.dim;
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+        // of the k-th head
+        const int from = lane - part + k;
+        const double b = KEPT == 1 ? below : __shfl(below, from), r = KEPT == 1 ? inv : __shfl(inv, from), half_b = 0.5 * b;
+        if (item0 + k * HEADS >= items) break;
+        v4i h = kept[k];
+        const int16_t* gains = heads[k] < a.heads ? a.q_gain : a.k_gain;
+        if (gains) {
+            const v4i g = load(gains);
+            auto normed = [&](int x, int gain) {
+                const double top = __builtin_fma(n2, static_cast<double>(__mul24(x, gain)), half_b);
+                const double est = __builtin_floor(__builtin_fma(top, r, 0x1p-20));
+                const double rest = __builtin_fma(-est, b, top);
+                return clamp(static_cast<int>(est) + (__builtin_bit_cast(int64_t, rest) < 0 ? -1 : 0));
+            };
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                h[i] = pair_of(normed(static_cast<int16_t>(h[i]), static_cast<int16_t>(g[i])), normed(h[i] >> 16, g[i] >> 16));
+        }
+        if (first < a.pairs) {
+            const int64_t place = a.positions[rows[k]];
+            if (place >= 0 && static_cast<size_t>(place) < a.angle_rows) {
+                const v4i turns = load8(a.angles + (static_cast<size_t>(place) * a.pairs + first) * 2, 0, 2 * (a.pairs - first));
+                const int half = a.angle_shift ? 1 << (a.angle_shift - 1) : 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (first + i >= a.pairs) continue;
+                    const int pair = h[i], less = pair ^ static_cast<int>(0xffff0000), cs = turns[i];
+                    const int sc = static_cast<int>(__builtin_amdgcn_perm(cs, cs, 0x01000302u));
+                    auto dot = [](int p, int q, int acc) {
+                        return __builtin_amdgcn_sdot2(__builtin_bit_cast(v2s, p), __builtin_bit_cast(v2s, q), acc, true);
+                    };
+                    h[i] = pair_of(clamp(dot(less, cs, half + (cs >> 16)) >> a.angle_shift),
+                                   clamp(dot(pair, sc, half) >> a.angle_shift));
+                }
             }
         }
-    }
-    if (whole && joint) {
-        reinterpret_cast<Row16*>(out + 2 * first)->v = h;
-    } else if (whole) {
-        reinterpret_cast<Row8*>(out + first)->v =
-            make_uint2(__builtin_amdgcn_perm(h[1], h[0], 0x05040100u), __builtin_amdgcn_perm(h[3], h[2], 0x05040100u));
-        reinterpret_cast<Row8*>(out + first + a.pairs)->v =
-            make_uint2(__builtin_amdgcn_perm(h[1], h[0], 0x07060302u), __builtin_amdgcn_perm(h[3], h[2], 0x07060302u));
-    } else {
+        int16_t* out = a.out + rows[k] * a.out_stride + static_cast<size_t>(heads[k]) * a.dim;
+        if (whole && joint) {
+            reinterpret_cast<Row16*>(out + 2 * first)->v = h;
+        } else if (whole) {
+            reinterpret_cast<Row8*>(out + first)->v =
+                make_uint2(__builtin_amdgcn_perm(h[1], h[0], 0x05040100u), __builtin_amdgcn_perm(h[3], h[2], 0x05040100u));
+            reinterpret_cast<Row8*>(out + first + a.pairs)->v =
+                make_uint2(__builtin_amdgcn_perm(h[1], h[0], 0x07060302u), __builtin_amdgcn_perm(h[3], h[2], 0x07060302u));
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (one(first + i) < a.dim) out[one(first + i)] = static_cast<int16_t>(h[i]);
-            if (two(first + i) < a.dim) out[two(first + i)] = static_cast<int16_t>(h[i] >> 16);
+            for (int i = 0; i < 4; ++i) {
+                if (one(first + i) < a.dim) out[one(first + i)] = static_cast<int16_t>(h[i]);
+                if (two(first + i) < a.dim) out[two(first + i)] = static_cast<int16_t>(h[i] >> 16);
+            }
         }
     }
 }
@@ -351,8 +386,15 @@ __global__ __launch_bounds__(256) void fx_rotate_kernel(FxRotate a, uint32_t ite
 template <int LANES>
 void launch_rotate(Context* c, const FxRotate& a) {
     const uint32_t items = static_cast<uint32_t>(a.rows) * a.all_heads;
-    hipLaunchKernelGGL(fx_rotate_kernel<LANES>, dim3((items + 256 / LANES - 1) / (256 / LANES)), dim3(256), 0, c->stream,
-                       a, items);
+    auto launch = [&](auto kernel, uint32_t each) {
+        hipLaunchKernelGGL(kernel, dim3((items + each - 1) / each), dim3(256), 0, c->stream, a, items);
+    };
+    // Two heads a lane where they have norms and are many.  16,384 rows of 24 heads of 64, us with
+    // one, two and four: 30.5, 28.5, 32.1.
+    if ((a.q_gain || a.k_gain) && items >= 512u / LANES * 4 * static_cast<uint32_t>(c->cu_count))
+        launch(fx_rotate_kernel<LANES, 2>, 512 / LANES);
+    else
+        launch(fx_rotate_kernel<LANES, 1>, 256 / LANES);
 }
 
 template <int THREADS, int KEPT>
