@@ -162,17 +162,23 @@ __global__ __launch_bounds__((64 * WAVES<DC, SUMS>)) void fx_prefix_kernel(Atten
     const bool no_offset = !__any(mine.o);
     // index of this lane's row in a part's tops
     const size_t mine_at = static_cast<size_t>(token) * heads + static_cast<size_t>(head) * a.group + member;
+    // Whether block b of tile t needs no offsets.
+    auto is_plain = [&](const Tile& t, int b, const Keys<DC>& k) {
+        return no_offset && !__any(t.first + b * 32 + (lane & 31) < t.written && (k.extra & 128));
+    };
+    // Whether all rows see tile t whole, without offsets: most tiles, and the first ones.
+    auto is_whole = [&](const Tile& t, const Keys<DC>* k) {
+        return a.s2 == 0 && t.seq < 0 && t.first + FX_TILE <= t.written && is_plain(t, 0, k[0]) && is_plain(t, 1, k[1]);
+    };
     // Scores of block b of tile t from keys k, which then are on their way for tile `next`.
     auto scores_of = [&](const Tile& t, int b, Keys<DC>* k, const Tile& next) {
         const Raw raw = products<DC>(*k, mine);
-        const bool large = t.first + b * 32 + (lane & 31) < t.written && (k->extra & 128);
-        const bool plain = no_offset && !__any(large);
+        const bool plain = is_plain(t, b, *k);
         load_keys<DC>(next.rec, b, lane, k);
         return scores<DC>(raw, reinterpret_cast<const int*>(t.rec + Record<DC>::EXTRA), mine, b, lane, a.s1, a.s2, plain);
     };
-    // Keys of a tile that this lane's row sees, and whether all rows see 32 from `first` on.
+    // Keys of a tile that this lane's row sees.
     auto limit_in = [&](const Tile& t) { return t.seq < 0 ? t.written : t.seq == static_cast<int>(seq) ? limit : 0; };
-    auto all_see = [&](const Tile& t, int first) { return t.seq < 0 && first + 32 <= t.written; };
 
     if constexpr (!SUMS) {
         int top = INT_MIN;
@@ -183,7 +189,7 @@ __global__ __launch_bounds__((64 * WAVES<DC, SUMS>)) void fx_prefix_kernel(Atten
             for (int b = 0; b < 2; ++b) {
                 const int first = t->first + b * 32;
                 const v16i z = scores_of(*t, b, &k[b], next);
-                if (all_see(*t, first)) {
+                if (t->seq < 0 && first + 32 <= t->written) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) top = max(top, z[r]);
                 } else {
@@ -215,13 +221,12 @@ __global__ __launch_bounds__((64 * WAVES<DC, SUMS>)) void fx_prefix_kernel(Atten
         const uint32_t last = a.entries - 1;
         v16i hh[2 * DC] = {}, mid[2 * DC] = {}, ll[2 * DC] = {};
         int sum_h = 0, sum_l = 0;
-        auto exponentials = [&](const v16i& z, const Tile& t, int b, v4i* eh, v4i* el) {
-            const int first = t.first + b * 32;
+        // of 32 tokens with scores z(r), from `first` on, of which the lane's row sees those below `here`
+        auto exponentials = [&](auto&& z, bool whole, int first, int here, v4i* eh, v4i* el) {
             uint32_t e[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z[r]), last)];
-            if (!all_see(t, first)) {
-                const int here = limit_in(t);
+            for (int r = 0; r < 16; ++r) e[r] = table[min(static_cast<uint32_t>(top) - static_cast<uint32_t>(z(r)), last)];
+            if (!whole) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (first + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= here) e[r] = 0;
@@ -252,18 +257,36 @@ __global__ __launch_bounds__((64 * WAVES<DC, SUMS>)) void fx_prefix_kernel(Atten
                 mid[d] = mfma32(v.l[d], eh, mid[d]);
             }
         };
-        Values values[2];
-        if (begin < to) load_values(now[0], 0, &values[0]);
-        for (int i = begin; i < to; i += W) {
-            // the next block's values on their way while this one's are used
+        // (Sums added beside the next block's exponentials, in an order set for it, would overlap the matrix
+        // cores and the vector units; the registers that takes spilled: 105 us for 40.)
+        Values values;
+        int i = begin;
+        for (; i < to; i += W) {
+            const Tile t = now[0];
+            if (!is_whole(t, keys[0])) break;
+            const Tile next = tile(min(i + W, to - 1));
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                load_values(t, b, &values);
+                const Raw s = products<DC>(keys[0][b], mine);
+                load_keys<DC>(next.rec, b, lane, &keys[0][b]);
+                v4i eh, el;
+                exponentials([&](int r) { return score(s, r, a.s1); }, true, 0, 0, &eh, &el);
+                add(values, eh, el);
+            }
+            now[0] = next;
+        }
+        for (; i < to; i += W) {
             const Tile t = now[0], next = tile(min(i + W, to - 1));
-            v4i eh, el;
-            exponentials(scores_of(t, 0, &keys[0][0], next), t, 0, &eh, &el);
-            load_values(t, 1, &values[1]);
-            add(values[0], eh, el);
-            exponentials(scores_of(t, 1, &keys[0][1], next), t, 1, &eh, &el);
-            load_values(next, 0, &values[0]);
-            add(values[1], eh, el);
+            const int here = limit_in(t);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                load_values(t, b, &values);
+                const v16i z = scores_of(t, b, &keys[0][b], next);
+                v4i eh, el;
+                exponentials([&](int r) { return z[r]; }, false, t.first + b * 32, here, &eh, &el);
+                add(values, eh, el);
+            }
             now[0] = next;
         }
         // Each wave's sums to LDS, then their sums to memory.  (Additions in LDS took 5 us.)
