@@ -93,6 +93,30 @@ def test_choices(backend):
             b.fixed_choose_device(l, *args, **kw)
 
 
+def test_unused_lists_may_start_anywhere(backend):
+    """What reaches the library: rows without entries do not count, wherever their lists start."""
+    b, calls = backend, []
+
+    class Library:
+        def volta_mi355x_fixed_choose_device(self, raw, args, choices, rows):
+            calls.append((args.history_id, args.bias_tokens_id, rows))
+            return 0
+
+    b.lib = Library()
+    l, i, out = b.alloc_device(400, np.int64), b.alloc_device(100, np.int32), b.alloc_device(9, np.int32)
+    for n in (1, 2, 9):
+        c = choices(n, history_first=(1 << 64) - 1, bias_first=1 << 63)
+        b.fixed_choose_device(l, n, 10, c, out=out)
+        c["history_first"][-1], c["history_count"][-1] = 98, 2
+        b.fixed_choose_device(l, n, 10, c, history=i, out=out)
+        c["bias_first"][-1], c["bias_count"][-1] = 0, 100
+        b.fixed_choose_device(l, n, 10, c, history=i, bias_tokens=i, bias_values=i, out=out)
+        c["history_first"][-1] = 99
+        with pytest.raises(InvalidInput):
+            b.fixed_choose_device(l, n, 10, c, history=i, bias_tokens=i, bias_values=i, out=out)
+    assert calls == [(h * i.id, t * i.id, n) for n in (1, 2, 9) for h, t in ((0, 0), (1, 0), (1, 1))]
+
+
 def test_entry_points_without_a_context_or_arguments():
     from volta_mi355x import load_library
     lib = load_library()

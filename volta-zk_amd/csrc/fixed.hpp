@@ -229,8 +229,8 @@ struct FxAttention {
 int fx_kv_append(Context* c, const FxCache& cache, const int16_t* k, size_t k_stride, const int16_t* v, size_t v_stride,
                  const FxSeq* seqs, size_t count);
 int fx_attention(Context* c, const FxCache& cache, const FxAttention& a, const FxSeq* seqs, size_t count);
-// Attention of few rows a sequence behind a prefix, which is read for all sequences at
-// once.  *no_space, with nothing launched, where its workspace may not grow.
+// Attention behind a prefix, which 32 rows of any sequences read at once.  *no_space, with
+// nothing launched, where its workspace may not grow or would be too large.
 int fx_prefix_attention(Context* c, const FxCache& cache, const FxAttention& a, const FxSeq* seqs, size_t count,
                         bool* no_space);
 

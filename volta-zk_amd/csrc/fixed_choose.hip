@@ -185,7 +185,7 @@ __global__ __launch_bounds__(THREADS) void fx_choose_kernel(FxChoose a, Settings
     __shared__ int64_t queued[THREADS / 64][128];     // logits
     __shared__ uint32_t queued_at[THREADS / 64][128];  // tokens of the chunk, and bit 31: allowed
     const uint32_t row_at = blockIdx.x / chunks, part = blockIdx.x - row_at * chunks;
-    const FxChoice r = rows ? rows[row_at] : settings.row[row_at];
+    const FxChoice r = row_at < FX_CHOICES ? settings.row[row_at] : rows[row_at - FX_CHOICES];
     const Row row(a, r, row_at);
     const uint32_t base = part * chunk, here = min(a.vocab - base, chunk);
     const bool listed = r.history_count | r.bias_count;
@@ -368,11 +368,12 @@ int fx_choose(Context* c, const FxChoose& a, const FxChoice* rows, size_t count)
         listed |= rows[i].history_count || rows[i].bias_count;
         dense |= rows[i].history_count > HISTORY_MAX || rows[i].bias_count > BIAS_MAX;
     }
-    // Chunks of at least 1,024 tokens, for a workgroup a CU: each counts all of its row's lists.  us
-    // with one, two (of half the threads), four and eight a CU: 256 rows of 50,257 43.7, 49.0,
-    // 55.8, 68.7; 64 rows 20.9, 20.9, 25.0, 36.9.
+    // Chunks of at least 1,024 tokens (many rows: a pass of all threads), for a workgroup a CU:
+    // each counts all of its row's lists.  us with one, two (of half the threads), four and
+    // eight a CU: 256 rows of 50,257 43.7, 49.0, 55.8, 68.7; 64 rows 20.9, 20.9, 25.0, 36.9.
     const size_t want = (c->cu_count + count - 1) / count;
-    const uint32_t least = (a.vocab + CHUNK - 1) / CHUNK, most = (a.vocab + 1023) / 1024;
+    const uint32_t least = (a.vocab + CHUNK - 1) / CHUNK, short_chunk = count < 32 ? 1024 : PAIRS * THREADS * 2,
+                   most = (a.vocab + short_chunk - 1) / short_chunk;
     uint32_t groups = std::max(least, static_cast<uint32_t>(std::min<size_t>(want, most)));
     const uint32_t chunk = ((a.vocab + groups - 1) / groups + 63) / 64 * 64;  // whole words of a mask
     groups = (a.vocab + chunk - 1) / chunk;
@@ -387,18 +388,19 @@ int fx_choose(Context* c, const FxChoose& a, const FxChoice* rows, size_t count)
         if (count > FX_CHOICES) in_memory = reinterpret_cast<FxChoice*>(ws<unsigned char>(c, WS_FIXED) + best_bytes);
     }
     Settings s;
-    for (size_t at = 0; at < count; at += FX_CHOICES) {
+    for (size_t at = dense || !in_memory ? 0 : FX_CHOICES; at < count; at += FX_CHOICES) {
         const size_t here = std::min<size_t>(count - at, FX_CHOICES);
         std::copy(rows + at, rows + at + here, s.row);
         if (dense)
             hipLaunchKernelGGL(fx_choose_dense_kernel, dim3(static_cast<unsigned>(here)), dim3(256), 0, c->stream, a, s,
                                static_cast<uint32_t>(at));
         else if (in_memory)
-            hipLaunchKernelGGL(fx_choose_settings_kernel, dim3(1), dim3(FX_CHOICES), 0, c->stream, s, in_memory + at,
-                               static_cast<uint32_t>(here));
+            hipLaunchKernelGGL(fx_choose_settings_kernel, dim3(1), dim3(FX_CHOICES), 0, c->stream, s,
+                               in_memory + at - FX_CHOICES, static_cast<uint32_t>(here));
         VMX_HIP(c, hipGetLastError());
     }
     if (dense) return 0;
+    std::copy(rows, rows + std::min<size_t>(count, FX_CHOICES), s.row);
     hipLaunchKernelGGL(fx_choose_kernel, dim3(static_cast<unsigned>(count * groups)), dim3(THREADS),
                        listed ? (chunk + 7) / 8 * 16 : 0, c->stream, a, s, in_memory, chunk, bests);
     VMX_HIP(c, hipGetLastError());

@@ -414,7 +414,7 @@ int fx_prefix_attention(Context* c, const FxCache& cache, const FxAttention& t, 
         const Launch l = make(at);
         most = std::max(most, rows_of(l) * (8 * places + 4) + 4 * l.tops.top_parts * l.rows() * t.heads);
     }
-    *no_space = !try_ws(c, WS_FIXED, workspace_step(most, FX_SPACE_MAX));
+    *no_space = most > FX_SPACE_MAX || !try_ws(c, WS_FIXED, workspace_step(most, FX_SPACE_MAX));
     if (*no_space) return 0;
     for (size_t at = 0; at < count; at += FX_SEQS) {
         Launch l = make(at);

@@ -1150,30 +1150,32 @@ class Backend:
             raise InvalidInput("biases have tokens and values")
         if not choices.flags.c_contiguous:
             choices = np.ascontiguousarray(choices)
-        # ends of the lists that the rows read, and the last mask
-        if rows <= 8:
-            history_end = bias_end = most = 0
-            top, least = -1, 1
-            for first, count, bias_first, bias_count, mask, _, _, repetition, _ in choices.tolist():
-                if count:
-                    history_end, most = max(history_end, first + count), max(most, count)
-                if bias_count:
-                    bias_end, most = max(bias_end, bias_first + bias_count), max(most, bias_count)
-                top, least = max(top, mask), min(least, repetition)
+        # Ends of the lists that the rows read and the last mask, from the largest entries of all rows: the exact
+        # ends where those are not inside the buffers.  (The entry point checks each row.)
+        m = choices.view(np.int64).reshape(rows, 8)
+        if rows == 1:
+            low = high = m[0].tolist()
         else:
-            ends = []
-            for name in ("history", "bias"):
-                count, first = choices[name + "_count"], choices[name + "_first"]
-                used = count > 0
-                # (sums past 2^64 are out of any buffer's bounds)
-                ends.append(int(np.where(first > (1 << 62), 1 << 62, first + count)[used].max(initial=0)))
-            history_end, bias_end = ends
-            most = int(max(choices["history_count"].max(), choices["bias_count"].max()))
-            top, least = int(choices["mask"].max()), int(choices["repetition"].min())
-        if least == 0:
+            low, high = m.min(axis=0).tolist(), m.max(axis=0).tolist()
+        history_end = high[0] + high[1] if high[1] else 0
+        bias_end = high[2] + high[3] if high[3] else 0
+        if rows > 1 and (min(low[0], low[2]) < 0 or
+                         history is not None and history_offset + history_end > history.len or
+                         bias_tokens is not None and bias_offset + bias_end > min(bias_tokens.len, bias_values.len)):
+            if min(low[:4]) >= 0 and max(high[0], high[2], high[1], high[3]) < 1 << 62:
+                ends = (m[:, 0:4:2] + m[:, 1:4:2]) * (m[:, 1:4:2] > 0)
+                history_end, bias_end = ends.max(axis=0).tolist()
+            else:
+                used = m[:, :4].astype(object) * (m[:, [1, 1, 3, 3]] > 0)
+                history_end, bias_end = (used[:, 0] + used[:, 1]).max(), (used[:, 2] + used[:, 3]).max()
+                low[0], low[2] = used[:, 0].min(), used[:, 2].min()
+        top = high[4]
+        if low[7] == 0:
             raise InvalidInput("repetition is zero")
-        if most > 1 << 24:
+        if max(high[1], high[3]) > 1 << 24 or min(low[1], low[3]) < 0:
             raise InvalidInput("a row's history or biases are too long")
+        if (high[1] and low[0] < 0) or (high[3] and low[2] < 0):  # past 2^63
+            raise InvalidInput("a row's history or biases are out of range")
         if (history_end and history is None) or (bias_end and bias_tokens is None) or (top >= 0 and allowed is None):
             raise InvalidInput("a row reads a list that is missing")
         words = (vocab + 31) // 32
