@@ -451,6 +451,12 @@ def test_choose_many_rows(backend, rows):
     check_choose(backend, logits, choice_rows(g, rows, 2500, history=60, biases=11), junk=3, mask_gap=2)
 
 
+def test_choose_more_rows_than_a_launch_takes(backend):
+    g = gen(8200)
+    logits = np.rint(g.normal(0, 3000, (8200, 5))).astype(np.int64)
+    check_choose(backend, logits, choice_rows(g, 8200, 5, history=4, biases=2), mask_gap=1, gap=2, adjusted="new")
+
+
 @pytest.mark.parametrize("bias_shift", [0, 30, 46])
 def test_choose_logits_at_the_ends(backend, bias_shift):
     """Products and sums far beyond 64 bits, clamped once."""

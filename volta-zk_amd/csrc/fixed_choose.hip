@@ -124,7 +124,7 @@ struct Rule {
     // l with n occurrences and a sum of biases below 2^55 in size (before the shift, which
     // is at most 46).
     __device__ int64_t operator()(int64_t l, uint32_t n, int64_t bias) const {
-        if (__all(narrow && bias < bias_max && bias > -bias_max && static_cast<uint32_t>(static_cast<int>(l >> 32) + 8) < 16))
+        if (__all(narrow && bias < bias_max && bias > -bias_max && static_cast<uint32_t>(l >> 32) + 8 < 16))
             return (n ? narrow_penalty(l, n) : l) + static_cast<int64_t>(static_cast<uint64_t>(bias) << bias_shift);
         const __int128 x = n ? penalized(l, n, r) : static_cast<__int128>(l);
         return clamped(x + (static_cast<__int128>(bias) << bias_shift));
@@ -360,9 +360,11 @@ __global__ __launch_bounds__(256) void fx_choose_dense_kernel(FxChoose a, Settin
     if (threadIdx.x == 0) a.tokens[first_row + blockIdx.x] = best.token;
 }
 
-}  // namespace
+// Rows of one launch: CALL_ROWS at most, as a grid holds less than 2^32 threads, and 2^24
+// tokens are 293 chunks.
+constexpr size_t CALL_ROWS = 4096;
 
-int fx_choose(Context* c, const FxChoose& a, const FxChoice* rows, size_t count) {
+int choose_rows(Context* c, const FxChoose& a, const FxChoice* rows, size_t count) {
     bool listed = false, dense = false;
     for (size_t i = 0; i < count; ++i) {
         listed |= rows[i].history_count || rows[i].bias_count;
@@ -382,8 +384,7 @@ int fx_choose(Context* c, const FxChoose& a, const FxChoice* rows, size_t count)
     FxChoice* in_memory = nullptr;
     if (!dense && (groups > 1 || count > FX_CHOICES)) {
         const size_t best_bytes = count * groups * sizeof(Best);
-        dense = count * groups > INT32_MAX ||
-                !try_ws(c, WS_FIXED, workspace_step(best_bytes + count * sizeof(FxChoice), FX_SPACE_MAX));
+        dense = !try_ws(c, WS_FIXED, workspace_step(best_bytes + count * sizeof(FxChoice), FX_SPACE_MAX));
         bests = ws<Best>(c, WS_FIXED);
         if (count > FX_CHOICES) in_memory = reinterpret_cast<FxChoice*>(ws<unsigned char>(c, WS_FIXED) + best_bytes);
     }
@@ -408,6 +409,19 @@ int fx_choose(Context* c, const FxChoose& a, const FxChoice* rows, size_t count)
         hipLaunchKernelGGL(fx_choose_join_kernel, dim3(static_cast<unsigned>(count)), dim3(64), 0, c->stream, bests, groups,
                            a.tokens);
         VMX_HIP(c, hipGetLastError());
+    }
+    return 0;
+}
+
+}  // namespace
+
+int fx_choose(Context* c, const FxChoose& a, const FxChoice* rows, size_t count) {
+    FxChoose part = a;
+    for (size_t row = 0; row < count; row += CALL_ROWS) {
+        part.logits = a.logits + row * a.logits_stride;
+        part.adjusted = a.adjusted ? a.adjusted + row * a.adjusted_stride : nullptr;
+        part.tokens = a.tokens + row;
+        if (choose_rows(c, part, rows + row, std::min(count - row, CALL_ROWS))) return -1;
     }
     return 0;
 }

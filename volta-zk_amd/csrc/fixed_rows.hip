@@ -238,6 +238,10 @@ __global__ __launch_bounds__(256) void fx_embed_kernel(FxEmbed a, uint32_t piece
 // pairs that stay): a head's sum takes log2 LANES steps between neighbours, and both
 // places of a pair are in one lane, in one register.
 //
+// With gains, bound by vector instructions (f64: 0.70 of their issue) beside memory: 16,384 rows
+// of 24 heads of 64 28.5 us, 101 MB at 3.5 TB/s.  Without them by memory: 4,095 rows of 40 heads
+// of 128, 96 places of each turned, 16 us, 84 MB at 5.2 TB/s.
+//
 // KEPT heads a lane, in turn: the root and the reciprocal cost as much as eight places'
 // quotients, and lane k of a head's lanes computes those of the k-th head for all.
 //
