@@ -547,6 +547,19 @@ def test_choose_one_token_that_often(backend, history):
     check_choose(backend, g.integers(-10 ** 6, 10 ** 6, (1, 200)), rows)
 
 
+@pytest.mark.parametrize("vocab", [1, 2815, 2816, 2817, 20480, 20481, 60001])
+@pytest.mark.parametrize("biases", [0, 512, 513, 2048, 2049, 5000])
+@pytest.mark.parametrize("rows", [2, 70])
+def test_choose_lists_beyond_the_short_ones(backend, vocab, biases, rows):
+    """Histories that 15 bits do not count, more biases than half a table holds, on the edges of their chunks."""
+    g = gen(vocab + biases)
+    some = choice_rows(g, rows, vocab, history=30, biases=20)
+    for r in (some[0], some[-1]):
+        r["history"] = np.concatenate([np.full(32768, vocab // 2), g.integers(0, vocab, 900)])
+        r["biases"] = [(int(t), int(v)) for t, v in zip(g.integers(-3, vocab + 3, biases), g.integers(-9999, 9999, biases))]
+    check_choose(backend, np.rint(g.normal(0, 9000, (rows, vocab))).astype(np.int64), some, bias_shift=4)
+
+
 @pytest.mark.parametrize("vocab", [57343, 57344, 57345, 130001])
 def test_choose_rows_of_the_largest_chunks(backend, vocab):
     """A workgroup a chunk of up to 57,344 tokens, of as many rows as there are CUs; three rows have lists."""

@@ -10,14 +10,15 @@
 // its tie-break: no order of threads or workgroups changes a result.
 //
 // A workgroup takes a chunk of a row's vocabulary.  It counts the history's entries that
-// fall into it in LDS, 15 bits a token, and goes over its logits once.  Few tokens are in
-// a list, but nearly every 64 hold one: a wave queues those with their logits and changes
-// 64 at a time, all lanes at work.  (In place, all waves went through the arithmetic; in a
-// second pass over the lists their logits came from memory again.  256 rows of 50,257,
-// 6,100 tokens of history each: 50 and 48 us, 32 by the queue.)  The sum of a token's biases is in a hash table
-// in LDS, which a bit beside the count says to look into.  A second launch joins the
-// chunks' best.  Where lists are too long for that, or no workspace may grow, a workgroup
-// takes a row, with a wide count and sum for each token of a small chunk at a time.
+// fall into it in LDS, 15 bits a token (31 behind histories that need them), and goes over
+// its logits once.  Few tokens are in a list, but nearly every 64 hold one: a wave queues
+// those with their logits and changes 64 at a time, all lanes at work.  (In place, all waves
+// went through the arithmetic; in a second pass over the lists their logits came from memory
+// again.  256 rows of 50,257, 6,100 tokens of history each: 50 and 48 us, 35 by the queue,
+// 110 MB at 3.1 TB/s.)  The sum of a token's biases is in a hash table in LDS, which a bit
+// beside the count says to look into.  A second launch joins the chunks' best.  Where no
+// workspace may grow, a workgroup takes a row, with a count and a sum for each token of a
+// small chunk at a time.
 #include <algorithm>
 #include <climits>
 
@@ -29,9 +30,27 @@ namespace {
 using namespace fx;
 
 constexpr int DENSE = 2048;            // tokens of a chunk with wide counts and sums
-constexpr uint32_t CHUNK = 56 * 1024;  // and, at most, of one with counts of 15 bits
-constexpr uint32_t HISTORY_MAX = 0x7fff, BIASED = 0x8000;
-constexpr uint32_t BIAS_MAX = 512, SLOTS = 1024;  // biases of a row, and slots of their table
+// A chunk's lists in LDS: occurrences of its tokens, each with a bit that says that it has
+// biases, and a table of the biases' sums.  Short lists have two tokens a word and a small table.
+template <bool WIDE>
+struct Lists {
+    static constexpr uint32_t BIASED = WIDE ? 1u << 31 : 0x8000, MOST = BIASED - 1;
+    static constexpr uint32_t CHUNK = (WIDE ? 20 : 56) * 1024;  // tokens of a chunk, at most
+    // Half of the slots hold all biases of a row, or, where those are more, those of a chunk
+    // of FEW tokens.
+    static constexpr uint32_t BITS = WIDE ? 12 : 10, SLOTS = 1u << BITS, BIASES = SLOTS / 2, FEW = SLOTS / 16 * 11;
+    __device__ static uint32_t slot_of(uint32_t token) { return (token * 0x9e3779b1u) >> (32 - BITS); }
+    __device__ static uint32_t word(uint32_t t) { return WIDE ? t : t >> 1; }
+    __device__ static uint32_t shift(uint32_t t) { return WIDE ? 0 : 16 * (t & 1); }
+    __device__ static uint32_t of(const uint32_t* counts, uint32_t t) {
+        return WIDE ? counts[t] : counts[t >> 1] >> (16 * (t & 1)) & 0xffff;
+    }
+    // of t and t + 1, t even
+    __device__ static uint2 two(const uint32_t* counts, uint32_t t) {
+        if constexpr (WIDE) return *reinterpret_cast<const uint2*>(counts + t);
+        return make_uint2(counts[t >> 1] & 0xffff, counts[t >> 1] >> 16);
+    }
+};
 constexpr int THREADS = 1024, PAIRS = 4;           // pairs of logits of a thread on their way
 
 struct Settings {
@@ -172,15 +191,15 @@ struct Row {
           bias_values(a.bias_values + r.bias) {}
 };
 
-__device__ inline uint32_t slot_of(uint32_t token) { return (token * 0x9e3779b1u) >> 22; }  // of 2^10
-
 // Bound by memory where rows are many, by the chain of a call where they are few.
+template <bool WIDE>
 __global__ __launch_bounds__(THREADS) void fx_choose_kernel(FxChoose a, Settings settings, const FxChoice* rows,
                                                             uint32_t chunk, Best* bests_of) {
-    extern __shared__ __attribute__((aligned(16))) uint32_t counts[];  // of two tokens each
+    using L = Lists<WIDE>;
+    extern __shared__ __attribute__((aligned(16))) uint32_t counts[];
     const uint32_t chunks = (a.vocab + chunk - 1) / chunk;
-    __shared__ uint32_t keys[SLOTS];
-    __shared__ unsigned long long biases[SLOTS];
+    __shared__ uint32_t keys[L::SLOTS];
+    __shared__ unsigned long long biases[L::SLOTS];
     __shared__ Best bests[THREADS / 64];
     __shared__ int64_t queued[THREADS / 64][128];     // logits
     __shared__ uint32_t queued_at[THREADS / 64][128];  // tokens of the chunk, and bit 31: allowed
@@ -205,27 +224,27 @@ __global__ __launch_bounds__(THREADS) void fx_choose_kernel(FxChoose a, Settings
     };
     load(0);  // on their way while the lists are counted
     if (listed) {
-        for (uint32_t i = threadIdx.x; i < (here + 7) / 8; i += THREADS)
+        for (uint32_t i = threadIdx.x; i < (WIDE ? (here + 3) / 4 : (here + 7) / 8); i += THREADS)
             reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
         if (r.bias_count)
-            for (uint32_t i = threadIdx.x; i < SLOTS; i += THREADS) keys[i] = ~0u, biases[i] = 0;
+            for (uint32_t i = threadIdx.x; i < L::SLOTS; i += THREADS) keys[i] = ~0u, biases[i] = 0;
         __syncthreads();
         for (uint32_t i = threadIdx.x * 4; i < r.history_count; i += THREADS * 4) {
             const v4i four = entries(row.history, i, r.history_count);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t t = static_cast<uint32_t>(four[k]) - base;
-                if (t < here) atomicAdd(&counts[t >> 1], 1u << (16 * (t & 1)));
+                if (t < here) atomicAdd(&counts[L::word(t)], 1u << L::shift(t));
             }
         }
         for (uint32_t i = threadIdx.x; i < r.bias_count; i += THREADS) {
             const uint32_t t = static_cast<uint32_t>(row.bias_tokens[i]) - base;
             if (t >= here) continue;
-            atomicOr(&counts[t >> 1], BIASED << (16 * (t & 1)));
-            // at most BIAS_MAX of the slots are taken: there is a free one, or the token's own
-            uint32_t slot = slot_of(t);
+            atomicOr(&counts[L::word(t)], L::BIASED << L::shift(t));
+            // at most FEW of the slots are taken: there is a free one, or the token's own
+            uint32_t slot = L::slot_of(t);
             for (uint32_t old = atomicCAS(&keys[slot], ~0u, t); old != ~0u && old != t; old = atomicCAS(&keys[slot], ~0u, t))
-                slot = (slot + 1) % SLOTS;
+                slot = (slot + 1) % L::SLOTS;
             atomicAdd(&biases[slot], static_cast<unsigned long long>(static_cast<int64_t>(row.bias_values[i])));
         }
         __syncthreads();
@@ -241,15 +260,15 @@ __global__ __launch_bounds__(THREADS) void fx_choose_kernel(FxChoose a, Settings
         if (lane < waiting) {
             const int64_t l = queue[lane];
             const uint32_t at = queue_at[lane], t = at & 0x7fffffff;
-            const uint32_t count = counts[t >> 1] >> (16 * (t & 1)) & 0xffff;
+            const uint32_t count = L::of(counts, t);
             int64_t bias = 0;
-            if (count & BIASED) {
-                uint32_t slot = slot_of(t);
-                while (keys[slot] != t) slot = (slot + 1) % SLOTS;
+            if (count & L::BIASED) {
+                uint32_t slot = L::slot_of(t);
+                while (keys[slot] != t) slot = (slot + 1) % L::SLOTS;
                 bias = static_cast<int64_t>(biases[slot]);
             }
             const bool allowed = at >> 31;
-            const int64_t changed = allowed ? rule(l, count & HISTORY_MAX, bias) : INT64_MIN;
+            const int64_t changed = allowed ? rule(l, count & L::MOST, bias) : INT64_MIN;
             if (allowed) take(&best, changed, static_cast<int>(base + t));
             if (row.adjusted) row.adjusted[base + t] = changed;
         }
@@ -280,13 +299,13 @@ __global__ __launch_bounds__(THREADS) void fx_choose_kernel(FxChoose a, Settings
         for (int i = 0; i < PAIRS; ++i) {
             const uint32_t t = from + (i * THREADS + threadIdx.x) * 2;
             const bool one = t < here, two = t + 2 <= here;
-            const uint32_t count = listed && one ? counts[t >> 1] : 0;
+            const uint2 count = listed && one ? L::two(counts, t) : make_uint2(0, 0);
             Pair p = pairs[i];
             if (listed) {
-                push(one && (count & 0xffff), t, p.v[0], bits[i] & 1);
-                push(two && (count >> 16), t + 1, p.v[1], bits[i] & 2);
+                push(one && count.x, t, p.v[0], bits[i] & 1);
+                push(two && count.y, t + 1, p.v[1], bits[i] & 2);
             }
-            const bool first = one && !(count & 0xffff), second = two && !(count >> 16);
+            const bool first = one && !count.x, second = two && !count.y;
             if (first) p.v[0] = masked(p.v[0], bits[i] & 1, base + t, &best);
             if (second) p.v[1] = masked(p.v[1], bits[i] & 2, base + t + 1, &best);
             if (!row.adjusted) continue;
@@ -360,31 +379,39 @@ __global__ __launch_bounds__(256) void fx_choose_dense_kernel(FxChoose a, Settin
     if (threadIdx.x == 0) a.tokens[first_row + blockIdx.x] = best.token;
 }
 
-// Rows of one launch: CALL_ROWS at most, as a grid holds less than 2^32 threads, and 2^24
-// tokens are 293 chunks.
-constexpr size_t CALL_ROWS = 4096;
+// Rows of one launch, at most; a grid holds less than 2^32 threads.
+constexpr size_t CALL_ROWS = 4096, CALL_GROUPS = size_t{1} << 21;
 
 int choose_rows(Context* c, const FxChoose& a, const FxChoice* rows, size_t count) {
-    bool listed = false, dense = false;
+    uint32_t history = 0, biases = 0;
     for (size_t i = 0; i < count; ++i) {
-        listed |= rows[i].history_count || rows[i].bias_count;
-        dense |= rows[i].history_count > HISTORY_MAX || rows[i].bias_count > BIAS_MAX;
+        history = std::max(history, rows[i].history_count);
+        biases = std::max(biases, rows[i].bias_count);
     }
+    // Long lists, us by the wide lists and by a count and a sum a token (the kernel below): one, 64
+    // and 256 rows of 50,257, 40,000 tokens of history 11.4, 27.8, 79 and 633, 713, 2,873; 600
+    // biases 11.1, 20.2, 53 and 84, 178, 505; 64 rows, 5,000 biases 50 and 268.
+    const bool wide = history > Lists<false>::MOST || biases > Lists<false>::BIASES;
+    const uint32_t longest =
+        !wide ? Lists<false>::CHUNK : biases <= Lists<true>::BIASES ? Lists<true>::CHUNK : Lists<true>::FEW;
     // Chunks of at least 1,024 tokens (many rows: a pass of all threads), for a workgroup a CU:
     // each counts all of its row's lists.  us with one, two (of half the threads), four and
     // eight a CU: 256 rows of 50,257 43.7, 49.0, 55.8, 68.7; 64 rows 20.9, 20.9, 25.0, 36.9.
     const size_t want = (c->cu_count + count - 1) / count;
-    const uint32_t least = (a.vocab + CHUNK - 1) / CHUNK, short_chunk = count < 32 ? 1024 : PAIRS * THREADS * 2,
+    const uint32_t least = (a.vocab + longest - 1) / longest, short_chunk = count < 32 ? 1024 : PAIRS * THREADS * 2,
                    most = (a.vocab + short_chunk - 1) / short_chunk;
     uint32_t groups = std::max(least, static_cast<uint32_t>(std::min<size_t>(want, most)));
-    const uint32_t chunk = ((a.vocab + groups - 1) / groups + 63) / 64 * 64;  // whole words of a mask
+    // whole words of a mask (of which CHUNK and FEW are multiples)
+    const uint32_t chunk = ((a.vocab + groups - 1) / groups + 63) / 64 * 64;
     groups = (a.vocab + chunk - 1) / chunk;
     // Candidates, and settings that are no arguments; where no space is to be had, a workgroup a row.
     Best* bests = nullptr;
     FxChoice* in_memory = nullptr;
-    if (!dense && (groups > 1 || count > FX_CHOICES)) {
+    bool dense = false;
+    if (groups > 1 || count > FX_CHOICES) {
         const size_t best_bytes = count * groups * sizeof(Best);
-        dense = !try_ws(c, WS_FIXED, workspace_step(best_bytes + count * sizeof(FxChoice), FX_SPACE_MAX));
+        dense = count * groups > CALL_GROUPS ||
+                !try_ws(c, WS_FIXED, workspace_step(best_bytes + count * sizeof(FxChoice), FX_SPACE_MAX));
         bests = ws<Best>(c, WS_FIXED);
         if (count > FX_CHOICES) in_memory = reinterpret_cast<FxChoice*>(ws<unsigned char>(c, WS_FIXED) + best_bytes);
     }
@@ -402,8 +429,9 @@ int choose_rows(Context* c, const FxChoose& a, const FxChoice* rows, size_t coun
     }
     if (dense) return 0;
     std::copy(rows, rows + std::min<size_t>(count, FX_CHOICES), s.row);
-    hipLaunchKernelGGL(fx_choose_kernel, dim3(static_cast<unsigned>(count * groups)), dim3(THREADS),
-                       listed ? (chunk + 7) / 8 * 16 : 0, c->stream, a, s, in_memory, chunk, bests);
+    const auto kernel = wide ? fx_choose_kernel<true> : fx_choose_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(count * groups)), dim3(THREADS),
+                       history || biases ? chunk * (wide ? 4 : 2) : 0, c->stream, a, s, in_memory, chunk, bests);
     VMX_HIP(c, hipGetLastError());
     if (groups > 1) {
         hipLaunchKernelGGL(fx_choose_join_kernel, dim3(static_cast<unsigned>(count)), dim3(64), 0, c->stream, bests, groups,
