@@ -577,6 +577,26 @@ def test_choose_rows_of_the_largest_chunks(backend, vocab):
     assert np.array_equal(got, tokens) and np.array_equal(out, adjusted)
 
 
+@pytest.mark.parametrize("vocab", [20479, 20480, 20481, 61440])
+@pytest.mark.parametrize("history,biases", [(33000, 100), (9000, 2048), (40000, 2100)])
+def test_choose_rows_of_the_largest_chunks_of_long_lists(backend, vocab, history, biases):
+    """The same with counts of 31 bits: chunks of up to 20,480 tokens, or of 2,816 where biases are many."""
+    g = gen(vocab + history)
+    n = 256
+    logits = g.integers(-(1 << 30), 1 << 30, (n, vocab))
+    plain = dict(history=[], biases=[], mask=None, frequency=0, presence=0, repetition=65536)
+    rows = [plain] * n
+    some = [1, 255]
+    for i, r in zip(some, choice_rows(g, 2, vocab)):
+        rows[i] = r
+        r["history"] = np.concatenate([np.full(history - 500, vocab - 1), g.integers(0, vocab, 500)])
+        r["biases"] = [(int(t), int(v)) for t, v in zip(g.permutation(vocab)[:biases], g.integers(-9999, 9999, biases))]
+    tokens, adjusted = logits.argmax(1), logits.copy()
+    tokens[some], adjusted[some] = want.choose(logits[some], [rows[i] for i in some], bias_shift=9)
+    got, out = run_choose(backend, logits, rows, bias_shift=9)
+    assert np.array_equal(got, tokens) and np.array_equal(out, adjusted)
+
+
 def test_choose_without_choices_is_the_largest(backend):
     g = gen(1)
     logits = g.integers(-99, 99, (70, 4000))
