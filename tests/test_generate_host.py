@@ -1,0 +1,76 @@
+"""What FixedDecoder.generate and share do on the host: a decoder without a GPU, whose steps and choices are written down."""
+import numpy as np
+import pytest
+from volta_mi355x import InvalidInput, forward
+
+SIZES = dict(layers=1, heads=2, kv_heads=1, dim=8, hidden=16, vocab=50, positions=24)
+
+
+class Buffer:
+    def __init__(self, values):
+        self.values = np.array(values)
+
+
+class Library:
+    """The calls of `generate` on a backend: the token chosen is one more than the last of the step."""
+
+    def __init__(self):
+        self.choices = []
+
+    def upload_device(self, values):
+        return Buffer(values)
+
+    def upload_into(self, buf, offset, values):
+        buf.values[offset:offset + len(values)] = values
+
+    def download_device(self, buf, *_):
+        return buf.values
+
+    def free_device(self, buf):
+        pass
+
+    def fixed_choose_device(self, logits, rows, vocab, choices, *, out, **lists):
+        self.choices.append((choices.copy(), {k: v.values.copy() if isinstance(v, Buffer) else v for k, v in lists.items()}))
+        out.values[0] = (logits.values[0] + 1) % vocab
+
+
+class Decoder(forward.FixedDecoder):
+    """Steps keep their tokens."""
+
+    def __init__(self, slots=2, rows=None, **kw):
+        self.config = c = forward.FixedConfig(**{**SIZES, **kw})
+        self.backend, self.slots, self.rows = Library(), slots, rows or slots * c.positions
+        self.lengths, self.prefix, self.steps = [0] * slots, None, []
+        self._history, self._next = Buffer(np.zeros(c.positions + 1, np.int32)), Buffer(np.zeros(1, np.int32))
+        self._allowed = Buffer(np.zeros((c.vocab + 31) // 32, np.uint32))
+
+    def step_device(self, prompts, slots):
+        prompts = [self._prompt(p) for p in prompts]
+        if not all(len(p) for p in prompts) or sum(map(len, prompts)) > self.rows:
+            raise InvalidInput("a step takes one non-empty prompt for each of its slots, within the decoder's rows")
+        for p, s in zip(prompts, slots):
+            self.steps.append((s, p.tolist()))
+            self.lengths[s] += len(p)
+        return Buffer([int(p[-1]) for p in prompts])
+
+
+@pytest.mark.parametrize("prompt", [[3, 1, 4], (3, 1, 4), np.array([3, 1, 4], np.uint8), iter([3, 1, 4]),
+                                    (t for t in (3, 1, 4)), dict.fromkeys([3, 1, 4]), map(int, "314")])
+def test_generate_takes_tokens_from_any_iterable(prompt):
+    model = Decoder()
+    assert model.generate(prompt, 3, slot=1) == [5, 6, 7]
+    assert model.steps == [(1, [3, 1, 4]), (1, [5]), (1, [6])]
+
+
+def test_generate_takes_a_set_and_a_range():
+    model = Decoder()
+    assert model.generate({7}, 1) == [8] and model.generate(range(2, 5), 2, slot=1) == [5, 6]
+
+
+@pytest.mark.parametrize("prompt", [5, None, "314", [1.5], iter([1.5]), iter([]), iter([50]), (t for t in (1, -1)),
+                                    iter([[1, 2]]), np.array([[1, 2]]), np.array(3)])
+def test_generate_refuses_what_gives_no_tokens(prompt):
+    model = Decoder()
+    with pytest.raises(InvalidInput):
+        model.generate(prompt, 3)
+    assert model.steps == [] and model.lengths == [0, 0]

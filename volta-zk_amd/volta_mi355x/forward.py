@@ -23,6 +23,7 @@ a window a token sees the last of its keys and the sequence's first ones.
 """
 from __future__ import annotations
 
+from collections.abc import Iterable
 from dataclasses import dataclass
 
 import numpy as np
@@ -345,6 +346,8 @@ class FixedDecoder:
         if any(not 0 <= t < c.vocab or not abs(v) < 2.0 ** (31 - bits) - 1 for t, v in bias.items()):
             raise InvalidInput("a bias is out of range")
         penalized = repetition != 1.0 or frequency or presence
+        if not isinstance(prompt, np.ndarray) and isinstance(prompt, Iterable):
+            prompt = list(prompt)  # of an iterator or a set too
         tokens = self._prompt(prompt)
         before = self.lengths[slot] + (self.prefix[1] if self.prefix is not None else 0)
         if before + len(tokens) + count > c.positions + 1:
