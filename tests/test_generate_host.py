@@ -74,3 +74,26 @@ def test_generate_refuses_what_gives_no_tokens(prompt):
     with pytest.raises(InvalidInput):
         model.generate(prompt, 3)
     assert model.steps == [] and model.lengths == [0, 0]
+
+
+@pytest.mark.parametrize("act,weight", [(10, 13), (10, 2), (3, 0), (13, 46), (14, 46), (15, 46), (15, 44)])
+def test_biases_at_every_binary_point_of_the_logits(act, weight):
+    """What reaches the operator is the bias at the logits' binary point, to half a step of 2^-13 or of a logit, or of
+    2^-15 where the operator's shift, at most 46, asks for more bits."""
+    model = Decoder(act_bits=act, weight_bits=weight, gain_bits=max(act, 12))
+    bias = {4: 2.5, 7: -3.3, 9: 100.0, 11: 1e-5}
+    model.generate([1], 2, bias=bias)
+    for _, lists in model.backend.choices:
+        assert 0 <= lists["bias_shift"] <= 46
+        got = dict(zip(lists["bias_tokens"].tolist(), lists["bias_values"].astype(object) << lists["bias_shift"]))
+        assert got.keys() == bias.keys()
+        for t, v in bias.items():
+            assert abs(got[t] / 2.0 ** (act + weight) - v) <= 2.0 ** (-1 - min(13, act + weight))
+
+
+@pytest.mark.parametrize("act,weight,most", [(10, 13, 1 << 18), (15, 46, 1 << 16)])
+def test_the_largest_biases(act, weight, most):
+    model = Decoder(act_bits=act, weight_bits=weight, gain_bits=max(act, 12))
+    model.generate([1], 1, bias={0: most - 2.0, 1: 2.0 - most})
+    with pytest.raises(InvalidInput):
+        model.generate([1], 1, bias={0: float(most)})

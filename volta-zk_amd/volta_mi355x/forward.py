@@ -340,8 +340,8 @@ class FixedDecoder:
             raise InvalidInput("a penalty is out of range")
         choice["repetition"], choice["mask"] = round(scale), -1
         choice["frequency"], choice["presence"] = self._fixed(frequency), self._fixed(presence)
-        # biases at 2^-13, or as finely as the logits are
-        bits = min(13, unit)
+        # biases at 2^-13, or as finely as the logits are; the operator shifts them by 46 at most
+        bits = max(min(13, unit), unit - 46)
         bias = bias or {}
         if any(not 0 <= t < c.vocab or not abs(v) < 2.0 ** (31 - bits) - 1 for t, v in bias.items()):
             raise InvalidInput("a bias is out of range")
