@@ -97,3 +97,13 @@ def test_the_largest_biases(act, weight, most):
     model.generate([1], 1, bias={0: most - 2.0, 1: 2.0 - most})
     with pytest.raises(InvalidInput):
         model.generate([1], 1, bias={0: float(most)})
+
+
+@pytest.mark.parametrize("token", [1.5, np.float32(2.25), "1", None, 50, -1, (1,), np.float64("nan"), 2 + 0j])
+def test_biases_of_what_is_no_token_are_refused(token):
+    """A fraction would turn into another token."""
+    model = Decoder()
+    with pytest.raises(InvalidInput):
+        model.generate([1], 1, bias={0: 1.0, token: 2.0})
+    assert model.steps == [] and model.generate([1], 1, bias={0: 1.0, np.int64(2): 2.0, np.uint8(3): 1, 4.0: 2}) == [2]
+    assert model.backend.choices[-1][1]["bias_tokens"].tolist() == [0, 2, 3, 4]

@@ -25,6 +25,7 @@ from __future__ import annotations
 
 from collections.abc import Iterable
 from dataclasses import dataclass
+from numbers import Real
 
 import numpy as np
 
@@ -343,7 +344,9 @@ class FixedDecoder:
         # biases at 2^-13, or as finely as the logits are; the operator shifts them by 46 at most
         bits = max(min(13, unit), unit - 46)
         bias = bias or {}
-        if any(not 0 <= t < c.vocab or not abs(v) < 2.0 ** (31 - bits) - 1 for t, v in bias.items()):
+        if any(not isinstance(t, Real) or not 0 <= t < c.vocab or t != int(t) for t in bias):
+            raise InvalidInput("a bias is for a token of the vocabulary")
+        if any(not abs(v) < 2.0 ** (31 - bits) - 1 for v in bias.values()):
             raise InvalidInput("a bias is out of range")
         penalized = repetition != 1.0 or frequency or presence
         if not isinstance(prompt, np.ndarray) and isinstance(prompt, Iterable):
