@@ -107,3 +107,32 @@ def test_biases_of_what_is_no_token_are_refused(token):
         model.generate([1], 1, bias={0: 1.0, token: 2.0})
     assert model.steps == [] and model.generate([1], 1, bias={0: 1.0, np.int64(2): 2.0, np.uint8(3): 1, 4.0: 2}) == [2]
     assert model.backend.choices[-1][1]["bias_tokens"].tolist() == [0, 2, 3, 4]
+
+
+@pytest.mark.parametrize("rows,pieces", [(None, [9]), (9, [9]), (8, [8, 1]), (4, [4, 4, 1]), (1, [1] * 9)])
+def test_a_prefix_longer_than_a_step_is_shared(rows, pieces):
+    model = Decoder(rows=rows)
+    model.share(range(10, 19), 1)
+    assert model.prefix == (1, 9) and model.lengths == [0, 9]
+    assert [len(p) for _, p in model.steps] == pieces and {s for s, _ in model.steps} == {1}
+    assert sum((p for _, p in model.steps), []) == list(range(10, 19))
+
+
+def test_a_prefix_that_cannot_be_shared_leaves_no_tokens():
+    for prompt, slot in (([], 0), ([1] * 25, 0), ([1, 50], 0), ([1], 2), ([1], -1), ([1] * 5 + [1.5], 0)):
+        model = Decoder(rows=2)
+        with pytest.raises(InvalidInput):
+            model.share(prompt, slot)
+        assert model.steps == [] and model.lengths == [0, 0] and model.prefix is None
+    model = Decoder(rows=2)
+    step = model.step_device
+
+    def fails_later(prompts, slots):
+        if model.steps:
+            raise RuntimeError
+        return step(prompts, slots)
+
+    model.step_device = fails_later
+    with pytest.raises(RuntimeError):
+        model.share([1, 2, 3], 0)
+    assert model.lengths == [0, 0] and model.prefix is None

@@ -172,3 +172,24 @@ def test_generate_refusals(decoder):
     assert model.generate([1], 0) == []
     assert len(model.generate([1], 120)) == 120 and model.lengths[0] == 120
 
+
+
+@pytest.mark.parametrize("rows", [1, 7, 69, 70])
+def test_a_prefix_longer_than_the_decoders_rows(backend, rows):
+    """Shared in steps of those: the same logits behind it as behind the tokens themselves."""
+    from volta_mi355x import forward
+    c = forward.FixedConfig(**BASE, rotary=16)
+    t = model_tensors(c, 4)
+    g = np.random.Generator(np.random.PCG64(rows))
+    start, seq = g.integers(0, c.vocab, 70), g.integers(0, c.vocab, 6)
+    dev = {name: backend.upload_device(v.reshape(-1)) for name, v in t.items()}
+    model = forward.FixedDecoder(backend, c, dev, slots=2, rows=rows)
+    try:
+        model.share(start, 0)
+        want_all = host_logits(c, t, np.concatenate([start, seq]))
+        for i, token in enumerate(seq):
+            assert np.array_equal(model.step([[token]], [1])[0], want_all[70 + i]), i
+    finally:
+        model.close()
+        for b in dev.values():
+            backend.free_device(b)

@@ -214,14 +214,24 @@ class FixedDecoder:
         self.lengths[slot] = 0
 
     def share(self, prompt, slot: int) -> None:
-        """Runs `prompt` in `slot` and makes its tokens the beginning of the sequences of all other slots, which are
-        empty.  They are kept once, and attention reads them once for all sequences of a step."""
+        """Runs `prompt` in `slot`, in steps of the decoder's rows, and makes its tokens the beginning of the sequences of
+        all other slots, which are empty.  They are kept once, and attention reads them once for all sequences of a step."""
         if self.config.window:
             raise InvalidInput("a window and a shared prefix do not go together")
         if self.prefix is not None or any(self.lengths):
             raise InvalidInput("a prefix is shared before any sequence begins")
-        self.step_device([prompt], [slot])
-        self.prefix = (slot, self.lengths[slot])
+        tokens = self._prompt(prompt)
+        if not 0 <= slot < self.slots:
+            raise InvalidInput("slot is outside the decoder's")
+        if not 0 < len(tokens) <= self.config.positions:
+            raise InvalidInput("a prefix holds one token to the model's positions")
+        try:
+            for at in range(0, len(tokens), self.rows):
+                self.step_device([tokens[at:at + self.rows]], [slot])
+        except Exception:
+            self.lengths[slot] = 0
+            raise
+        self.prefix = (slot, len(tokens))
 
     def unshare(self) -> None:
         """Forgets the shared prefix and all sequences."""
