@@ -1,5 +1,6 @@
 // host_check.cpp -- host build of the device arithmetic headers, exported so
-// CPU tests can check every compile-time shift form against big integers.
+// CPU tests can check every compile-time shift form against big integers, and the
+// rules that choose kernels.
 // Not part of the product library.
 #include <stdint.h>
 
@@ -10,6 +11,7 @@
 
 #include "enc13_mfma.hpp"
 #include "enc13_phase_b.hpp"
+#include "fixed_rules.hpp"
 #include "gl64.hpp"
 #include "gl64_shift.hpp"
 #include "ntt_rr.hpp"
@@ -380,4 +382,17 @@ extern "C" __attribute__((visibility("default"))) int glc_ntt_rr_msg(const uint6
                                                                      uint64_t* out) {
     return bits == 13 ? rr_msg_dispatch<3>(fwd, w, pads, cols, pad, rows, blocks, out)
                       : rr_msg_dispatch<4>(fwd, w, pads, cols, pad, rows, blocks, out);
+}
+
+// Rows up to which sequences behind a prefix read it together (fixed_rules.hpp).
+extern "C" __attribute__((visibility("default"))) size_t glc_prefix_limit(size_t dim, size_t kv_heads, size_t heads,
+                                                                         size_t prefix, const uint32_t* counts,
+                                                                         const uint32_t* lengths, size_t sequences) {
+    std::vector<vmx::FxSeq> seqs;
+    for (size_t i = 0; i < sequences; ++i)
+        if (counts[i]) seqs.push_back(vmx::FxSeq{0, 0, counts[i], lengths[i]});
+    vmx::FxAttention t{};
+    t.heads = static_cast<uint32_t>(heads);
+    t.prefix = static_cast<uint32_t>(prefix);
+    return vmx::fx::prefix_limit(vmx::FxCache{nullptr, 1, kv_heads, dim, 1}, t, seqs.data(), seqs.data() + seqs.size());
 }
