@@ -368,3 +368,26 @@ def test_one_call_after_another_in_the_same_space(backend):
     for i in range(3):
         for j in (0, 1):
             assert all(np.array_equal(x, y) for x, y in zip(got[3 * j], got[3 * j + i]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,heads,refused", [(1 << 24, 257, True), (1 << 24, 128, True), (32769, 65535, True),
+                                                 (32767, 65535, False), (1 << 24, 127, False)])
+def test_rows_that_32_bits_do_not_hold_are_refused(backend, count, heads, refused):
+    """Tokens x heads of a sequence from 2^31 - 127 on, 8 GB of queries of one place: before anything else of the call is
+    looked at.  (One row less is refused here for its buffers, which hold none of it.)"""
+    from volta_mi355x import accel
+    b = backend
+    cache = b.fixed_kv_cache(2, 1, 1, 64)
+    x, exp = b.upload_device(np.zeros(64, np.int16)), b.upload_device(exponentials())
+    try:
+        a = accel._FixedAttention(x.id, 0, heads, exp.id, 0, 8192, x.id, 0, heads, heads, 12, 0)
+        s = np.array([[0, 0, count, 5]], np.int64)
+        for call in (lambda: b.lib.volta_mi355x_fixed_attention_device(b.raw, cache._args(), a, s.ctypes.data, 1),
+                     lambda: b.lib.volta_mi355x_fixed_prefix_attention_device(b.raw, cache._args(), a, 1, 5, s.ctypes.data, 1)):
+            assert call() != 0
+            assert ("32 bits" in b.last_error()) == refused, b.last_error()
+    finally:
+        b.free_fixed_kv_cache(cache)
+        b.free_device(x)
+        b.free_device(exp)

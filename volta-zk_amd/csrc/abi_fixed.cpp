@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstdint>
 #include <exception>
 #include <string>
 #include <vector>
@@ -240,6 +241,9 @@ int attention(Context* c, const VoltaFixedCache* cache, const VoltaFixedAttentio
         for (const FxSeq& s : seqs) {
             if (seen.prefix && s.slot == seen.prefix_slot) return fail_msg(c, "a sequence is in the prefix's slot");
             if (seen.prefix + s.length > FX_CACHE_MAX) return fail_msg(c, "prefix and sequence are longer than 65,536 tokens");
+            // a launch's 32-bit rows: tokens x query heads of a key head, in blocks of 128
+            if (s.count * (a->heads / kv.kv_heads) > INT32_MAX - 127)
+                return fail_msg(c, "a sequence has more rows than 32 bits hold");
         }
         if (!rows) return empty_op(c, OP_GEMM);
         const size_t cols = a->heads * kv.dim;
