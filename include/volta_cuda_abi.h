@@ -477,7 +477,8 @@ int volta_mi355x_fixed_kv_append_device(void* ctx, const VoltaFixedCache* cache,
  * zeros where it sees none or all e are 0.  table: 1 .. 8,192 u16, at most
  * 2^14 each (larger entries count as 2^14); 8 <= shift <= 24.  Rows are heads x
  * dim; the output may not overlap the queries, and rows of two sequences may
- * not overlap.  Only without `causal` may count exceed length. */
+ * not overlap.  Only without `causal` may count exceed length; count x heads /
+ * kv_heads is at most 2^31 - 128. */
 typedef struct VoltaFixedAttention {
     uint64_t q_id;
     size_t q_off, q_stride;

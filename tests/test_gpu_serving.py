@@ -161,7 +161,8 @@ def test_prefix_of_tokens_of_many_sequences(backend, dim, heads, kv_heads, batch
     check_prefix(backend, batch + prefix, [new] * batch, lengths, prefix, heads, kv_heads, dim)
 
 
-# Few rows of many sequences behind a long prefix read it together: 33 tiles and 124 units of 16 rows.
+# Few rows of many sequences behind a prefix of 33 tiles, 124 units of 16 rows: near the bounds of the rule that has them
+# read it together or not.  test_serving_paths.py holds cases to each of its outcomes.
 TOGETHER = dict(counts=[1] * 31, prefix=2100, kv_heads=4)
 
 

@@ -299,7 +299,7 @@ struct FxChoice {
     uint32_t repetition;  // at 2^-16
     uint32_t reserved;
 };
-constexpr int FX_CHOICES = 64;  // rows a launch: their settings are a kernel's arguments
+constexpr int FX_CHOICES = 64;  // rows whose settings are a launch's arguments; those of the others are in the workspace
 
 struct FxChoose {
     const int64_t* logits;

@@ -14,11 +14,12 @@
 // its logits once.  Few tokens are in a list, but nearly every 64 hold one: a wave queues
 // those with their logits and changes 64 at a time, all lanes at work.  (In place, all waves
 // went through the arithmetic; in a second pass over the lists their logits came from memory
-// again.  256 rows of 50,257, 6,100 tokens of history each: 50 and 48 us, 35 by the queue,
-// 110 MB at 3.1 TB/s.)  The sum of a token's biases is in a hash table in LDS, which a bit
-// beside the count says to look into.  A second launch joins the chunks' best.  Where no
-// workspace may grow, a workgroup takes a row, with a count and a sum for each token of a
-// small chunk at a time.
+// again.  256 rows of 50,257, 6,100 tokens of history each, the same in each launch: 50 and 48
+// us, 35 by the queue, 110 MB at 3.1 TB/s.  The call takes 42 to 43 us on the same logits, which
+// the last-level cache holds, and 48 to 49 on others.)  The sum of a token's biases is in a hash
+// table in LDS, which a bit beside the count says to look into.  A second launch joins the
+// chunks' best.  Where no workspace may grow, a workgroup takes a row, with a count and a sum for
+// each token of a small chunk at a time.
 #include <algorithm>
 #include <climits>
 
@@ -388,9 +389,10 @@ int choose_rows(Context* c, const FxChoose& a, const FxChoice* rows, size_t coun
         history = std::max(history, rows[i].history_count);
         biases = std::max(biases, rows[i].bias_count);
     }
-    // Long lists, us by the wide lists and by a count and a sum a token (the kernel below): one, 64
-    // and 256 rows of 50,257, 40,000 tokens of history 11.4, 27.8, 79 and 633, 713, 2,873; 600
-    // biases 11.1, 20.2, 53 and 84, 178, 505; 64 rows, 5,000 biases 50 and 268.
+    // Long lists, us by the wide lists and by a count and a sum a token (fx_choose_dense_kernel): one,
+    // 64 and 256 rows of 50,257, 40,000 tokens of history 12, 25, 76 and 633, 713, 2,873; 600 biases
+    // 11, 20, 51 and 84, 178, 505; 64 rows, 5,000 biases 46 and 268.  Counts of 31 bits need three
+    // chunks a row, and each reads the row's lists: without them the 256 rows take 31.
     const bool wide = history > Lists<false>::MOST || biases > Lists<false>::BIASES;
     const uint32_t longest =
         !wide ? Lists<false>::CHUNK : biases <= Lists<true>::BIASES ? Lists<true>::CHUNK : Lists<true>::FEW;

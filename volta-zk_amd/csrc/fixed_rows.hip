@@ -239,8 +239,9 @@ __global__ __launch_bounds__(256) void fx_embed_kernel(FxEmbed a, uint32_t piece
 // places of a pair are in one lane, in one register.
 //
 // With gains, bound by vector instructions (f64: 0.70 of their issue) beside memory: 16,384 rows
-// of 24 heads of 64 28.5 us, 101 MB at 3.5 TB/s.  Without them by memory: 4,095 rows of 40 heads
-// of 128, 96 places of each turned, 16 us, 84 MB at 5.2 TB/s.
+// of 24 heads of 64 28.5 to 32.5 us where the last-level cache still holds a part of the rows, 36
+// where it does not (101 MB at 3.5 to 2.8 TB/s).  Without them by memory: 4,095 rows of 40 heads
+// of 128, 96 places of each turned, 16.5 and 21 us, 84 MB at 5.1 and 4.0 TB/s.
 //
 // KEPT heads a lane, in turn: the root and the reciprocal cost as much as eight places'
 // quotients, and lane k of a head's lanes computes those of the k-th head for all.
@@ -393,8 +394,8 @@ void launch_rotate(Context* c, const FxRotate& a) {
     auto launch = [&](auto kernel, uint32_t each) {
         hipLaunchKernelGGL(kernel, dim3((items + each - 1) / each), dim3(256), 0, c->stream, a, items);
     };
-    // Two heads a lane where they have norms and are many.  16,384 rows of 24 heads of 64, us with
-    // one, two and four: 30.5, 28.5, 32.1.
+    // Two heads a lane where they have norms and are many.  16,384 rows of 24 heads of 64, the same
+    // each time, us with one, two and four: 30.5, 28.5, 32.1.
     if ((a.q_gain || a.k_gain) && items >= 512u / LANES * 4 * static_cast<uint32_t>(c->cu_count))
         launch(fx_rotate_kernel<LANES, 2>, 512 / LANES);
     else

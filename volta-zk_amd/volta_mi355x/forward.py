@@ -40,7 +40,8 @@ class FixedConfig:
 
     Positions are learned (wpe) or, with `rotary`, turn the first `rotary` places of each query and key, in pairs of
     places half of them apart or adjacent.  `head_norm` gives queries and keys an RMS norm of each head before that.
-    `window` (0: none) bounds what a token sees to the last keys, its own among them, and the sequence's first `sinks`."""
+    `window` (0: none) bounds what a token sees to the last keys, its own among them, and the sequence's first `sinks`;
+    a slot keeps `positions` tokens all the same."""
     layers: int
     heads: int
     kv_heads: int
@@ -333,11 +334,14 @@ class FixedDecoder:
 
     def generate(self, prompt, count: int, slot: int = 0, *, repetition: float = 1.0, frequency: float = 0.0,
                  presence: float = 0.0, bias: dict[int, float] | None = None, allowed=None) -> list[int]:
-        """The `count` tokens of the largest logits (the lowest index of equal ones) after the prompt.
+        """The `count` tokens of the largest logits (the lowest index of equal ones) after the prompt, any iterable of
+        tokens.
 
         The logit of a token that the prompt and the answer hold n > 0 times is divided by `repetition` (multiplied, if
-        negative) and lowered by frequency n + presence.  `bias` is added to its tokens' logits.  `allowed`: a truth value
-        for each token, or a function that gives them for the answer so far; where it allows nothing, the answer ends."""
+        negative) and lowered by frequency n + presence: all three count the prompt's tokens, and none counts those that
+        the slot held before or a shared prefix.  `bias` is added to its tokens' logits, to the nearest 2^-13 (or step of
+        the logits, if that is coarser).  `allowed`: a truth value for each token, or a function that gives them for the
+        answer so far; where it allows nothing, the answer ends."""
         c, b = self.config, self.backend
         if count <= 0:
             return []
